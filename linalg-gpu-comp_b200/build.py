@@ -68,7 +68,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     return OUT
 
 
-ENTRY_SRC = PKG / "qr_b200" / "_entry.cpp"
+ENTRY_SRC = sorted((PKG / "qr_b200").glob("_entry*.cpp"))
 
 
 def _entry_out() -> Path:
@@ -77,7 +77,7 @@ def _entry_out() -> Path:
 
 
 def build_entry(force: bool = False, verbose: bool = False) -> Path:
-    """Compile qr_b200/_entry.cpp (the torch-facing call path, pybind11) against the
+    """Compile qr_b200/_entry*.cpp (the torch-facing call path, pybind11) against the
     in-tree libqrb200.so, with rpath $ORIGIN so the pair travels together."""
     import sysconfig
 
@@ -85,24 +85,35 @@ def build_entry(force: bool = False, verbose: bool = False) -> Path:
     import torch.utils.cpp_extension as ce
 
     out = _entry_out()
-    deps = [ENTRY_SRC, OUT, INCLUDE / "qrb200.h", Path(__file__)]
+    deps = [*ENTRY_SRC, PKG / "qr_b200" / "_entry.h", OUT, *INCLUDE.glob("*.h"), Path(__file__)]
     if not force and out.exists() and all(d.stat().st_mtime <= out.stat().st_mtime for d in deps):
         return out
     cxx = shutil.which("g++") or "c++"
     inc = [f"-I{p}" for p in ce.include_paths()] + [f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}",
                                                    "-I/usr/local/cuda/include"]
     libdirs = ce.library_paths()
-    cmd = [cxx, "-O2", "-shared", "-fPIC", "-std=c++17", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-DTORCH_EXTENSION_NAME=_entry", "-DTORCH_API_INCLUDE_EXTENSION_H", *inc, str(ENTRY_SRC),
-           "-o", str(out.with_suffix(".tmp")), *[f"-L{d}" for d in libdirs], f"-L{OUT.parent}",
-           "-lqrb200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python",
-           "-Wl,-rpath,$ORIGIN", *[f"-Wl,-rpath,{d}" for d in libdirs]]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"g++ failed on {ENTRY_SRC.name}:\n{r.stdout}\n{r.stderr}")
+    OBJ.mkdir(exist_ok=True)
+    flags = ["-O2", "-fPIC", "-std=c++17", "-fvisibility=hidden",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             "-DTORCH_EXTENSION_NAME=_entry", "-DTORCH_API_INCLUDE_EXTENSION_H", *inc]
+
+    def run(cmd: list[str], what: str) -> None:
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"g++ failed on {what}:\n{r.stdout}\n{r.stderr}")
+
+    def compile_one(src: Path) -> str:
+        obj = OBJ / (src.stem + ".o")
+        run([cxx, *flags, "-c", str(src), "-o", str(obj)], src.name)
+        return str(obj)
+
+    with cf.ThreadPoolExecutor(max_workers=min(len(ENTRY_SRC), os.cpu_count() or 4)) as ex:
+        objs = list(ex.map(compile_one, ENTRY_SRC))
+    run([cxx, "-shared", *objs, "-o", str(out.with_suffix(".tmp")), *[f"-L{d}" for d in libdirs], f"-L{OUT.parent}",
+         "-lqrb200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+         "-Wl,-rpath,$ORIGIN", *[f"-Wl,-rpath,{d}" for d in libdirs]], out.name)
     os.replace(out.with_suffix(".tmp"), out)
     return out
 

@@ -1,0 +1,218 @@
+// Gradients of q, k, g and beta of the gated delta rule, chunk by chunk (mathematics in
+// qrb_delta.cuh).
+//
+// With every chunk's S0, e, dS' and du in the workspace the chunks are independent: one block
+// per (chunk, q/k head) adds the heads that share it in order, so no atomics are needed and
+// results repeat.  Value columns pass through in tiles of 32 by cp.async; 16 warps hold, as
+// 16 x 32 pieces, the products with S0 and dS' (kept apart: their rows scale differently) and
+// 16 x 16 pieces of dO e^T and du e^T, which then meet K and Q.  beta is applied to rows and
+// columns of products, so that e and du serve as they are.  The sums dg and dbeta are made of come
+// from the recurrences; here they are added up in order.
+#include "qrb_delta.cuh"
+
+namespace qrb {
+namespace delta {
+namespace {
+
+template <int DKP, typename T>
+struct GLayout {
+  static constexpr int P = Pieces<T>::kIn, PS = Pieces<T>::kS;
+  static constexpr int kStages = PS == 2 ? 2 : 1;
+  static constexpr int kK = tile_bytes(kChunk, P, DKP);
+  static constexpr int kS = tile_bytes(DKP, PS, kTile);
+  static constexpr int kF = tile_bytes(kChunk, PS, kTile);
+  static constexpr int kD = tile_bytes(kChunk, P, kTile);
+  // tiles in the workspace have kBackPieces pieces; the first kS of them are a prefix
+  static constexpr int kWS = tile_bytes(DKP, kBackPieces, kTile), kWF = tile_bytes(kChunk, kBackPieces, kTile);
+  static constexpr int kOffE = 0, kOffDU = kF, kOffS0 = 2 * kF, kOffDS = kOffS0 + kS;
+  static constexpr int kStage = kOffDS + kS;
+  static constexpr int kZ = tile_bytes(kChunk, PS, kChunk);
+  static constexpr int kOffQ = kK, kOffD = 2 * kK, kOffT = kOffD + kD;
+  // Z and N are formed when the last tile is consumed and lie over the tiles
+  static constexpr int kTiles = kStages * kStage > 2 * kZ ? kStages * kStage : 2 * kZ;
+  static constexpr int kOffG = kOffT + kTiles;     // G (64 doubles), gates, row sums, reductions
+  static constexpr int kBytes = kOffG + 64 * 8 + 3 * 64 * 4;
+};
+
+template <int DKP, typename T>
+__global__ void __launch_bounds__(512) grad_kernel(Params p) {
+  using L = GLayout<DKP, T>;
+  constexpr int P = L::P, PS = L::PS;
+  constexpr int NT = DKP / 32;           // 8-column blocks of q / k columns a warp holds
+  extern __shared__ __align__(128) unsigned char sm[];
+  unsigned char *K = sm, *Q = sm + L::kOffQ, *D = sm + L::kOffD, *TT = sm + L::kOffT;
+  unsigned char *Z = TT, *N = TT + L::kZ;
+  double* G = reinterpret_cast<double*>(sm + L::kOffG);
+  float* gates = reinterpret_cast<float*>(G + 64);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, tq = lane & 3;
+  const int c = blockIdx.x, hk = blockIdx.y;
+  const int m0 = 16 * (warp & 3), cq = warp >> 2, d0 = cq * (DKP / 4);
+  const Chunk ch = chunk_at(p, c);
+  if (ch.seq < 0) return;
+  {
+    const size_t at = ((size_t)c * p.hk + hk) * L::kK;
+    cp_tile(K, p.kt + at, L::kK);
+    cp_tile(Q, p.qt + at, L::kK);
+    cp_commit();
+  }
+  float tq_[NT][4], tk_[NT][4];          // sums over the heads of the group
+  zero(tq_);
+  zero(tk_);
+  const int er = tid >> 3, ec = (tid & 7) * 4;   // elementwise work on 64 x 32 tiles: row, first column
+  for (int hh = 0; hh < p.group; ++hh) {
+    const int h = hk * p.group + hh;
+    const size_t at = slot_head(p, c, h);
+    auto load = [&](int n, int stage) {
+      unsigned char* d = TT + stage * L::kStage;
+      const size_t t = at * p.nv + n;
+      cp_tile(d + L::kOffE, p.ep + t * L::kWF, L::kF);
+      cp_tile(d + L::kOffDU, p.dup + t * L::kWF, L::kF);
+      cp_tile(d + L::kOffS0, p.s0p + t * L::kWS, L::kS);
+      cp_tile(d + L::kOffDS, p.dsp + t * L::kWS, L::kS);
+      cp_commit();
+    };
+    __syncthreads();                     // the previous head's Z, N and sums are consumed
+    if (tid < 64) G[tid] = p.gsum[at * 64 + tid];
+    if (tid < 192) gates[tid] = p.gates[at * 192 + tid];
+    float aq[NT][4], ay[NT][4], au[NT][4], az[2][4], an[2][4];
+    zero(aq);
+    zero(ay);
+    zero(au);
+    zero(az);
+    zero(an);
+    if (L::kStages == 2) load(0, 0);
+    for (int n = 0; n < p.nv; ++n) {
+      const int stage = L::kStages == 2 ? (n & 1) : 0;
+      unsigned char* d = TT + stage * L::kStage;
+      const unsigned char *E = d + L::kOffE, *DU = d + L::kOffDU, *S0 = d + L::kOffS0, *DS = d + L::kOffDS;
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int col = n * kTile + ec + i;
+        const bool in = er < ch.len && col < p.dv;
+        x[i] = in ? to_f(static_cast<const T*>(p.d_o)[ch.b * p.dos.b + (ch.t0 + er) * p.dos.t + h * p.dos.h + col]) : 0.f;
+      }
+      if (L::kStages == 2) {
+        cp_wait_all();
+        __syncthreads();
+        if (n + 1 < p.nv) load(n + 1, stage ^ 1);
+      } else {
+        __syncthreads();
+        load(n, 0);
+        cp_wait_all();
+      }
+      put2<P>(D, kChunk, kTile, er, ec, x[0], x[1]);
+      put2<P>(D, kChunk, kTile, er, ec + 2, x[2], x[3]);
+      __syncthreads();
+      mma_tile<NT, false, false, P, PS, PS>(aq, D, kChunk, kTile, m0, S0, DKP, kTile, d0, 0, kTile);
+      mma_tile<NT, false, false, PS, PS, PS>(ay, DU, kChunk, kTile, m0, S0, DKP, kTile, d0, 0, kTile);
+      mma_tile<NT, false, false, PS, PS, PS>(au, E, kChunk, kTile, m0, DS, DKP, kTile, d0, 0, kTile);
+      if (16 * cq <= m0) {               // Z, N are lower triangular
+        mma_tile<2, false, false, P, PS, PS>(az, D, kChunk, kTile, m0, E, kChunk, kTile, 16 * cq, 0, kTile);
+        mma_tile<2, false, false, PS, PS, PS>(an, DU, kChunk, kTile, m0, E, kChunk, kTile, 16 * cq, 0, kTile);
+      }
+    }
+    __syncthreads();                     // tiles consumed: Z and N may overwrite them
+    const float* gam = gates;
+    const float* tail = gates + 64;
+    const float* bet = gates + 128;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int i = m0 + gr + 8 * r, l = 16 * cq + 8 * j + 2 * tq;
+        float z[2], w[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float dc = l + e <= i ? expf((float)(G[i] - G[l + e])) * bet[l + e] : 0.f;
+          z[e] = l + e <= i ? p.scale * dc * az[j][2 * r + e] : 0.f;
+          w[e] = l + e < i ? -dc * bet[i] * an[j][2 * r + e] : 0.f;
+        }
+        put2<PS>(Z, kChunk, kChunk, i, l, z[0], z[1]);
+        put2<PS>(N, kChunk, kChunk, i, l, w[0], w[1]);
+      }
+    // row scalings
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = m0 + gr + 8 * (r >> 1);
+        aq[j][r] *= p.scale * gam[i];
+        ay[j][r] = tail[i] * bet[i] * au[j][r] - gam[i] * bet[i] * ay[j][r];
+      }
+    __syncthreads();
+    mma_tile<NT, false, true, PS, P, PS>(aq, Z, kChunk, kChunk, m0, K, kChunk, DKP, d0, 0, m0 + 16);
+    mma_tile<NT, true, true, PS, P, PS>(ay, Z, kChunk, kChunk, m0, Q, kChunk, DKP, d0, m0, kChunk);
+    mma_tile<NT, false, true, PS, P, PS>(ay, N, kChunk, kChunk, m0, K, kChunk, DKP, d0, 0, m0 + 16);
+    mma_tile<NT, true, true, PS, P, PS>(ay, N, kChunk, kChunk, m0, K, kChunk, DKP, d0, m0, kChunk);
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        tq_[j][r] += aq[j][r];
+        tk_[j][r] += ay[j][r];
+      }
+    if (warp == 0) {                     // dbeta, dg: two tokens a lane
+      float x[2] = {0.f, 0.f}, db[2] = {0.f, 0.f}, sds = 0.f;
+      for (int n = 0; n < 2 * p.nv; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const size_t i = (at * p.nv * 2 + n) * kChunk + 2 * lane + e;
+          x[e] += p.odo[i] - p.vdv[i];
+          db[e] += p.edu[i];
+        }
+      for (int i = lane; i < 8 * p.nv; i += 32) sds += p.sds[at * p.nv * 8 + i];
+      sds = warp_sum(sds);
+      float s = x[0] + x[1];             // suffix sums
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const float y = __shfl_down_sync(0xffffffffu, s, o);
+        if (lane + o < 32) s += y;
+      }
+      const int64_t to = (ch.b * p.time + ch.t0 + 2 * lane) * p.hv + h;
+      if (2 * lane < ch.len) {
+        p.dg[to] = s + sds;
+        p.dbeta[to] = db[0];
+      }
+      if (2 * lane + 1 < ch.len) {
+        p.dg[to + p.hv] = s - x[0] + sds;
+        p.dbeta[to + p.hv] = db[1];
+      }
+    }
+  }
+  const int64_t tok = ch.b * p.time + ch.t0;
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = m0 + gr + 8 * (r >> 1), col = d0 + 8 * j + 2 * tq + (r & 1);
+      if (i < ch.len && col < p.dk) {
+        const size_t at = ((size_t)(tok + i) * p.hk + hk) * p.dk + col;
+        static_cast<T*>(p.dq)[at] = from_f<T>(tq_[j][r]);
+        static_cast<T*>(p.dk_)[at] = from_f<T>(tk_[j][r]);
+      }
+    }
+}
+
+template <int DKP, typename T>
+cudaError_t run_grad(const Params& p, cudaStream_t s) {
+  constexpr int smem = GLayout<DKP, T>::kBytes;
+  static_assert(smem <= 232448, "shared memory of one block");
+  const double rows = (double)p.bound * kChunk * p.hv;
+  LaunchTimer t("delta_grad_kernel", s, rows * 4.0 * p.dk * sizeof(T), rows * (6.0 * p.dv + 8.0 * kChunk) * p.dk);
+  cudaError_t e = allow_smem(grad_kernel<DKP, T>, smem);
+  if (e != cudaSuccess) return e;
+  grad_kernel<DKP, T><<<dim3((unsigned)p.bound, (unsigned)p.hk), 512, smem, s>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_grad(const Params& p, int dtype, cudaStream_t s) {
+  if (dtype == 1) return p.dk <= 64 ? run_grad<64, __nv_bfloat16>(p, s) : run_grad<128, __nv_bfloat16>(p, s);
+  if (dtype == 2) return p.dk <= 64 ? run_grad<64, __half>(p, s) : run_grad<128, __half>(p, s);
+  return p.dk <= 64 ? run_grad<64, float>(p, s) : run_grad<128, float>(p, s);
+}
+
+}  // namespace delta
+}  // namespace qrb

@@ -7,6 +7,11 @@ Public API mirrors the reference's submission interface:
 * ``qr(A) -> (H, tau, Q)``              (both, one library call)
 * ``geqrf`` / ``orgqr``                 (aliases with explicit names)
 
+Sequence operators that share QR's compact-WY products:
+
+* ``gated_delta_rule(q, k, v, g, beta) -> (o, final_state)``, ``gated_delta_rule_backward`` and
+  ``gated_delta_step`` (one token per row)
+
 The ops (and with them ``libqrb200.so``) load on first attribute access, so that
 ``qr_b200.inputs`` -- the seeded input generators -- can be imported by code that
 must not map the library (the CPU reference arm of ``bench.py``).
@@ -16,14 +21,17 @@ from __future__ import annotations
 import importlib
 
 _OPS = ("custom_kernel", "form_q", "geqrf", "orgqr", "qr", "qr_host")
+_DELTA = ("gated_delta_rule", "gated_delta_rule_backward", "gated_delta_step")
 _LIB = ("QRBError", "lib")
 
-__all__ = [*_OPS, *_LIB]
+__all__ = [*_OPS, *_DELTA, *_LIB]
 
 
 def __getattr__(name: str):
     if name in _OPS:
         return getattr(importlib.import_module(".ops", __name__), name)
+    if name in _DELTA:
+        return getattr(importlib.import_module(".delta", __name__), name)
     if name in _LIB:
         return getattr(importlib.import_module("._lib", __name__), name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

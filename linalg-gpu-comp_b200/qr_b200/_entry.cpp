@@ -8,21 +8,11 @@
 // Inputs arrive already checked and contiguous (ops._check_batch), so the errors a user
 // sees keep their Python types; a failing library status raises RuntimeError with the
 // library's message, like _lib.check.
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/extension.h>
-
-#include "qrb200.h"
+#include "_entry.h"
 
 namespace {
 
-void check_status(int status) {
-  if (status != QRB_OK) {
-    char buf[512];
-    qrb_last_error(buf, sizeof buf);
-    TORCH_CHECK(false, "libqrb200 error ", status, ": ", buf);
-  }
-}
+using qrb_entry::check_status;
 
 struct Call {
   int64_t batch;
@@ -65,4 +55,5 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> qr(const at::Tensor& A) {
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("geqrf", &geqrf, "(H, tau) = geqrf(A) for a checked, contiguous (batch, n, n) float32 CUDA tensor");
   m.def("qr", &qr, "(H, tau, Q) for a checked, contiguous (batch, n, n) float32 CUDA tensor");
+  qrb_entry::bind_delta(m);
 }

@@ -39,6 +39,15 @@ SIGNATURES = {
     "qrb_qr_f32_host": (ctypes.c_int, [_fp, _fp, _fp, _fp, _c_int64, ctypes.c_int, _vp, _c_size, _vp]),
 }
 
+# The entry points of include/qrb200_nn.h (called through the compiled call path, qr_b200/_entry_*.cpp);
+# argument structs are passed by address.
+SIGNATURES.update({
+    "qrb_delta_workspace_size": (_c_size, [_vp, ctypes.c_int]),
+    "qrb_delta_forward": (ctypes.c_int, [_vp, _vp, _c_size, _vp]),
+    "qrb_delta_backward": (ctypes.c_int, [_vp, _vp, _c_size, _vp]),
+    "qrb_delta_step": (ctypes.c_int, [_vp, _vp]),
+})
+
 _lock = threading.Lock()
 _lib = None
 
