@@ -91,6 +91,51 @@ typedef struct {
 } qrb_delta_step_args;
 QRB_API int qrb_delta_step(const qrb_delta_step_args* a, void* stream);
 
+/* The linear layer y = act(x w^T + bias) + residual: x (m x k), w (n x k), y (m x n), row-major with
+ * row strides ldx, ldw, ... in elements, all of one dtype; fp32 accumulation, rounded once.  bias (n),
+ * residual and pre (m x n) may be NULL; pre receives x w^T + bias, rounded, for the backward pass.
+ * fp32 products carry fp32 accuracy (three bf16 planes per operand).  Results repeat.  y may be
+ * residual (same rows); it must not alias x, w or bias.  The workspace size depends on the pointers'
+ * alignment as well as on the sizes. */
+typedef struct {
+  int dtype, activation;           /* qrb_dtype, qrb_activation (GELU: the exact, erf form) */
+  int64_t m, k, n;
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw;
+  const void* bias;
+  const void* residual;
+  int64_t ldr;
+  void* y;
+  int64_t ldy;
+  void* pre;
+  int64_t ldpre;
+} qrb_linear_args;
+QRB_API size_t qrb_linear_workspace_size(const qrb_linear_args* a);
+QRB_API int qrb_linear_forward(const qrb_linear_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its backward pass: dp = dy act'(pre), dx = dp w, dw = dp^T x, dbias = column sums of dp (the
+ * residual's gradient is dy).  pre is what the forward call stored (not read without an activation);
+ * dx (m x k), dw (n x k) and dbias (n) are dense and each may be NULL; x is read for dw, w for dx.  dp
+ * of the 16-bit types is rounded to the type once before its two products; dbias is summed before. */
+typedef struct {
+  int dtype, activation;
+  int64_t m, k, n;
+  const void* dy;
+  int64_t lddy;
+  const void* pre;
+  int64_t ldpre;
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw;
+  void *dx, *dw, *dbias;
+} qrb_linear_backward_args;
+QRB_API size_t qrb_linear_backward_workspace_size(const qrb_linear_backward_args* a);
+QRB_API int qrb_linear_backward(const qrb_linear_backward_args* a, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
 #ifdef __cplusplus
 }
 #endif

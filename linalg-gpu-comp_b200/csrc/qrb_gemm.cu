@@ -1,0 +1,537 @@
+// y = epilogue(A B^T) on the 5th-generation tensor cores: the linear layer's forward product
+// (x w^T with bias, activation and residual in the epilogue) and both products of its backward.
+//
+// Persistent warp-specialised blocks, one per SM: a TMA producer fills a ring of 64-deep stages
+// (128-byte swizzle; operands with k along their rows and operands with k across them are both
+// read as they lie, so no backward product transposes anything), one thread issues
+// 128 x BN x 16 MMAs into TMEM, and four warps run the epilogue of one tile while the next one's
+// MMAs fill the other accumulator buffer.  BN = 256 reads 12 KB of shared memory per 128-cycle
+// MMA; narrower tiles serve small outputs.
+//
+//   * Few rows (m <= 128): the operands change places, so the 128-row side of the MMA is the weight
+//     and its 16 .. 128 column side the rows: no tensor-core row is wasted on padding, and the
+//     weight streams through once.
+//   * Few tiles: the blocks divide k; fp32 partials are added in order by reduce_kernel, which
+//     then runs the epilogue, so results repeat.
+//   * fp32: three bf16 planes per operand, x = x0 + x1 + x2 to 2^-27; the six products x_i w_j with
+//     i + j < 3.  The five small ones have an accumulator of their own, and k is cut at 4096 (fp32
+//     partials beyond): the tensor cores' accumulation truncates, and its bias grows with the
+//     number of additions to the large sum.
+//
+// Every wait is bounded (mbar_wait_abort); see qrb_wide.cu.  No TMA load uses cluster multicast.
+#include "qrb_gemm.cuh"
+
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <mutex>
+
+#include "qrb_sm100.cuh"
+
+namespace qrb {
+namespace gemm {
+namespace {
+
+using namespace sm100;
+
+constexpr int kBM = 128, kBK = 64, kThreads = 256;   // warps: producer, MMA, 2 idle, 4 epilogue
+constexpr int kMaxTerms = 6;
+constexpr int64_t kMaxSplitK32 = 4096;   // longest k of one fp32 accumulation
+
+struct GemmArgs {
+  int64_t M, N;                 // MMA orientation: A's rows, B's rows
+  int tiles_m, tiles_n, splits;
+  int kblocks, per_split;       // 64-deep blocks of k in all and per split
+  int terms, sets;              // piece products; accumulators per tile (2: small products apart)
+  int a_mn, b_mn, swap;         // swap: A's rows are the output's columns
+  uint32_t idesc;
+  signed char pa[kMaxTerms], pb[kMaxTerms], set[kMaxTerms];
+  float* partial;               // splits > 1: [split][m][n] of the output
+  int64_t out_m, out_n;
+  Epilogue e;
+  int* err;
+};
+
+template <int BN>
+struct Cfg {
+  static constexpr uint32_t kA = kBM * kBK * 2, kB = BN * kBK * 2, kStage = kA + kB;
+  static constexpr int kStages = BN == 256 ? 4 : 6;
+  static constexpr uint32_t kBar = kStages * kStage;
+  static constexpr uint32_t kSmem = kBar + 256 + 1024;
+};
+
+struct Bars {
+  uint64_t full[6], empty[6], accf[2], acce[2], drain;
+  uint32_t tmem;
+  int abort;
+};
+static_assert(sizeof(Bars) <= 256, "barrier block");
+
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d),
+      "l"(ad), "l"(bd), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ float load1(const void* p, int64_t i, int dtype) {
+  if (dtype == QRB_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  if (dtype == QRB_F16) return __half2float(static_cast<const __half*>(p)[i]);
+  return static_cast<const float*>(p)[i];
+}
+__device__ __forceinline__ void store1(void* p, int64_t i, int dtype, float x) {
+  if (dtype == QRB_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+  else if (dtype == QRB_F16) static_cast<__half*>(p)[i] = __float2half_rn(x);
+  else static_cast<float*>(p)[i] = x;
+}
+
+__device__ __forceinline__ uint32_t pack16(float a, float b, int dtype) {
+  if (dtype == QRB_BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Eight neighbouring outputs, 16-byte aligned where `vec`.
+__device__ __forceinline__ void store8(void* p, int64_t i, int dtype, const float* x, int count, bool vec) {
+  if (vec && count == 8) {
+    if (dtype == QRB_F32) {
+      float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
+      q[0] = make_float4(x[0], x[1], x[2], x[3]);
+      q[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) =
+          make_uint4(pack16(x[0], x[1], dtype), pack16(x[2], x[3], dtype), pack16(x[4], x[5], dtype),
+                     pack16(x[6], x[7], dtype));
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < count) store1(p, i + j, dtype, x[j]);
+}
+
+__device__ __forceinline__ void add8(const void* p, int64_t i, int dtype, float* x, int count, bool vec) {
+  if (vec && count == 8 && dtype != QRB_F32) {
+    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (dtype == QRB_BF16) {
+        x[2 * j] += __uint_as_float(u[j] << 16);
+        x[2 * j + 1] += __uint_as_float(u[j] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
+        x[2 * j] += f.x;
+        x[2 * j + 1] += f.y;
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < count) x[j] += load1(p, i + j, dtype);
+}
+
+__device__ __forceinline__ bool aligned_rows(const void* p, int64_t ld, int dtype) {
+  const int64_t v = dtype == QRB_F32 ? 4 : 8;
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % v == 0;
+}
+
+// Work unit u: split fastest (the splits of a tile run together), then tiles in groups of eight
+// rows of tiles, so that blocks running together share operand tiles in L2.
+__device__ __forceinline__ void tile_of(const GemmArgs& g, int u, int& tm, int& tn, int& sp) {
+  sp = u % g.splits;
+  const int t = u / g.splits;
+  const int group = 8 * g.tiles_n, gi = t / group, first = gi * 8;
+  const int rows = min(8, g.tiles_m - first), r = t - gi * group;
+  tm = first + r % rows;
+  tn = r / rows;
+}
+
+template <int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+            const __grid_constant__ GemmArgs g) {
+  using C = Cfg<BN>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                                       ~uintptr_t(1023));
+  Bars& bars = *reinterpret_cast<Bars*>(sm + C::kBar);
+  volatile int* abort = &bars.abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int units = g.tiles_m * g.tiles_n * g.splits;
+  const int bufs = 2 * g.sets * BN <= 512 ? 2 : 1;
+  const uint32_t cols = (uint32_t)(bufs * g.sets * BN) < 32u ? 32u : (uint32_t)(bufs * g.sets * BN);
+
+  if (tid == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&bars.full[i], 1);
+      mbar_init(&bars.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.accf[i], 1);
+      mbar_init(&bars.acce[i], 4);
+    }
+    mbar_init(&bars.drain, 1);
+    bars.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(&bars.tmem, cols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      prefetch_tensormap(&map_a);
+      prefetch_tensormap(&map_b);
+      int64_t it = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        int tm, tn, sp;
+        tile_of(g, u, tm, tn, sp);
+        const int kb0 = sp * g.per_split, kb1 = min(g.kblocks, kb0 + g.per_split);
+        for (int t = 0; t < g.terms && ok; ++t)
+          for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int st = (int)(it % C::kStages);
+            const int64_t use = it / C::kStages;
+            if (use > 0 && !mbar_wait_abort(&bars.empty[st], (uint32_t)((use - 1) & 1), abort, g.err, 41)) {
+              ok = false;
+              break;
+            }
+            unsigned char* sa = sm + st * C::kStage;
+            unsigned char* sb = sa + C::kA;
+            mbar_arrive_expect_tx(&bars.full[st], C::kStage);
+            if (g.a_mn) {
+              tma_load_3d(sa, &map_a, tm * kBM, kb * kBK, g.pa[t], &bars.full[st]);
+              tma_load_3d(sa + 8192, &map_a, tm * kBM + 64, kb * kBK, g.pa[t], &bars.full[st]);
+            } else {
+              tma_load_3d(sa, &map_a, kb * kBK, tm * kBM, g.pa[t], &bars.full[st]);
+            }
+            if (g.b_mn) {
+              for (int j = 0; j < BN / 64; ++j)
+                tma_load_3d(sb + j * 8192, &map_b, tn * BN + 64 * j, kb * kBK, g.pb[t], &bars.full[st]);
+            } else {
+              tma_load_3d(sb, &map_b, kb * kBK, tn * BN, g.pb[t], &bars.full[st]);
+            }
+          }
+      }
+      if (*abort) {   // let every load this block issued land before its shared memory goes away
+        for (int st = 0; st < C::kStages; ++st)
+          if (it > st) mbar_wait(&bars.full[st], (uint32_t)(((it - 1 - st) / C::kStages) & 1), 1u << 22);
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      int64_t it = 0;
+      int n = 0;
+      bool ok = true, issued = false;
+      const uint32_t a_lbo = g.a_mn ? 8192 : 16, a_step = g.a_mn ? 2048 : 32;
+      const uint32_t b_lbo = g.b_mn ? 8192 : 16, b_step = g.b_mn ? 2048 : 32;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++n) {
+        int tm, tn, sp;
+        tile_of(g, u, tm, tn, sp);
+        const int kb0 = sp * g.per_split, kb1 = min(g.kblocks, kb0 + g.per_split);
+        const int buf = n % bufs, use = n / bufs;
+        if (use > 0 && !mbar_wait_abort(&bars.acce[buf], (uint32_t)((use - 1) & 1), abort, g.err, 42)) break;
+        tc_fence_after();
+        int seen = 0;   // accumulators that hold something already
+        for (int t = 0; t < g.terms && ok; ++t) {
+          const uint32_t d = tmem + (uint32_t)((buf * g.sets + g.set[t]) * BN);
+          for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int st = (int)(it % C::kStages);
+            if (!mbar_wait_abort(&bars.full[st], (uint32_t)((it / C::kStages) & 1), abort, g.err, 43)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t sa = smem_u32(sm + st * C::kStage), sb = sa + C::kA;
+#pragma unroll
+            for (int kk = 0; kk < kBK / 16; ++kk) {
+              mma_f16(d, sdesc_sw128(sa + kk * a_step, a_lbo, 1024), sdesc_sw128(sb + kk * b_step, b_lbo, 1024),
+                      g.idesc, ((seen >> g.set[t]) & 1) | (kk > 0));
+            }
+            seen |= 1 << g.set[t];
+            mma_commit(&bars.empty[st]);
+            issued = true;
+          }
+        }
+        if (ok) mma_commit(&bars.accf[buf]);
+      }
+      if (*abort && issued) {   // tensor memory must not be released under running MMAs
+        mma_commit(&bars.drain);
+        mbar_wait(&bars.drain, 0, 1u << 22);
+      }
+    }
+  } else if (warp >= 4) {
+    // ---------------- epilogue: TMEM lane = A's row ----------------
+    const int q = warp & 3;
+    const uint32_t tl = (uint32_t)(32 * q) << 16;
+    const Epilogue& e = g.e;
+    const bool vec = (e.y == nullptr || aligned_rows(e.y, e.ldy, e.dtype)) &&
+                     (e.residual == nullptr || aligned_rows(e.residual, e.ldr, e.dtype)) &&
+                     (e.pre == nullptr || aligned_rows(e.pre, e.ldpre, e.dtype));
+    int n = 0;
+    for (int u = blockIdx.x; u < units; u += gridDim.x, ++n) {
+      int tm, tn, sp;
+      tile_of(g, u, tm, tn, sp);
+      const int buf = n % bufs, use = n / bufs;
+      const int64_t r = (int64_t)tm * kBM + 32 * q + lane, c0 = (int64_t)tn * BN;
+      const float rb = g.swap && e.bias != nullptr && r < g.M ? load1(e.bias, r, e.dtype) : 0.f;
+      // the whole warp goes on or leaves: tensor memory loads are collective
+      if (!__all_sync(0xffffffffu, mbar_wait_abort(&bars.accf[buf], (uint32_t)(use & 1), abort, g.err, 44))) break;
+      tc_fence_after();
+      constexpr int kCh = 32;
+#pragma unroll 1
+      for (int c = 0; c < BN; c += kCh) {
+        float x[32];
+        const uint32_t at = tmem + tl + (uint32_t)(buf * g.sets * BN + c);
+        tmem_ld32(at, x);
+        if (g.sets == 2) {
+          float y[32];
+          tmem_ld32(at + BN, y);
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (fabsf(x[j]) <= 3.4e38f) x[j] += y[j];   // inf * 0 among the small products is no NaN of the sum
+        }
+        if (c + kCh >= BN) {   // this warp's last read of the buffer
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.acce[buf]);
+        }
+        float cb = 0.f;   // lane j: the bias of column c + j
+        if (!g.swap && g.splits == 1 && e.bias != nullptr && c0 + c + lane < g.N) cb = load1(e.bias, c0 + c + lane, e.dtype);
+        if (!g.swap && g.splits == 1) {
+#pragma unroll
+          for (int j = 0; j < kCh; ++j) x[j] += __shfl_sync(0xffffffffu, cb, j);
+        }
+        if (r >= g.M) continue;
+        if (g.splits > 1) {
+          if (g.swap) {
+#pragma unroll
+            for (int j = 0; j < kCh; ++j)
+              if (c0 + c + j < g.N) g.partial[((int64_t)sp * g.out_m + c0 + c + j) * g.out_n + r] = x[j];
+          } else {
+            float* to = g.partial + ((int64_t)sp * g.out_m + r) * g.out_n + c0 + c;
+            const bool v4 = g.out_n % 4 == 0;
+#pragma unroll
+            for (int j = 0; j < kCh; j += 4) {
+              if (v4 && c0 + c + j + 3 < g.N) *reinterpret_cast<float4*>(to + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+              else
+                for (int i = 0; i < 4; ++i)
+                  if (c0 + c + j + i < g.N) to[j + i] = x[j + i];
+            }
+          }
+          continue;
+        }
+        if (g.swap) {
+#pragma unroll
+          for (int j = 0; j < kCh; ++j) {
+            const int64_t m = c0 + c + j;
+            if (m >= g.N) continue;
+            float v = x[j] + rb;
+            if (e.pre != nullptr) store1(e.pre, m * e.ldpre + r, e.dtype, v);
+            v = activate(v, e.act);
+            if (e.residual != nullptr) v += load1(e.residual, m * e.ldr + r, e.dtype);
+            store1(e.y, m * e.ldy + r, e.dtype, v);
+          }
+          continue;
+        }
+#pragma unroll
+        for (int j = 0; j < kCh; j += 8) {
+          const int64_t left = g.N - (c0 + c + j);
+          const int count = left < 8 ? (left < 0 ? 0 : (int)left) : 8;
+          if (e.pre != nullptr) store8(e.pre, r * e.ldpre + c0 + c + j, e.dtype, x + j, count, vec);
+          if (e.act != QRB_ACT_NONE) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[j + i] = activate(x[j + i], e.act);
+          }
+          if (e.residual != nullptr) add8(e.residual, r * e.ldr + c0 + c + j, e.dtype, x + j, count, vec);
+          store8(e.y, r * e.ldy + c0 + c + j, e.dtype, x + j, count, vec);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, cols);
+  }
+}
+
+// y = epilogue(sum of the splits' partials, in order).
+__global__ void __launch_bounds__(256) reduce_kernel(const float* part, int splits, int64_t m, int64_t n, Epilogue e) {
+  const int64_t total = m * n;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    float x = 0.f;
+    for (int s = 0; s < splits; ++s) x += part[s * total + i];
+    const int64_t r = i / n, c = i - r * n;
+    if (e.bias != nullptr) x += load1(e.bias, c, e.dtype);
+    if (e.pre != nullptr) store1(e.pre, r * e.ldpre + c, e.dtype, x);
+    x = activate(x, e.act);
+    if (e.residual != nullptr) x += load1(e.residual, r * e.ldr + c, e.dtype);
+    store1(e.y, r * e.ldy + c, e.dtype, x);
+  }
+}
+
+// ---- host side ----
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+bool make_map(CUtensorMap* map, const Operand& o, int64_t mn, int64_t k, bool half, int rows) {
+  auto fn = encoder();
+  if (fn == nullptr) return false;
+  const uint64_t inner = (uint64_t)(o.mn_major ? mn : k), outer = (uint64_t)(o.mn_major ? k : mn);
+  cuuint64_t dims[3] = {inner, outer, (cuuint64_t)o.pieces};
+  cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(o.pieces > 1 ? o.plane : o.ld * (int64_t)outer) * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)(o.mn_major ? kBK : rows), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.p),
+            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Plan {
+  int bn, swap, tiles_m, tiles_n, splits, kblocks, per_split;
+};
+
+// Tile width and split of an m x n x k product.  Up to 128 rows: swapped, the narrowest tile that
+// holds them.  Otherwise the widest of 256, 128, 64 columns whose tiles still fill two thirds of the
+// SMs (a wide tile reads the least shared memory per MMA, an idle SM costs more), and where even 64
+// does not, k is split.
+Plan plan(int64_t m, int64_t n, int64_t k, int pieces) {
+  Plan p{};
+  const int sms = sm_count();
+  p.kblocks = (int)((k + kBK - 1) / kBK);
+  p.swap = m <= 128;
+  auto tiles = [&](int bn) {
+    p.bn = bn;
+    p.tiles_m = (int)(((p.swap ? n : m) + kBM - 1) / kBM);
+    p.tiles_n = (int)(((p.swap ? m : n) + bn - 1) / bn);
+    return (int64_t)p.tiles_m * p.tiles_n;
+  };
+  int64_t t;
+  if (p.swap) {
+    t = tiles(m <= 64 ? 64 : 128);
+  } else {
+    t = tiles(256);
+    if (t * 3 < sms * 2) t = tiles(128);
+    if (t * 3 < sms * 2) t = tiles(64);
+  }
+  // a split is worth at least four stages of work, and there are 16 at most
+  int64_t splits = t * 2 <= sms ? sms / t : 1;
+  if (splits > (p.kblocks + 3) / 4) splits = (p.kblocks + 3) / 4;
+  if (splits > 16) splits = 16;
+  if (splits < 1) splits = 1;
+  if (pieces > 1) {
+    const int64_t need = (p.kblocks + kMaxSplitK32 / kBK - 1) / (kMaxSplitK32 / kBK);
+    if (splits < need) splits = need;
+  }
+  p.per_split = (int)((p.kblocks + splits - 1) / splits);
+  p.splits = (p.kblocks + p.per_split - 1) / p.per_split;
+  return p;
+}
+
+template <int BN>
+cudaError_t run(const CUtensorMap& ma, const CUtensorMap& mb, const GemmArgs& g, cudaStream_t s) {
+  constexpr int smem = Cfg<BN>::kSmem;
+  cudaError_t e = cudaFuncSetAttribute(gemm_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const int64_t units = (int64_t)g.tiles_m * g.tiles_n * g.splits;
+  const int sms = sm_count();
+  gemm_kernel<BN><<<(unsigned)(units < sms ? units : sms), kThreads, smem, s>>>(ma, mb, g);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+bool supported() { return encoder() != nullptr; }
+
+size_t scratch(int64_t m, int64_t n, int64_t k, int pieces) {
+  if (m < 1 || n < 1 || k < 1) return 0;
+  const Plan p = plan(m, n, k, pieces);
+  return p.splits > 1 ? (size_t)p.splits * m * n : 0;
+}
+
+int launches(int64_t m, int64_t n, int64_t k, int pieces) { return plan(m, n, k, pieces).splits > 1 ? 2 : 1; }
+
+cudaError_t multiply(const Operand& A, const Operand& B, int64_t m, int64_t n, int64_t k, bool half, const Epilogue& e,
+                     float* ws, cudaStream_t s) {
+  const Plan p = plan(m, n, k, A.pieces);
+  GemmArgs g{};
+  const Operand &a = p.swap ? B : A, &b = p.swap ? A : B;
+  g.M = p.swap ? n : m;
+  g.N = p.swap ? m : n;
+  g.tiles_m = p.tiles_m;
+  g.tiles_n = p.tiles_n;
+  g.splits = p.splits;
+  g.kblocks = p.kblocks;
+  g.per_split = p.per_split;
+  g.a_mn = a.mn_major;
+  g.b_mn = b.mn_major;
+  g.swap = p.swap;
+  const uint32_t fmt = half ? 0 : 1;
+  g.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a.mn_major << 15) | ((uint32_t)b.mn_major << 16) |
+            ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
+  if (a.pieces == 1) {
+    g.terms = 1;
+    g.sets = 1;
+  } else {   // smallest products first; the large one alone in accumulator 0
+    static const signed char pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0}, set[6] = {1, 1, 1, 1, 1, 0};
+    g.terms = 6;
+    g.sets = 2;
+    for (int i = 0; i < 6; ++i) {
+      g.pa[i] = pa[i];
+      g.pb[i] = pb[i];
+      g.set[i] = set[i];
+    }
+  }
+  g.partial = ws;
+  g.out_m = m;
+  g.out_n = n;
+  g.e = e;
+  g.err = device_error_flag();
+  if (g.err == nullptr) return cudaErrorInvalidValue;
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, a, g.M, k, half, kBM) || !make_map(&mb, b, g.N, k, half, p.bn)) return cudaErrorInvalidValue;
+  cudaError_t r;
+  {
+    const double bytes = (double)(m * k + n * k) * 2 * A.pieces + (double)m * n * (e.dtype == QRB_F32 ? 4 : 2);
+    LaunchTimer t("linear_gemm_kernel", s, bytes, 2.0 * m * n * k);
+    switch (p.bn) {
+      case 64: r = run<64>(ma, mb, g, s); break;
+      case 128: r = run<128>(ma, mb, g, s); break;
+      default: r = run<256>(ma, mb, g, s); break;
+    }
+  }
+  if (r != cudaSuccess || p.splits == 1) return r;
+  LaunchTimer t("linear_reduce_kernel", s, 4.0 * p.splits * m * n, (double)p.splits * m * n);
+  const int64_t blocks = (m * n + 255) / 256, most = (int64_t)sm_count() * 8;
+  reduce_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(ws, p.splits, m, n, e);
+  return cudaGetLastError();
+}
+
+}  // namespace gemm
+}  // namespace qrb

@@ -1,0 +1,431 @@
+// The linear layer y = act(x w^T + b) + r and its backward pass: C ABI (include/qrb200_nn.h), and
+// the elementwise kernels around the products of qrb_gemm.cu.
+//
+//   forward:  [lay out x, w] product with the epilogue
+//   backward: dp = dy act'(pre) and the column sums of dp (dbias), then dx = dp w, dw = dp^T x
+// Operands the tensor maps cannot address (rows not 16-byte aligned) are laid out in the workspace
+// first, fp32 ones as three bf16 planes.  dp of the 16-bit types is rounded to the type once: it is
+// an operand of 16-bit products, whose sums average the roundings out.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdarg>
+#include <cstdio>
+
+#include "qrb_gemm.cuh"
+
+namespace qrb {
+namespace gemm {
+namespace {
+
+template <typename T>
+__device__ __forceinline__ float tof(T x);
+template <>
+__device__ __forceinline__ float tof(float x) { return x; }
+template <>
+__device__ __forceinline__ float tof(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float tof(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ T fromf(float x);
+template <>
+__device__ __forceinline__ float fromf(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 fromf(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half fromf(float x) { return __float2half_rn(x); }
+
+// One value of a laid-out operand: the value itself, or the three bf16 planes of an fp32 one.  A
+// value that is not finite keeps its first plane only (inf - inf would put NaN into the others).
+template <typename T>
+__device__ __forceinline__ void put(void* to, int64_t i, int64_t plane, float x) {
+  static_cast<T*>(to)[i] = fromf<T>(x);
+}
+template <>
+__device__ __forceinline__ void put<float>(void* to, int64_t i, int64_t plane, float x) {
+  __nv_bfloat16* p = static_cast<__nv_bfloat16*>(to);
+  const __nv_bfloat16 a = __float2bfloat16_rn(x);
+  float r = x - __bfloat162float(a);
+  if (!(fabsf(r) <= 3.4e38f)) r = 0.f;
+  const __nv_bfloat16 b = __float2bfloat16_rn(r);
+  p[i] = a;
+  p[i + plane] = b;
+  p[i + 2 * plane] = __float2bfloat16_rn(r - __bfloat162float(b));
+}
+
+// rows x cols of `from` (row stride ld) to rows of `pitch` elements.
+template <typename T>
+__global__ void __launch_bounds__(256) layout_kernel(const T* from, int64_t ld, int64_t rows, int64_t cols, void* to,
+                                                     int64_t pitch) {
+  const int64_t total = rows * cols, plane = rows * pitch;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / cols, c = i - r * cols;
+    put<T>(to, r * pitch + c, plane, tof(from[r * ld + c]));
+  }
+}
+
+__device__ __forceinline__ float slope(float x, int act) {
+  if (act == QRB_ACT_RELU) return x > 0.f ? 1.f : (x != x ? x : 0.f);
+  if (act == QRB_ACT_SILU) {
+    const float s = 1.f / (1.f + expf(-x));
+    return s * (1.f + x * (1.f - s));
+  }
+  if (act == QRB_ACT_GELU)
+    return 0.5f * (1.f + erff(x * 0.70710678118654752f)) + x * 0.39894228040143268f * expf(-0.5f * x * x);
+  return 1.f;
+}
+
+constexpr int kSumRows = 128, kSumCols = 64;   // rows and columns a block of dp_kernel covers
+
+// dp = dy act'(pre) into a laid-out operand (to, unless null) and its column sums over the block's
+// rows (sums[row block][n], unless null).  Sums are of the fp32 products, before any rounding.
+template <typename T>
+__global__ void __launch_bounds__(256) dp_kernel(const T* dy, int64_t ldy, const T* pre, int64_t ldp, int act,
+                                                 int64_t m, int64_t n, void* to, int64_t pitch, float* sums) {
+  __shared__ float part[4][kSumCols];
+  const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
+  const int64_t col = (int64_t)blockIdx.x * kSumCols + c, r0 = (int64_t)blockIdx.y * kSumRows;
+  float s = 0.f;
+  if (col < n) {
+#pragma unroll 8
+    for (int i = g; i < kSumRows; i += 4) {
+      const int64_t r = r0 + i;
+      if (r >= m) break;
+      float x = tof(dy[r * ldy + col]);
+      if (act != QRB_ACT_NONE) x *= slope(tof(pre[r * ldp + col]), act);
+      s += x;
+      if (to != nullptr) put<T>(to, r * pitch + col, m * pitch, x);
+    }
+  }
+  if (sums == nullptr) return;
+  part[g][c] = s;
+  __syncthreads();
+  if (g == 0 && col < n)
+    sums[(int64_t)blockIdx.y * n + col] = (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) colsum_kernel(const float* sums, int64_t blocks, int64_t n, T* out) {
+  __shared__ float part[8][32];
+  const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int64_t col = (int64_t)blockIdx.x * 32 + c;
+  float s = 0.f;
+  if (col < n)
+    for (int64_t b = g; b < blocks; b += 8) s += sums[b * n + col];
+  part[g][c] = s;
+  __syncthreads();
+  if (g == 0 && col < n) {
+    for (int i = 1; i < 8; ++i) s += part[i][c];
+    out[col] = fromf<T>(s);
+  }
+}
+
+}  // namespace
+}  // namespace gemm
+}  // namespace qrb
+
+namespace {
+
+using qrb::gemm::Epilogue;
+using qrb::gemm::Operand;
+
+int fail(int status, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  return qrb::set_error(status, buf);
+}
+
+#define TRY(x)                   \
+  do {                           \
+    int _s = (x);                \
+    if (_s != QRB_OK) return _s; \
+  } while (0)
+#define CUDA(x, what)                                                                               \
+  do {                                                                                              \
+    cudaError_t _e = (x);                                                                           \
+    if (_e != cudaSuccess)                                                                          \
+      return fail(QRB_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorName(_e), cudaGetErrorString(_e)); \
+  } while (0)
+
+size_t al(size_t x) { return (x + 255) & ~size_t(255); }
+size_t esize(int dtype) { return dtype == QRB_F32 ? 4 : 2; }
+int64_t pitch_of(int64_t cols) { return (cols + 7) / 8 * 8; }
+
+// Whether the tensor maps can read the rows as they lie.
+bool direct(int dtype, const void* p, int64_t ld, int64_t cols) {
+  return dtype != QRB_F32 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0 && ld >= cols;
+}
+size_t layout_bytes(int dtype, int64_t rows, int64_t cols) {
+  return al((size_t)rows * pitch_of(cols) * 2 * (dtype == QRB_F32 ? 3 : 1));
+}
+
+int check_common(int dtype, int act, int64_t m, int64_t k, int64_t n) {
+  if (dtype != QRB_F32 && dtype != QRB_BF16 && dtype != QRB_F16)
+    return fail(QRB_ERR_INVALID_ARG, "dtype must be QRB_F32, QRB_BF16 or QRB_F16 (got %d)", dtype);
+  if (act < QRB_ACT_NONE || act > QRB_ACT_GELU) return fail(QRB_ERR_INVALID_ARG, "unknown activation %d", act);
+  if (m < 0 || n < 1 || k < 1)
+    return fail(QRB_ERR_INVALID_ARG, "m must be >= 0, k and n >= 1 (got %lld, %lld, %lld)", (long long)m, (long long)k,
+                (long long)n);
+  const int64_t top = (int64_t)1 << 30;
+  if (m > top || n > top || k > top || (m > 0 && m * n / (128 * 64) > top / 16) || k * n / (128 * 64) > top / 16 ||
+      m * k / (128 * 64) > top / 16 || m > (int64_t)128 * 65535)
+    return fail(QRB_ERR_UNSUPPORTED, "sizes m = %lld, k = %lld, n = %lld are too large", (long long)m, (long long)k,
+                (long long)n);
+  return QRB_OK;
+}
+
+int check_ptr(const void* p, const char* name, int dtype) {
+  if (p == nullptr) return fail(QRB_ERR_INVALID_ARG, "%s is null", name);
+  if ((reinterpret_cast<uintptr_t>(p) & (esize(dtype) - 1)) != 0)
+    return fail(QRB_ERR_INVALID_ARG, "%s must be %zu-byte aligned", name, esize(dtype));
+  return QRB_OK;
+}
+
+int check_ld(int64_t ld, int64_t cols, const char* name) {
+  if (ld < cols) return fail(QRB_ERR_INVALID_ARG, "%s must be at least %lld (got %lld)", name, (long long)cols, (long long)ld);
+  return QRB_OK;
+}
+
+int check_device() {
+  int dev = 0, major = 0;
+  CUDA(cudaGetDevice(&dev), "cudaGetDevice");
+  static int cache[64] = {0};
+  if (dev < 64) major = cache[dev];
+  if (major == 0) {
+    CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev), "cudaDeviceGetAttribute");
+    if (dev < 64) cache[dev] = major;
+  }
+  if (major != 10)
+    return fail(QRB_ERR_DEVICE, "device %d has compute capability %d.x; libqrb200 needs sm_100", dev, major);
+  if (!qrb::gemm::supported()) return fail(QRB_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+  return QRB_OK;
+}
+
+int check_ws(const void* ws, size_t have, size_t need) {
+  if (need > 0 && (ws == nullptr || have < need))
+    return fail(QRB_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given%s", need, have,
+                ws == nullptr ? " (null)" : "");
+  if (need > 0 && (reinterpret_cast<uintptr_t>(ws) & 255u) != 0)
+    return fail(QRB_ERR_INVALID_ARG, "workspace must be 256-byte aligned");
+  return QRB_OK;
+}
+
+unsigned elem_grid(int64_t total) {
+  const int64_t blocks = (total + 255) / 256, most = (int64_t)qrb::sm_count() * 16;
+  return (unsigned)(blocks < most ? blocks : most);
+}
+
+template <typename T>
+void layout_t(const void* p, int64_t ld, int64_t rows, int64_t cols, void* to, cudaStream_t s) {
+  qrb::gemm::layout_kernel<T><<<elem_grid(rows * cols), 256, 0, s>>>(static_cast<const T*>(p), ld, rows, cols, to,
+                                                                    pitch_of(cols));
+}
+
+// The operand a product reads: x itself, or its copy at `to`.
+int operand(Operand& o, int dtype, const void* p, int64_t ld, int64_t rows, int64_t cols, bool mn_major, void* to,
+            cudaStream_t s) {
+  o.mn_major = mn_major;
+  o.pieces = dtype == QRB_F32 ? 3 : 1;
+  if (direct(dtype, p, ld, cols)) {
+    o.p = p;
+    o.ld = ld;
+    o.plane = 0;
+    return QRB_OK;
+  }
+  o.p = to;
+  o.ld = pitch_of(cols);
+  o.plane = rows * o.ld;
+  qrb::LaunchTimer t("linear_layout_kernel", s, (double)rows * cols * 2 * esize(dtype), 0);
+  if (dtype == QRB_F32) layout_t<float>(p, ld, rows, cols, to, s);
+  else if (dtype == QRB_BF16) layout_t<__nv_bfloat16>(p, ld, rows, cols, to, s);
+  else layout_t<__half>(p, ld, rows, cols, to, s);
+  CUDA(cudaGetLastError(), "linear layout launch");
+  return QRB_OK;
+}
+
+struct FwdLayout {
+  size_t x, w, part, total;
+};
+FwdLayout fwd_layout(const qrb_linear_args& a) {
+  FwdLayout l{};
+  size_t at = 0;
+  l.x = at;
+  if (!direct(a.dtype, a.x, a.ldx, a.k)) at += layout_bytes(a.dtype, a.m, a.k);
+  l.w = at;
+  if (!direct(a.dtype, a.w, a.ldw, a.k)) at += layout_bytes(a.dtype, a.n, a.k);
+  l.part = at;
+  at += al(qrb::gemm::scratch(a.m, a.n, a.k, a.dtype == QRB_F32 ? 3 : 1) * 4);
+  l.total = at;
+  return l;
+}
+
+int check_forward(const qrb_linear_args* a) {
+  if (a == nullptr) return fail(QRB_ERR_INVALID_ARG, "args is null");
+  TRY(check_common(a->dtype, a->activation, a->m, a->k, a->n));
+  TRY(check_ld(a->ldx, a->k, "ldx"));
+  TRY(check_ld(a->ldw, a->k, "ldw"));
+  return QRB_OK;
+}
+
+struct BwdLayout {
+  size_t dp, x, w, sums, part, total;
+};
+bool makes_dp(const qrb_linear_backward_args& a) {
+  return a.activation != QRB_ACT_NONE || !direct(a.dtype, a.dy, a.lddy, a.n);
+}
+BwdLayout bwd_layout(const qrb_linear_backward_args& a) {
+  const int pieces = a.dtype == QRB_F32 ? 3 : 1;
+  BwdLayout l{};
+  size_t at = 0;
+  l.dp = at;
+  if (makes_dp(a)) at += layout_bytes(a.dtype, a.m, a.n);
+  l.x = at;
+  if (!direct(a.dtype, a.x, a.ldx, a.k)) at += layout_bytes(a.dtype, a.m, a.k);
+  l.w = at;
+  if (!direct(a.dtype, a.w, a.ldw, a.k)) at += layout_bytes(a.dtype, a.n, a.k);
+  l.sums = at;
+  at += al((size_t)((a.m + 127) / 128) * a.n * 4);
+  l.part = at;
+  size_t p1 = qrb::gemm::scratch(a.m, a.k, a.n, pieces), p2 = qrb::gemm::scratch(a.n, a.k, a.m, pieces);
+  at += al((p1 > p2 ? p1 : p2) * 4);
+  l.total = at;
+  return l;
+}
+
+int check_backward(const qrb_linear_backward_args* a) {
+  if (a == nullptr) return fail(QRB_ERR_INVALID_ARG, "args is null");
+  TRY(check_common(a->dtype, a->activation, a->m, a->k, a->n));
+  TRY(check_ld(a->lddy, a->n, "lddy"));
+  TRY(check_ld(a->ldx, a->k, "ldx"));
+  TRY(check_ld(a->ldw, a->k, "ldw"));
+  if (a->activation != QRB_ACT_NONE) TRY(check_ld(a->ldpre, a->n, "ldpre"));
+  return QRB_OK;
+}
+
+template <typename T>
+int run_dp(const qrb_linear_backward_args& a, void* to, float* sums, cudaStream_t s) {
+  const int64_t rb = (a.m + qrb::gemm::kSumRows - 1) / qrb::gemm::kSumRows;
+  {
+    qrb::LaunchTimer t("linear_dp_kernel", s, (double)a.m * a.n * sizeof(T) * 3, (double)a.m * a.n);
+    const dim3 grid((unsigned)((a.n + qrb::gemm::kSumCols - 1) / qrb::gemm::kSumCols), (unsigned)rb);
+    qrb::gemm::dp_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(a.dy), a.lddy, static_cast<const T*>(a.pre),
+                                                 a.ldpre, a.activation, a.m, a.n, to, pitch_of(a.n), sums);
+    CUDA(cudaGetLastError(), "linear dp launch");
+  }
+  if (sums != nullptr) {
+    qrb::LaunchTimer t("linear_colsum_kernel", s, 4.0 * rb * a.n, (double)rb * a.n);
+    qrb::gemm::colsum_kernel<T><<<(unsigned)((a.n + 31) / 32), 256, 0, s>>>(sums, rb, a.n, static_cast<T*>(a.dbias));
+    CUDA(cudaGetLastError(), "linear column sum launch");
+  }
+  return QRB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t qrb_linear_workspace_size(const qrb_linear_args* a) {
+  if (check_forward(a) != QRB_OK || a->m == 0) return 0;
+  return fwd_layout(*a).total;
+}
+
+int qrb_linear_forward(const qrb_linear_args* a, void* ws, size_t wsb, void* stream) {
+  TRY(check_forward(a));
+  if (a->m == 0) return QRB_OK;
+  TRY(check_ptr(a->x, "x", a->dtype));
+  TRY(check_ptr(a->w, "w", a->dtype));
+  TRY(check_ptr(a->y, "y", a->dtype));
+  TRY(check_ld(a->ldy, a->n, "ldy"));
+  if (a->bias != nullptr) TRY(check_ptr(a->bias, "bias", a->dtype));
+  if (a->residual != nullptr) {
+    TRY(check_ptr(a->residual, "residual", a->dtype));
+    TRY(check_ld(a->ldr, a->n, "ldr"));
+  }
+  if (a->pre != nullptr) {
+    TRY(check_ptr(a->pre, "pre", a->dtype));
+    TRY(check_ld(a->ldpre, a->n, "ldpre"));
+  }
+  const FwdLayout l = fwd_layout(*a);
+  TRY(check_ws(ws, wsb, l.total));
+  TRY(check_device());
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  char* w8 = static_cast<char*>(ws);
+  Operand x, w;
+  TRY(operand(x, a->dtype, a->x, a->ldx, a->m, a->k, false, w8 + l.x, s));
+  TRY(operand(w, a->dtype, a->w, a->ldw, a->n, a->k, false, w8 + l.w, s));
+  const Epilogue e{a->dtype, a->activation, a->y, a->ldy, a->bias, a->residual, a->ldr, a->pre, a->ldpre};
+  CUDA(qrb::gemm::multiply(x, w, a->m, a->n, a->k, a->dtype == QRB_F16, e, reinterpret_cast<float*>(w8 + l.part), s),
+       "linear product launch");
+  return QRB_OK;
+}
+
+size_t qrb_linear_backward_workspace_size(const qrb_linear_backward_args* a) {
+  if (check_backward(a) != QRB_OK || a->m == 0) return 0;
+  return bwd_layout(*a).total;
+}
+
+int qrb_linear_backward(const qrb_linear_backward_args* a, void* ws, size_t wsb, void* stream) {
+  TRY(check_backward(a));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const size_t es = esize(a->dtype);
+  if (a->dw != nullptr) TRY(check_ptr(a->dw, "dw", a->dtype));
+  if (a->dbias != nullptr) TRY(check_ptr(a->dbias, "dbias", a->dtype));
+  if (a->m == 0) {   // sums over no rows
+    if (a->dw != nullptr) CUDA(cudaMemsetAsync(a->dw, 0, (size_t)a->n * a->k * es, s), "dw = 0");
+    if (a->dbias != nullptr) CUDA(cudaMemsetAsync(a->dbias, 0, (size_t)a->n * es, s), "dbias = 0");
+    return QRB_OK;
+  }
+  TRY(check_ptr(a->dy, "dy", a->dtype));
+  if (a->activation != QRB_ACT_NONE) TRY(check_ptr(a->pre, "pre", a->dtype));
+  if (a->dw != nullptr) TRY(check_ptr(a->x, "x", a->dtype));
+  if (a->dx != nullptr) {
+    TRY(check_ptr(a->w, "w", a->dtype));
+    TRY(check_ptr(a->dx, "dx", a->dtype));
+  }
+  const BwdLayout l = bwd_layout(*a);
+  TRY(check_ws(ws, wsb, l.total));
+  TRY(check_device());
+  char* w8 = static_cast<char*>(ws);
+  const bool half = a->dtype == QRB_F16, dp = makes_dp(*a) && (a->dx != nullptr || a->dw != nullptr);
+  float* sums = a->dbias != nullptr ? reinterpret_cast<float*>(w8 + l.sums) : nullptr;
+  if (dp || sums != nullptr) {
+    void* to = dp ? w8 + l.dp : nullptr;
+    if (a->dtype == QRB_F32) TRY(run_dp<float>(*a, to, sums, s));
+    else if (half) TRY(run_dp<__half>(*a, to, sums, s));
+    else TRY(run_dp<__nv_bfloat16>(*a, to, sums, s));
+  }
+  Operand p{};
+  p.pieces = a->dtype == QRB_F32 ? 3 : 1;
+  if (makes_dp(*a)) {
+    p.p = w8 + l.dp;
+    p.ld = pitch_of(a->n);
+    p.plane = a->m * p.ld;
+  } else {
+    p.p = a->dy;
+    p.ld = a->lddy;
+  }
+  float* part = reinterpret_cast<float*>(w8 + l.part);
+  Epilogue e{};
+  e.dtype = a->dtype;
+  e.ldy = a->k;
+  if (a->dx != nullptr) {
+    Operand w;
+    TRY(operand(w, a->dtype, a->w, a->ldw, a->n, a->k, true, w8 + l.w, s));
+    p.mn_major = 0;
+    e.y = a->dx;
+    CUDA(qrb::gemm::multiply(p, w, a->m, a->k, a->n, half, e, part, s), "linear dx launch");
+  }
+  if (a->dw != nullptr) {
+    Operand x;
+    TRY(operand(x, a->dtype, a->x, a->ldx, a->m, a->k, true, w8 + l.x, s));
+    p.mn_major = 1;
+    e.y = a->dw;
+    CUDA(qrb::gemm::multiply(p, x, a->n, a->k, a->m, half, e, part, s), "linear dw launch");
+  }
+  return QRB_OK;
+}
+
+}  // extern "C"

@@ -11,6 +11,7 @@ Sequence operators that share QR's compact-WY products:
 
 * ``gated_delta_rule(q, k, v, g, beta) -> (o, final_state)``, ``gated_delta_rule_backward`` and
   ``gated_delta_step`` (one token per row)
+* ``linear(x, w, bias, activation=..., residual=...) -> y`` and ``linear_backward``
 
 The ops (and with them ``libqrb200.so``) load on first attribute access, so that
 ``qr_b200.inputs`` -- the seeded input generators -- can be imported by code that
@@ -22,9 +23,10 @@ import importlib
 
 _OPS = ("custom_kernel", "form_q", "geqrf", "orgqr", "qr", "qr_host")
 _DELTA = ("gated_delta_rule", "gated_delta_rule_backward", "gated_delta_step")
+_LINEAR = ("linear", "linear_backward")
 _LIB = ("QRBError", "lib")
 
-__all__ = [*_OPS, *_DELTA, *_LIB]
+__all__ = [*_OPS, *_DELTA, *_LINEAR, *_LIB]
 
 
 def __getattr__(name: str):
@@ -32,6 +34,8 @@ def __getattr__(name: str):
         return getattr(importlib.import_module(".ops", __name__), name)
     if name in _DELTA:
         return getattr(importlib.import_module(".delta", __name__), name)
+    if name in _LINEAR:
+        return getattr(importlib.import_module("._linear", __name__), name)
     if name in _LIB:
         return getattr(importlib.import_module("._lib", __name__), name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -56,4 +56,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("geqrf", &geqrf, "(H, tau) = geqrf(A) for a checked, contiguous (batch, n, n) float32 CUDA tensor");
   m.def("qr", &qr, "(H, tau, Q) for a checked, contiguous (batch, n, n) float32 CUDA tensor");
   qrb_entry::bind_delta(m);
+  qrb_entry::bind_linear(m);
 }

@@ -18,5 +18,6 @@ inline void check_status(int status) {
 }
 
 void bind_delta(pybind11::module_& m);
+void bind_linear(pybind11::module_& m);
 
 }  // namespace qrb_entry

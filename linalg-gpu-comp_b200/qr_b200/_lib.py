@@ -46,6 +46,10 @@ SIGNATURES.update({
     "qrb_delta_forward": (ctypes.c_int, [_vp, _vp, _c_size, _vp]),
     "qrb_delta_backward": (ctypes.c_int, [_vp, _vp, _c_size, _vp]),
     "qrb_delta_step": (ctypes.c_int, [_vp, _vp]),
+    "qrb_linear_workspace_size": (_c_size, [_vp]),
+    "qrb_linear_forward": (ctypes.c_int, [_vp, _vp, _c_size, _vp]),
+    "qrb_linear_backward_workspace_size": (_c_size, [_vp]),
+    "qrb_linear_backward": (ctypes.c_int, [_vp, _vp, _c_size, _vp]),
 })
 
 _lock = threading.Lock()
