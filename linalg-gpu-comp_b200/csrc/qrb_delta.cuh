@@ -74,10 +74,10 @@ struct Params {
   int zero_tail, backward;         // zero the rows behind the last sequence
   // workspace, per chunk slot and head
   unsigned char *kt, *qt, *xt, *pt, *s0p, *dsp, *ep, *dup;
+  unsigned char *vt, *dot;         // v, dO: kChunk x 128 tiles, zero behind the sequence and dv
   float* gates;                    // gamma[64], tail[64], beta[64]
   double* gsum;                    // G[64]
-  // backward, per chunk slot, head and tile: o.do, v.dv and e.du of 64 tokens in two halves, and
-  // <S', dS'> in eight parts
+  // backward, per chunk slot, head and tile: o.do, v.dv and e.du of 64 tokens, <S', dS'> in four parts
   float *odo, *vdv, *edu, *sds;
   float* s_last;                   // backward: every sequence's final state
 };
@@ -120,6 +120,17 @@ __host__ __device__ constexpr int tile_bytes(int rows, int pieces, int cols) {
 // Byte offset of (row, col) in a tile of `rows` rows.
 __device__ __forceinline__ uint32_t tile_off(int rows, int row, int col) {
   return (uint32_t)((col >> 6) * rows * 128 + row * 128 + ((((col >> 3) ^ row) & 7) << 4) + ((col & 7) << 1));
+}
+
+// The same for the tiles the recurrences leave behind (32 value columns as rows): 16-byte units of a
+// row lie one tile column apart, so that a warp whose lanes own the rows writes 512 contiguous bytes,
+// and ldmatrix still reads eight rows of a unit as 128 contiguous ones.
+__device__ __forceinline__ uint32_t unit_off(int rows, int row, int col) {
+  return (uint32_t)((col >> 3) * rows * 16 + row * 16 + ((col & 7) << 1));
+}
+template <bool U>
+__device__ __forceinline__ uint32_t any_off(int rows, int row, int col) {
+  return U ? unit_off(rows, row, col) : tile_off(rows, row, col);
 }
 
 __device__ __forceinline__ uint32_t pack2(__nv_bfloat16 a, __nv_bfloat16 b) {
@@ -181,11 +192,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 
 // acc (16 x 8 NT) += A[m0 .. m0+15][k0 .. k1) B[k0 .. k1)[n0 .. n0 + 8 NT).
 // AT: A is stored with k along the rows; BT: B is stored with k along the rows (otherwise n).
+// AU / BU: A / B is a tile of the recurrences (unit_off).
 // PA / PB pieces lie apc / bpc columns apart; products of pieces i + j >= PM are dropped
 // (PM is the piece count of the fp32 operands: what is dropped is below their own rounding).
 // One warp; k0, k1 multiples of 16, NT even.  Fragment layout of m16n8k16: lane 4 g + t holds
 // rows g and g + 8, columns 2 t and 2 t + 1 of each 16 x 8 block of acc.
-template <int NT, bool AT, bool BT, int PA, int PB, int PM>
+template <int NT, bool AT, bool BT, int PA, int PB, int PM, bool AU = false, bool BU = false>
 __device__ __forceinline__ void mma_tile(float (&acc)[NT][4], const unsigned char* A, int arows, int apc, int m0,
                                          const unsigned char* B, int brows, int bpc, int n0, int k0, int k1) {
   const int lane = threadIdx.x & 31;
@@ -195,10 +207,10 @@ __device__ __forceinline__ void mma_tile(float (&acc)[NT][4], const unsigned cha
 #pragma unroll
     for (int p = 0; p < PA; ++p) {
       if (AT)
-        ldsm4t(a[p], ab + tile_off(arows, k + (lane & 7) + ((lane >> 4) & 1) * 8,
+        ldsm4t(a[p], ab + any_off<AU>(arows, k + (lane & 7) + ((lane >> 4) & 1) * 8,
                                    p * apc + m0 + ((lane >> 3) & 1) * 8));
       else
-        ldsm4(a[p], ab + tile_off(arows, m0 + (lane & 15), p * apc + k + (lane >> 4) * 8));
+        ldsm4(a[p], ab + any_off<AU>(arows, m0 + (lane & 15), p * apc + k + (lane >> 4) * 8));
     }
 #pragma unroll
     for (int j = 0; j < NT; j += 2) {
@@ -206,9 +218,9 @@ __device__ __forceinline__ void mma_tile(float (&acc)[NT][4], const unsigned cha
       for (int q = 0; q < PB; ++q) {
         uint32_t b[4];
         if (BT)
-          ldsm4t(b, bb + tile_off(brows, k + (lane & 15), q * bpc + n0 + 8 * j + (lane >> 4) * 8));
+          ldsm4t(b, bb + any_off<BU>(brows, k + (lane & 15), q * bpc + n0 + 8 * j + (lane >> 4) * 8));
         else
-          ldsm4(b, bb + tile_off(brows, n0 + 8 * j + (lane & 7) + ((lane >> 4) & 1) * 8,
+          ldsm4(b, bb + any_off<BU>(brows, n0 + 8 * j + (lane & 7) + ((lane >> 4) & 1) * 8,
                                  q * bpc + k + ((lane >> 3) & 1) * 8));
 #pragma unroll
         for (int p = 0; p < PA; ++p) {

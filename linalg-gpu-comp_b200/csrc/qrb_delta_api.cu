@@ -85,7 +85,7 @@ int check_args(const qrb_delta_args* a) {
 }
 
 struct Layout {
-  size_t cstart, kt, qt, xt, pt, gates, gsum, s0p, dsp, ep, dup, odo, vdv, edu, sds, s_last, total;
+  size_t cstart, kt, qt, xt, pt, gates, gsum, s0p, dsp, ep, dup, odo, vdv, edu, sds, s_last, vt, dot, total;
 };
 
 Layout layout(const qrb_delta_args& a, bool backward) {
@@ -105,16 +105,19 @@ Layout layout(const qrb_delta_args& a, bool backward) {
   l.xt = take(n * a.hv * tile_bytes(kChunk, ps, kChunk));
   l.pt = take(n * a.hv * tile_bytes(kChunk, ps, kChunk));
   l.gates = take(n * a.hv * 3 * kChunk * 4);
+  const size_t staged = n * a.hv * ((a.dv + 127) / 128) * kChunk * 128 * (a.dtype == QRB_F32 ? 4 : 2);
+  l.vt = take(staged);
   if (backward) {
+    l.dot = take(staged);
     l.gsum = take(n * a.hv * kChunk * 8);
-    l.s0p = take(n * a.hv * nv * tile_bytes(dkp, ps, kTile));
-    l.dsp = take(n * a.hv * nv * tile_bytes(dkp, ps, kTile));
-    l.ep = take(n * a.hv * nv * tile_bytes(kChunk, ps, kTile));
-    l.dup = take(n * a.hv * nv * tile_bytes(kChunk, ps, kTile));
-    l.odo = take(n * a.hv * nv * 2 * kChunk * 4);
-    l.vdv = take(n * a.hv * nv * 2 * kChunk * 4);
-    l.edu = take(n * a.hv * nv * 2 * kChunk * 4);
-    l.sds = take(n * a.hv * nv * 8 * 4);
+    l.s0p = take(n * a.hv * nv * tile_bytes(kTile, ps, dkp));
+    l.dsp = take(n * a.hv * nv * tile_bytes(kTile, ps, dkp));
+    l.ep = take(n * a.hv * nv * tile_bytes(kTile, ps, kChunk));
+    l.dup = take(n * a.hv * nv * tile_bytes(kTile, ps, kChunk));
+    l.odo = take(n * a.hv * nv * kChunk * 4);
+    l.vdv = take(n * a.hv * nv * kChunk * 4);
+    l.edu = take(n * a.hv * nv * kChunk * 4);
+    l.sds = take(n * a.hv * nv * 4 * 4);
     l.s_last = take((size_t)a.nseq * a.hv * a.dk * a.dv * 4);
   }
   l.total = at;
@@ -215,6 +218,8 @@ int run(const qrb_delta_args* a, void* ws, size_t wsb, void* stream, bool backwa
   p.qt = w + l.qt;
   p.xt = w + l.xt;
   p.pt = w + l.pt;
+  p.vt = w + l.vt;
+  p.dot = w + l.dot;
   p.gates = reinterpret_cast<float*>(w + l.gates);
   p.gsum = reinterpret_cast<double*>(w + l.gsum);
   p.s0p = w + l.s0p;

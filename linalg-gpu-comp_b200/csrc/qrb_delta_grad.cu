@@ -19,11 +19,11 @@ struct GLayout {
   static constexpr int P = Pieces<T>::kIn, PS = Pieces<T>::kS;
   static constexpr int kStages = PS == 2 ? 2 : 1;
   static constexpr int kK = tile_bytes(kChunk, P, DKP);
-  static constexpr int kS = tile_bytes(DKP, PS, kTile);
-  static constexpr int kF = tile_bytes(kChunk, PS, kTile);
+  static constexpr int kS = tile_bytes(kTile, PS, DKP);      // S0, dS': value columns as rows
+  static constexpr int kF = tile_bytes(kTile, PS, kChunk);   // e, du: the same
   static constexpr int kD = tile_bytes(kChunk, P, kTile);
   // tiles in the workspace have kBackPieces pieces; the first kS of them are a prefix
-  static constexpr int kWS = tile_bytes(DKP, kBackPieces, kTile), kWF = tile_bytes(kChunk, kBackPieces, kTile);
+  static constexpr int kWS = tile_bytes(kTile, kBackPieces, DKP), kWF = tile_bytes(kTile, kBackPieces, kChunk);
   static constexpr int kOffE = 0, kOffDU = kF, kOffS0 = 2 * kF, kOffDS = kOffS0 + kS;
   static constexpr int kStage = kOffDS + kS;
   static constexpr int kZ = tile_bytes(kChunk, PS, kChunk);
@@ -104,12 +104,12 @@ __global__ void __launch_bounds__(512) grad_kernel(Params p) {
       put2<P>(D, kChunk, kTile, er, ec, x[0], x[1]);
       put2<P>(D, kChunk, kTile, er, ec + 2, x[2], x[3]);
       __syncthreads();
-      mma_tile<NT, false, false, P, PS, PS>(aq, D, kChunk, kTile, m0, S0, DKP, kTile, d0, 0, kTile);
-      mma_tile<NT, false, false, PS, PS, PS>(ay, DU, kChunk, kTile, m0, S0, DKP, kTile, d0, 0, kTile);
-      mma_tile<NT, false, false, PS, PS, PS>(au, E, kChunk, kTile, m0, DS, DKP, kTile, d0, 0, kTile);
+      mma_tile<NT, false, true, P, PS, PS, false, true>(aq, D, kChunk, kTile, m0, S0, kTile, DKP, d0, 0, kTile);
+      mma_tile<NT, true, true, PS, PS, PS, true, true>(ay, DU, kTile, kChunk, m0, S0, kTile, DKP, d0, 0, kTile);
+      mma_tile<NT, true, true, PS, PS, PS, true, true>(au, E, kTile, kChunk, m0, DS, kTile, DKP, d0, 0, kTile);
       if (16 * cq <= m0) {               // Z, N are lower triangular
-        mma_tile<2, false, false, P, PS, PS>(az, D, kChunk, kTile, m0, E, kChunk, kTile, 16 * cq, 0, kTile);
-        mma_tile<2, false, false, PS, PS, PS>(an, DU, kChunk, kTile, m0, E, kChunk, kTile, 16 * cq, 0, kTile);
+        mma_tile<2, false, true, P, PS, PS, false, true>(az, D, kChunk, kTile, m0, E, kTile, kChunk, 16 * cq, 0, kTile);
+        mma_tile<2, true, true, PS, PS, PS, true, true>(an, DU, kTile, kChunk, m0, E, kTile, kChunk, 16 * cq, 0, kTile);
       }
     }
     __syncthreads();                     // tiles consumed: Z and N may overwrite them
@@ -154,14 +154,14 @@ __global__ void __launch_bounds__(512) grad_kernel(Params p) {
       }
     if (warp == 0) {                     // dbeta, dg: two tokens a lane
       float x[2] = {0.f, 0.f}, db[2] = {0.f, 0.f}, sds = 0.f;
-      for (int n = 0; n < 2 * p.nv; ++n)
+      for (int n = 0; n < p.nv; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const size_t i = (at * p.nv * 2 + n) * kChunk + 2 * lane + e;
+          const size_t i = (at * p.nv + n) * kChunk + 2 * lane + e;
           x[e] += p.odo[i] - p.vdv[i];
           db[e] += p.edu[i];
         }
-      for (int i = lane; i < 8 * p.nv; i += 32) sds += p.sds[at * p.nv * 8 + i];
+      for (int i = lane; i < 4 * p.nv; i += 32) sds += p.sds[at * p.nv * 4 + i];
       sds = warp_sum(sds);
       float s = x[0] + x[1];             // suffix sums
 #pragma unroll

@@ -2,7 +2,7 @@
 //
 //   plan_kernel  packed layout: first chunk slot of every sequence (one block, a prefix sum).
 //   prep_kernel  one block per (chunk, value head): the running decays, X and P of the chunk,
-//                and the chunk's q and k as zero-padded operand tiles.  These depend on no state,
+//                and the chunk's q, k, v (and dO) as zero-padded tiles.  These depend on no state,
 //                so all chunks run at once and the sequential kernels are left with products only.
 //
 // X is solved column by column in fp32: thread j owns column j, the rows of M are broadcast
@@ -93,6 +93,25 @@ __device__ void load_rows(unsigned char* tile, const T* x, int64_t row_stride, i
   }
 }
 
+// v or dO of the chunk as kChunk x 128 tiles (one per 128 value columns), zero-padded: what the
+// recurrences then read needs no test of rows, columns or alignment.
+template <typename T>
+__device__ void stage_rows(unsigned char* to, const T* x, int64_t row_stride, int len, int dv, bool vec) {
+  constexpr int V = 16 / sizeof(T);
+  const int nb = (dv + 127) / 128;
+  for (int u = threadIdx.x; u < nb * kChunk * (128 / V); u += blockDim.x) {
+    const int r = (u / (128 / V)) % kChunk, c = (u % (128 / V)) * V, col = u / (kChunk * 128 / V) * 128 + c;
+    alignas(16) T e[V];
+    if (r < len && vec && col + V <= dv) {
+      *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(x + r * row_stride + col);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) e[i] = r < len && col + i < dv ? x[r * row_stride + col + i] : from_f<T>(0.f);
+    }
+    *reinterpret_cast<uint4*>(to + (size_t)u * 16) = *reinterpret_cast<uint4*>(e);
+  }
+}
+
 template <typename T>
 __device__ void zero_rows(const Params& p, int idx, int h) {
   int64_t end = p.offsets[p.nseq];
@@ -137,6 +156,12 @@ __global__ void __launch_bounds__(128) prep_kernel(Params p, int vec) {
   load_rows<DKP, T>(qt, static_cast<const T*>(p.q) + ch.b * p.qs.b + ch.t0 * p.qs.t + hk * p.qs.h, p.qs.t, ch.len,
                     p.dk, vec & 2);
   const size_t sh = slot_head(p, c, h);
+  const size_t vat = sh * ((p.dv + 127) / 128) * kChunk * 128 * sizeof(T);
+  stage_rows<T>(p.vt + vat, static_cast<const T*>(p.v) + ch.b * p.vs.b + ch.t0 * p.vs.t + h * p.vs.h, p.vs.t, ch.len,
+                p.dv, vec & 4);
+  if (p.backward)
+    stage_rows<T>(p.dot + vat, static_cast<const T*>(p.d_o) + ch.b * p.dos.b + ch.t0 * p.dos.t + h * p.dos.h, p.dos.t,
+                  ch.len, p.dv, vec & 8);
   if (warp == 0) {
     // Running sums of g in fp64: differences of far apart sums keep their low bits.
     const int64_t gbase = ch.b * p.gs.b + ch.t0 * p.gs.t + h * p.gs.h;
@@ -241,10 +266,11 @@ template <int DKP, typename T, int PS>
 cudaError_t run_prep(const Params& p, cudaStream_t s) {
   const auto fits = [&](const void* x, const Strides& st) {
     const int64_t v = 16 / (int64_t)sizeof(T);
-    return (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && st.b % v == 0 && st.t % v == 0 && st.h % v == 0 &&
-           p.dk % v == 0;
+    return (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && st.b % v == 0 && st.t % v == 0 && st.h % v == 0;
   };
-  const int vec = (fits(p.k, p.ks) ? 1 : 0) | (fits(p.q, p.qs) ? 2 : 0);
+  const bool dk_ok = p.dk % (16 / (int)sizeof(T)) == 0;
+  const int vec = (dk_ok && fits(p.k, p.ks) ? 1 : 0) | (dk_ok && fits(p.q, p.qs) ? 2 : 0) | (fits(p.v, p.vs) ? 4 : 0) |
+                  (fits(p.d_o, p.dos) ? 8 : 0);
   constexpr int smem = prep_smem<DKP, T, PS>();
   cudaError_t e = allow_smem(prep_kernel<DKP, T, PS>, smem);
   if (e != cudaSuccess) return e;

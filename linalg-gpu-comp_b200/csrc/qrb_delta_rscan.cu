@@ -1,12 +1,14 @@
-// The backward recurrence of the gated delta rule: the state's gradient walks a sequence's
-// chunks from the last to the first (mathematics in qrb_delta.cuh).
+// The backward recurrence of the gated delta rule: the state's gradient walks a sequence's chunks
+// from the last to the first (mathematics in qrb_delta.cuh, data flow in qrb_delta_tc.cuh).
 //
-// As in the forward recurrence a block owns one (sequence, value head, 32-column tile), the
-// gradient's tile stays in accumulators and its pieces in shared memory.  Per chunk: K dS' and
-// P^T dO give du0, X^T (beta du0) gives du, then Q^T (scale gamma dO) and K^T (-gamma dV) give the
-// gradient before the chunk.  dS' and du go to the workspace for the gradients of q and k; the
-// sums over value columns that dbeta and dg are made of are taken here, from fp32 accumulators.
-#include "qrb_delta.cuh"
+// As in the forward recurrence a block owns one (sequence, value head, up to 128 value columns), a
+// thread a quarter of a column of the gradient.  Per chunk, transposed (lane = value column):
+//     K dS' -> du0 = tail (K dS') + P^T dO, F = beta du0 -> X^T F -> du = du0 + X^T F, dV = beta du
+//     -> Q^T (scale gamma dO) + K^T (-gamma dV) -> dS = gamma_last dS' + ...
+// P^T dO and Q^T (...) run in the shadow of the register work.  dS' and du go to the workspace for
+// the gradients of q and k; the sums over value columns that dbeta and dg are made of are taken here,
+// from fp32 values: e.du, v.dV per token and <S', dS'> per chunk.
+#include "qrb_delta_tc.cuh"
 
 namespace qrb {
 namespace delta {
@@ -18,209 +20,270 @@ struct RLayout {
   static constexpr int PG = Pieces<T>::kS;   // pieces of du and dS' the gradient kernel reads
   static constexpr int kK = tile_bytes(kChunk, P, DKP);
   static constexpr int kX = tile_bytes(kChunk, PS, kChunk);
+  static constexpr int kV = kChunk * kLanes * (int)sizeof(T);
   static constexpr int kGates = 3 * kChunk * 4;
-  static constexpr int kOffQ = kK, kOffX = 2 * kK, kOffP = kOffX + kX, kOffG = kOffP + kX;
-  static constexpr int kStage = kOffG + 1024;
-  static constexpr int kS = tile_bytes(DKP, PS, kTile);
-  static constexpr int kF = tile_bytes(kChunk, PS, kTile);
-  static constexpr int kD = tile_bytes(kChunk, P, kTile);
-  static constexpr int kStages = 2 * kStage + kS + kD + 2 * kF <= 232448 ? 2 : 1;
-  // beta du0 is consumed before -gamma dV is written, behind one more barrier: they share a tile
-  static constexpr int kOffS = kStages * kStage, kOffD = kOffS + kS, kOffDS = kOffD + kD, kOffF = kOffDS + kF;
-  static constexpr int kBytes = kOffF + kF;
-  static_assert(kBytes <= 232448, "shared memory of one block");
+  static constexpr int kOffQ = kK, kOffX = 2 * kK, kOffP = kOffX + kX, kOffV = kOffP + kX, kOffD = kOffV + kV;
+  static constexpr int kStage = kOffD + kV;
+  static constexpr int kStages = 2 * (kStage + kGates) + 256 + 1024 <= kSmemLimit ? 2 : 1;
+  static constexpr int kOffG = kStages * kStage;
+  static constexpr int kBar = kOffG + kStages * kGates;
+  static constexpr int kBytes = kBar + 256 + 1024;
+  static_assert(kBytes <= kSmemLimit, "shared memory of one block");
+  // tensor memory: pieces of dS', then the sum of K^T and Q^T products over them | K dS', then X^T F
+  // | P^T dO | scale gamma dO | dO, then F, then -gamma dV
+  static constexpr uint32_t kSp = PS * (DKP / 2);
+  static constexpr uint32_t tS = 0, tD = 0, tK = kSp > (uint32_t)DKP ? kSp : DKP, tP = tK + 64, tO = tP + 64,
+                            tF = tO + 32 * PS;
+  static_assert(tF + 32 * PS <= 512 && P <= PS, "tensor memory");
 };
 
+struct RBars {
+  uint64_t full[2], sp, dop, ks, pd, f, xf, uw, ds, done, share[4], drain;
+  uint32_t tmem;
+  int abort;
+};
+static_assert(sizeof(RBars) <= 256, "barrier block");
+
 template <int DKP, typename T>
-__global__ void __launch_bounds__(256) rscan_kernel(Params p) {
+__global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_constant__ Params p, int* err) {
   using L = RLayout<DKP, T>;
-  constexpr int P = L::P, PS = L::PS;
-  constexpr int SNT = DKP == 128 ? 4 : 2;
-  extern __shared__ __align__(128) unsigned char sm[];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, tq = lane & 3;
-  const int tile = blockIdx.x % p.nv, sh = blockIdx.x / p.nv, h = sh % p.hv, seq = sh / p.hv;
-  const int hk = h / p.group, n0 = tile * kTile;
-  const int sm0 = DKP == 128 ? 16 * warp : 16 * (warp & 3), sn0 = DKP == 128 ? 0 : 16 * (warp >> 2);
-  const int m0 = 16 * (warp & 3), c0 = 16 * (warp >> 2);
-  unsigned char *S = sm + L::kOffS, *D = sm + L::kOffD, *DS = sm + L::kOffDS, *F = sm + L::kOffF;
+  constexpr int P = L::P, PS = L::PS, PG = L::PG, HK = DKP / kParts;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                                       ~uintptr_t(1023));
+  RBars& bars = *reinterpret_cast<RBars*>(sm + L::kBar);
+  volatile int* abort = &bars.abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int nb = (p.dv + kLanes - 1) / kLanes;
+  const int vb = blockIdx.x % nb, sh = blockIdx.x / nb, h = sh % p.hv, seq = sh / p.hv;
+  const int hk = h / p.group;
+  const int quarters = min(4, (p.dv - vb * kLanes + 31) / 32);
   int64_t b, t0, n;
   seq_range(p, seq, b, t0, n);
   int slot0, nc;
   seq_slots(p, seq, slot0, nc);
 
-  float st[SNT][4];
-  const size_t sbase = ((size_t)seq * p.hv + h) * p.dk * p.dv;
-#pragma unroll
-  for (int j = 0; j < SNT; ++j)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = sm0 + gr + 8 * (r >> 1), col = n0 + sn0 + 8 * j + 2 * tq + (r & 1);
-      st[j][r] = p.ds_end != nullptr && row < p.dk && col < p.dv ? p.ds_end[sbase + (size_t)row * p.dv + col] : 0.f;
-    }
-  auto put_state = [&] {
-#pragma unroll
-    for (int j = 0; j < SNT; ++j)
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-        put2<PS>(S, DKP, kTile, sm0 + gr + 8 * r, sn0 + 8 * j + 2 * tq, st[j][2 * r], st[j][2 * r + 1]);
-  };
-  auto load = [&](int c, int stage) {
-    unsigned char* d = sm + stage * L::kStage;
-    const size_t qk = ((size_t)(slot0 + c) * p.hk + hk) * L::kK, at = slot_head(p, slot0 + c, h);
-    cp_tile(d, p.kt + qk, L::kK);
-    cp_tile(d + L::kOffQ, p.qt + qk, L::kK);
-    cp_tile(d + L::kOffX, p.xt + at * L::kX, L::kX);
-    cp_tile(d + L::kOffP, p.pt + at * L::kX, L::kX);
-    cp_tile(d + L::kOffG, reinterpret_cast<const unsigned char*>(p.gates + at * 3 * kChunk), L::kGates);
-    cp_commit();
-  };
-  put_state();
-  if (L::kStages == 2 && nc > 0) load(nc - 1, (nc - 1) & 1);
-  for (int c = nc - 1; c >= 0; --c) {
-    const int stage = L::kStages == 2 ? (c & 1) : 0;
-    unsigned char* d = sm + stage * L::kStage;
-    const float* gates = reinterpret_cast<const float*>(d + L::kOffG);
-    const int64_t left = n - (int64_t)c * kChunk;
-    const int len = left < kChunk ? (int)left : kChunk;
-    const int64_t tok = t0 + (int64_t)c * kChunk;
-    float v[2][4];
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = m0 + gr + 8 * (r >> 1), col = n0 + c0 + 8 * j + 2 * tq + (r & 1);
-        v[j][r] = row < len && col < p.dv
-                      ? to_f(static_cast<const T*>(p.d_o)[b * p.dos.b + (tok + row) * p.dos.t + h * p.dos.h + col])
-                      : 0.f;
-      }
-    if (L::kStages == 2) {
-      cp_wait_all();
-      __syncthreads();
-      if (c > 0) load(c - 1, stage ^ 1);
-    } else {
-      __syncthreads();
-      load(c, 0);
-      cp_wait_all();
-      __syncthreads();
-    }
-    const size_t at = slot_head(p, slot0 + c, h) * p.nv + tile;
-    {
-      unsigned char* to = p.dsp + at * L::kS;
-      for (int i = tid * 16; i < tile_bytes(DKP, L::PG, kTile); i += 256 * 16)
-        *reinterpret_cast<uint4*>(to + i) = *reinterpret_cast<const uint4*>(S + i);
-    }
-    // <S', dS'>: S' is the next chunk's first state, behind the last chunk the final state
-    float sds = 0.f;
-    {
-      const unsigned char* nx = c + 1 < nc ? p.s0p + (slot_head(p, slot0 + c + 1, h) * p.nv + tile) * L::kS : nullptr;
-#pragma unroll
-      for (int j = 0; j < SNT; ++j)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int row = sm0 + gr + 8 * r, col = sn0 + 8 * j + 2 * tq;
-          float2 x = make_float2(0.f, 0.f);
-          if (nx != nullptr) {
-            x = get2<PS>(nx, DKP, kTile, row, col);
-          } else if (row < p.dk) {
-            const float* y = p.s_last + sbase + (size_t)row * p.dv + n0 + col;
-            if (n0 + col < p.dv) x.x = y[0];
-            if (n0 + col + 1 < p.dv) x.y = y[1];
-          }
-          sds += x.x * st[j][2 * r] + x.y * st[j][2 * r + 1];
-        }
-    }
-    float gam[2], tail[2], bet[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int i = m0 + gr + 8 * r;
-      gam[r] = gates[i];
-      tail[r] = gates[kChunk + i];
-      bet[r] = gates[2 * kChunk + i];
-    }
-    const float glast = gates[kChunk - 1];
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = m0 + gr + 8 * r, col = c0 + 8 * j + 2 * tq;
-        put2<P>(D, kChunk, kTile, row, col, v[j][2 * r], v[j][2 * r + 1]);
-        const float sg = p.scale * gam[r];
-        put2<PS>(DS, kChunk, kTile, row, col, sg * v[j][2 * r], sg * v[j][2 * r + 1]);
-      }
-    float u[2][4];
-    zero(u);
-    mma_tile<2, false, true, P, PS, PS>(u, d, kChunk, DKP, m0, S, DKP, kTile, c0, 0, DKP);
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) u[j][r] *= tail[r >> 1];
-    __syncthreads();
-    // P^T and X^T are upper triangular: nothing left of this warp's rows
-    mma_tile<2, true, true, PS, P, PS>(u, d + L::kOffP, kChunk, kChunk, m0, D, kChunk, kTile, c0, m0, kChunk);
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-        put2<PS>(F, kChunk, kTile, m0 + gr + 8 * r, c0 + 8 * j + 2 * tq, bet[r] * u[j][2 * r],
-                 bet[r] * u[j][2 * r + 1]);
-    __syncthreads();
-    mma_tile<2, true, true, PS, PS, PS>(u, d + L::kOffX, kChunk, kChunk, m0, F, kChunk, kTile, c0, m0, kChunk);
-    __syncthreads();   // F is read before it is written again
-    float vdv[2] = {0.f, 0.f}, edu[2] = {0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = m0 + gr + 8 * r, col = c0 + 8 * j + 2 * tq;
-        put2<L::PG>(p.dup + at * L::kF, kChunk, kTile, row, col, u[j][2 * r], u[j][2 * r + 1]);
-        const float2 e = get2<PS>(p.ep + at * L::kF, kChunk, kTile, row, col);
-        edu[r] += e.x * u[j][2 * r] + e.y * u[j][2 * r + 1];
-        const float y0 = bet[r] * u[j][2 * r], y1 = bet[r] * u[j][2 * r + 1];
-        put2<PS>(F, kChunk, kTile, row, col, -gam[r] * y0, -gam[r] * y1);
-        if (row < len) {
-          T* dv = static_cast<T*>(p.dv_) + ((b * p.time + tok + row) * p.hv + h) * p.dv + n0 + col;
-          const T* vv = static_cast<const T*>(p.v) + b * p.vs.b + (tok + row) * p.vs.t + h * p.vs.h + n0 + col;
-          if (n0 + col < p.dv) {
-            dv[0] = from_f<T>(y0);
-            vdv[r] += to_f(vv[0]) * y0;
-          }
-          if (n0 + col + 1 < p.dv) {
-            dv[1] = from_f<T>(y1);
-            vdv[r] += to_f(vv[1]) * y1;
-          }
-        }
-      }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        vdv[r] += __shfl_xor_sync(0xffffffffu, vdv[r], o);
-        edu[r] += __shfl_xor_sync(0xffffffffu, edu[r], o);
-      }
-      if (tq == 0) {
-        p.vdv[(at * 2 + (warp >> 2)) * kChunk + m0 + gr + 8 * r] = vdv[r];
-        p.edu[(at * 2 + (warp >> 2)) * kChunk + m0 + gr + 8 * r] = edu[r];
-      }
-    }
-    sds = warp_sum(sds);
-    if (lane == 0) p.sds[at * 8 + warp] = sds;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < SNT; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) st[j][r] *= glast;
-    mma_tile<SNT, true, true, P, PS, PS>(st, d + L::kOffQ, kChunk, DKP, sm0, DS, kChunk, kTile, sn0, 0, kChunk);
-    mma_tile<SNT, true, true, P, PS, PS>(st, d, kChunk, DKP, sm0, F, kChunk, kTile, sn0, 0, kChunk);
-    put_state();
+  if (tid == 0) {
+    mbar_init(&bars.full[0], 1);
+    mbar_init(&bars.full[1], 1);
+    for (uint64_t* x : {&bars.ks, &bars.pd, &bars.xf, &bars.ds, &bars.drain}) mbar_init(x, 1);
+    for (uint64_t* x : {&bars.sp, &bars.dop, &bars.f, &bars.uw, &bars.done}) mbar_init(x, kParts * quarters);
+    for (int i = 0; i < 4; ++i) mbar_init(&bars.share[i], kParts);
+    bars.abort = 0;
+    fence_mbar_init();
   }
-  if (p.ds_init != nullptr) {
-#pragma unroll
-    for (int j = 0; j < SNT; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = sm0 + gr + 8 * (r >> 1), col = n0 + sn0 + 8 * j + 2 * tq + (r & 1);
-        if (row < p.dk && col < p.dv) p.ds_init[sbase + (size_t)row * p.dv + col] = st[j][r];
+  if (warp == 0) tmem_alloc(&bars.tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+  const int q = warp & 3, part = warp >> 2;
+
+  if (q < quarters) {
+    // ---- loads and MMAs: warp 0 waits, its first lane issues; step i handles chunk nc - 1 - i ----
+    int loaded = 0;
+    auto load = [&] {
+      const int i = loaded++;
+      if (lane != 0) return;
+      unsigned char* d = sm + (i % L::kStages) * L::kStage;
+      uint64_t* bar = &bars.full[i % L::kStages];
+      const int c = nc - 1 - i;
+      const size_t qk = ((size_t)(slot0 + c) * p.hk + hk) * L::kK, at = slot_head(p, slot0 + c, h);
+      mbar_arrive_expect_tx(bar, L::kStage + L::kGates);
+      bulk_load(d, p.kt + qk, L::kK, bar);
+      bulk_load(d + L::kOffQ, p.qt + qk, L::kK, bar);
+      bulk_load(d + L::kOffX, p.xt + at * L::kX, L::kX, bar);
+      bulk_load(d + L::kOffP, p.pt + at * L::kX, L::kX, bar);
+      bulk_load(d + L::kOffV, p.vt + (at * nb + vb) * L::kV, L::kV, bar);
+      bulk_load(d + L::kOffD, p.dot + (at * nb + vb) * L::kV, L::kV, bar);
+      bulk_load(sm + L::kOffG + (i % L::kStages) * L::kGates, p.gates + at * 3 * kChunk, L::kGates, bar);
+    };
+    auto tiles = [&](int i) { return smem_u32(sm + (i % L::kStages) * L::kStage); };
+    auto issue_ks = [&](int i) {   // K dS', once all pieces of the gradient are in place
+      if (!warp_wait(&bars.full[i % L::kStages], (i / L::kStages) & 1, abort, err, 72) ||
+          !warp_wait(&bars.sp, i & 1, abort, err, 73))
+        return;
+      tc_fence_after();
+      if (lane == 0) {
+        mma_pieces<64, DKP, false, PS, P, PS>(tmem + L::tK, tmem + L::tS, DKP / 2, tiles(i), 0);
+        mma_commit(&bars.ks);
       }
+      __syncwarp();
+    };
+    const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
+    const int lcol = 32 * q + lane, col = vb * kLanes + lcol;
+    const int tile = vb * 4 + q;
+    const int tb = kTok * part, kb = HK * part;
+    const bool on = col < p.dv;
+    const size_t sbase = ((size_t)seq * p.hv + h) * p.dk * p.dv;
+    const size_t scol = sbase + (size_t)kb * p.dv + min(col, p.dv - 1);
+    constexpr int kWS = tile_bytes(kTile, PS, DKP), kWF = tile_bytes(kTile, PS, kChunk);
+    float st[HK];
+    if (p.ds_end != nullptr)
+      load_column(p.ds_end + scol, p.dv, p.dk - kb, on, st);
+    else
+#pragma unroll
+      for (int j = 0; j < HK; ++j) st[j] = 0.f;
+    // pieces of dS' for the products, the first PG of them for the gradient kernel too
+    auto put_state = [&](int c) {
+      uint32_t w[PS][HK / 2], g[PG][HK / 2];
+      put_pieces<PS, HK>(tl + L::tS + kb / 2, DKP / 2, st, w);
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&bars.sp);
+#pragma unroll
+      for (int a = 0; a < PG; ++a)
+#pragma unroll
+        for (int i = 0; i < HK / 2; ++i) g[a][i] = w[a][i];
+      keep_pieces<PG>(p.dsp + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWS, lane, DKP, kb, g);
+    };
+    if (nc > 0) {
+      if (warp == 0)
+        while (loaded < nc && loaded < L::kStages) load();
+      put_state(nc - 1);
+      if (warp == 0) issue_ks(0);
+    }
+    for (int i = 0; i < nc; ++i) {
+      const uint32_t ph = i & 1;
+      const int c = nc - 1 - i;
+      const size_t at = slot_head(p, slot0 + c, h) * p.nv + tile;
+      const unsigned char* stage = sm + (i % L::kStages) * L::kStage;
+      const Gates gates(sm + L::kOffG + (i % L::kStages) * L::kGates, tb);
+      float x[kTok], u[kTok];
+      if (!warp_wait(&bars.full[i % L::kStages], (i / L::kStages) & 1, abort, err, 81)) break;
+      staged<T>(stage + L::kOffD, tb, lcol, x);
+      put_pieces<P, kTok>(tl + L::tF + tb / 2, 32, x);
+      with_tokens(gates.gam, [&](int j, float g) { x[j] *= p.scale * g; });
+      put_pieces<PS, kTok>(tl + L::tO + tb / 2, 32, x);
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&bars.dop);
+      if (warp == 0) {
+        if (!warp_wait(&bars.dop, ph, abort, err, 75)) break;
+        tc_fence_after();
+        if (lane == 0) {
+          mma_pieces<64, 64, true, P, PS, PS>(tmem + L::tP, tmem + L::tF, 32, tiles(i) + L::kOffP, 0);
+          mma_commit(&bars.pd);
+        }
+        __syncwarp();
+      }
+      {
+        // <S', dS'>: S' is the next chunk's first state, behind the last chunk the final state
+        float y[HK], sds = 0.f;
+        if (c + 1 < nc)
+          fetch_pieces<PS, HK>(p.s0p + (slot_head(p, slot0 + c + 1, h) * p.nv + tile) * kWS, lane, DKP, kb, y);
+        else
+          load_column(p.s_last + scol, p.dv, p.dk - kb, on, y);
+#pragma unroll
+        for (int a = 0; a < HK; ++a) sds += y[a] * st[a];
+        sds = warp_sum(sds);
+        if (lane == 0) p.sds[at * kParts + part] = sds;
+      }
+      if (!warp_wait(&bars.ks, ph, abort, err, 82)) break;
+      tc_fence_after();
+      ld_cols(tl + L::tK + tb, u);
+      with_tokens(gates.tail, [&](int j, float g) { u[j] *= g; });
+      if (!warp_wait(&bars.pd, ph, abort, err, 83)) break;
+      tc_fence_after();
+      ld_cols(tl + L::tP + tb, x);
+#pragma unroll
+      for (int j = 0; j < kTok; ++j) u[j] += x[j];
+      with_tokens(gates.bet, [&](int j, float g) { x[j] = g * u[j]; });
+      put_pieces<PS, kTok>(tl + L::tF + tb / 2, 32, x);
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&bars.f);
+      if (warp == 0) {
+        if (!warp_wait(&bars.f, ph, abort, err, 76)) break;
+        tc_fence_after();
+        if (lane == 0) {
+          mma_pieces<64, 64, true, PS, PS, PS>(tmem + L::tK, tmem + L::tF, 32, tiles(i) + L::kOffX, 0);
+          mma_commit(&bars.xf);
+          mma_pieces<DKP, 64, true, PS, P, PS>(tmem + L::tD, tmem + L::tO, 32, tiles(i) + L::kOffQ, 0);
+        }
+        __syncwarp();
+      }
+      if (!warp_wait(&bars.xf, ph, abort, err, 84)) break;
+      tc_fence_after();
+      ld_cols(tl + L::tK + tb, x);
+#pragma unroll
+      for (int j = 0; j < kTok; ++j) u[j] += x[j];
+      float y[kTok];   // dV
+      with_tokens(gates.bet, [&](int j, float g) { y[j] = g * u[j]; });
+      with_tokens(gates.gam, [&](int j, float g) { x[j] = -g * y[j]; });
+      put_pieces<PS, kTok>(tl + L::tF + tb / 2, 32, x);
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&bars.uw);
+      if (warp == 0) {
+        if (!warp_wait(&bars.uw, ph, abort, err, 77)) break;
+        tc_fence_after();
+        if (lane == 0) {
+          mma_pieces<DKP, 64, true, PS, P, PS>(tmem + L::tD, tmem + L::tF, 32, tiles(i), 1);
+          mma_commit(&bars.ds);
+        }
+        __syncwarp();
+      }
+      const float glast = *gates.last;
+      {
+        uint32_t g[PG][kTok / 2];
+        split_all<PG, kTok>(u, g);
+        keep_pieces<PG>(p.dup + at * kWF, lane, kChunk, tb, g);
+        fetch_pieces<PS, kTok>(p.ep + at * kWF, lane, kChunk, tb, x);
+#pragma unroll
+        for (int j = 0; j < kTok; ++j) x[j] *= u[j];
+        const float s = sum_columns(x);
+        if ((lane & 1) == 0) p.edu[at * kChunk + tb + lane / 2] = s;
+      }
+      {
+        staged<T>(stage + L::kOffV, tb, lcol, x);
+#pragma unroll
+        for (int j = 0; j < kTok; ++j) x[j] *= y[j];
+        const float s = sum_columns(x);
+        if ((lane & 1) == 0) p.vdv[at * kChunk + tb + lane / 2] = s;
+        const int64_t tok = (int64_t)c * kChunk + tb;
+        if (on)
+          store_tokens(static_cast<T*>(p.dv_) + ((b * p.time + t0 + tok) * p.hv + h) * p.dv + col,
+                       (int64_t)p.hv * p.dv, (int)min(n - tok, (int64_t)kTok), y);
+      }
+      fence_proxy_async();   // what this stage held is read before bulk copies may replace it
+      if (!warp_wait(&bars.ds, ph, abort, err, 85)) break;
+      tc_fence_after();
+      {
+        float d[HK];
+        ld_cols(tl + L::tD + kb, d);
+#pragma unroll
+        for (int a = 0; a < HK; ++a) st[a] = glast * st[a] + d[a];
+      }
+      tc_fence_before();
+      warp_arrive(&bars.done);
+      if (i + 1 < nc) {
+        warp_arrive(&bars.share[q]);   // the other quarters' columns are read before pieces go over them
+        if (!warp_wait(&bars.share[q], ph, abort, err, 86)) break;
+        tc_fence_after();
+        put_state(c - 1);
+        if (warp == 0) {
+          if (!warp_wait(&bars.done, ph, abort, err, 74)) break;
+          if (loaded < nc) load();
+          issue_ks(i + 1);
+        }
+      }
+    }
+    if (*abort && warp == 0 && lane == 0) {
+      // loads in flight must land, MMAs in flight end, before the block's memory goes
+      for (int s = 0; s < L::kStages; ++s)
+        if (loaded > s) mbar_wait(&bars.full[s], ((loaded - 1 - s) / L::kStages) & 1, 1u << 22);
+      mma_commit(&bars.drain);
+      mbar_wait(&bars.drain, 0, 1u << 22);
+    }
+    if (p.ds_init != nullptr && on && !*abort)
+      store_column(p.ds_init + sbase + (size_t)kb * p.dv + col, p.dv, p.dk - kb, st);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -228,10 +291,13 @@ template <int DKP, typename T>
 cudaError_t run_rscan(const Params& p, cudaStream_t s) {
   constexpr int smem = RLayout<DKP, T>::kBytes;
   const double rows = (double)p.bound * kChunk * p.hv;
+  int* err = device_error_flag();
+  if (err == nullptr) return cudaErrorInvalidValue;
   LaunchTimer t("delta_rscan_kernel", s, rows * 2.0 * p.dv * sizeof(T), rows * 6.0 * p.dk * p.dv);
   cudaError_t e = allow_smem(rscan_kernel<DKP, T>, smem);
   if (e != cudaSuccess) return e;
-  rscan_kernel<DKP, T><<<(unsigned)p.nseq * p.hv * p.nv, 256, smem, s>>>(p);
+  const unsigned grid = (unsigned)p.nseq * p.hv * ((p.dv + kLanes - 1) / kLanes);
+  rscan_kernel<DKP, T><<<grid, kTcThreads, smem, s>>>(p, err);
   return cudaGetLastError();
 }
 

@@ -1,210 +1,295 @@
-// The forward recurrence of the gated delta rule over the chunks of one sequence
-// (mathematics in qrb_delta.cuh).
+// The forward recurrence of the gated delta rule over the chunks of one sequence (mathematics in
+// qrb_delta.cuh, data flow in qrb_delta_tc.cuh).
 //
-// The columns of the state evolve independently, so a block owns one (sequence, value head,
-// 32-column tile) and walks its chunks: the state tile stays in the accumulators of the last
-// product for the whole sequence, and its pieces in shared memory.  Per chunk three dependent
-// products, K S0, X F and K^T U, with two block barriers between them; the output's products
-// Q S0 (sharing the fragments of S0) and P U fill the tensor pipe beside them.  The operand
-// tiles of the next chunk arrive by cp.async meanwhile.  32 columns: a narrower tile repeats
-// the loads of K, Q, X, P more often, a wider one leaves too few blocks for a single sequence.
-#include "qrb_delta.cuh"
+// The columns of the state evolve independently: a block owns one (sequence, value head, up to 128
+// value columns) and walks its chunks.  Four threads share a column, each with a quarter of its state
+// in fp32 registers for the whole sequence.  Per chunk, all transposed (lane = value column):
+//     K S0 -> e0 = v - gamma (K S0), F = beta e0 -> X F -> e = e0 + X F, u = beta e, W = tail u
+//     -> K^T W -> S = gamma_last S + K^T W -> pieces of S for the next chunk,
+// a chain of three products with register work between them.  Q S0 and P u, which o is made of, run
+// in the shadow of that work (the first is scaled in place and the second added to it), and o is stored
+// in the shadow of the next chunk's K S0.  Sixteen warps, because the register work between two
+// products is bound by latency; the first thread also loads the chunk tiles by bulk copies (two chunks
+// in flight where they fit) and issues the MMAs.
+#include "qrb_delta_tc.cuh"
 
 namespace qrb {
 namespace delta {
 namespace {
 
-template <int DKP, typename T, int PS>
+template <int DKP, typename T, int PS, bool STORE>
 struct ScanLayout {
   static constexpr int P = Pieces<T>::kIn;
   static constexpr int kK = tile_bytes(kChunk, P, DKP);
   static constexpr int kX = tile_bytes(kChunk, PS, kChunk);
+  static constexpr int kV = kChunk * kLanes * (int)sizeof(T);
   static constexpr int kGates = 3 * kChunk * 4;
-  static constexpr int kOffQ = kK, kOffX = 2 * kK, kOffP = kOffX + kX, kOffG = kOffP + kX;
-  static constexpr int kStage = kOffG + 1024;
-  static constexpr int kS = tile_bytes(DKP, PS, kTile);
-  static constexpr int kF = tile_bytes(kChunk, PS, kTile);
-  // two stages where they fit: not with two- or three-piece q and k of 128 columns
-  static constexpr int kStages = 2 * kStage + kS + 3 * kF <= 232448 ? 2 : 1;
-  static constexpr int kOffS = kStages * kStage, kOffF = kOffS + kS, kOffU = kOffF + kF, kOffT = kOffU + kF;
-  static constexpr int kBytes = kOffT + kF;
-  static_assert(kBytes <= 232448, "shared memory of one block");
+  static constexpr int kOffQ = kK, kOffX = 2 * kK, kOffP = kOffX + kX, kOffV = kOffP + kX, kOffD = kOffV + kV;
+  static constexpr int kStage = kOffD + (STORE ? kV : 0);   // a multiple of 1024; gates apart
+  static constexpr int kStages = 2 * (kStage + kGates) + 256 + 1024 <= kSmemLimit ? 2 : 1;
+  static constexpr int kOffG = kStages * kStage;
+  static constexpr int kBar = kOffG + kStages * kGates;
+  static constexpr int kBytes = kBar + 256 + 1024;   // 1024: alignment
+  static_assert(kBytes <= kSmemLimit, "shared memory of one block");
+  // tensor memory columns: pieces of S | K^T W | K S0, then X F | Q S0, then P u | F, then W | U.
+  // Three pieces: K^T W lies over the pieces of S (read by then), rewritten behind a barrier of the
+  // warps that share lanes.
+  static constexpr uint32_t kSp = PS * (DKP / 2);
+  static constexpr bool kOver = PS == 3;
+  static constexpr uint32_t tS = 0, tD = kOver ? 0 : kSp, tK = kOver ? (kSp > (uint32_t)DKP ? kSp : DKP) : kSp + DKP,
+                            tQ = tK + 64, tF = tQ + 64, tU = tF + 32 * PS;
+  static_assert(tU + 32 * PS <= 512, "tensor memory");
 };
 
-// STORE: for a backward pass, keep the chunk's first state, e and the sums o.do instead of o.
+struct ScanBars {
+  uint64_t full[2], sp, ks, qs, f, xf, uw, ds, pu, o, share[4], drain;
+  uint32_t tmem;
+  int abort;
+};
+static_assert(sizeof(ScanBars) <= 256, "barrier block");
+
+// STORE: for a backward pass, keep every chunk's first state, e and the sums o.do instead of o.
 template <int DKP, typename T, int PS, bool STORE>
-__global__ void __launch_bounds__(256) scan_kernel(Params p) {
-  using L = ScanLayout<DKP, T, PS>;
-  constexpr int P = L::P;
-  constexpr int SNT = DKP == 128 ? 4 : 2;   // 8-column blocks of the state a warp holds
-  extern __shared__ __align__(128) unsigned char sm[];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, tq = lane & 3;
-  const int tile = blockIdx.x % p.nv, sh = blockIdx.x / p.nv, h = sh % p.hv, seq = sh / p.hv;
-  const int hk = h / p.group, n0 = tile * kTile;
-  const int sm0 = DKP == 128 ? 16 * warp : 16 * (warp & 3), sn0 = DKP == 128 ? 0 : 16 * (warp >> 2);
-  const int m0 = 16 * (warp & 3), c0 = 16 * (warp >> 2);   // token rows, value columns of the other products
-  unsigned char *S = sm + L::kOffS, *F = sm + L::kOffF, *U = sm + L::kOffU, *W = sm + L::kOffT;
+__global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_constant__ Params p, int* err) {
+  using L = ScanLayout<DKP, T, PS, STORE>;
+  constexpr int P = L::P, HK = DKP / kParts;   // HK: state rows of one thread
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                                       ~uintptr_t(1023));
+  ScanBars& bars = *reinterpret_cast<ScanBars*>(sm + L::kBar);
+  volatile int* abort = &bars.abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int nb = (p.dv + kLanes - 1) / kLanes;
+  const int vb = blockIdx.x % nb, sh = blockIdx.x / nb, h = sh % p.hv, seq = sh / p.hv;
+  const int hk = h / p.group;
+  const int quarters = min(4, (p.dv - vb * kLanes + 31) / 32);   // 32-column groups that hold columns
   int64_t b, t0, n;
   seq_range(p, seq, b, t0, n);
   int slot0, nc;
   seq_slots(p, seq, slot0, nc);
 
-  float st[SNT][4];
-  const size_t sbase = ((size_t)seq * p.hv + h) * p.dk * p.dv;
-#pragma unroll
-  for (int j = 0; j < SNT; ++j)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = sm0 + gr + 8 * (r >> 1), col = n0 + sn0 + 8 * j + 2 * tq + (r & 1);
-      st[j][r] = p.s_init != nullptr && row < p.dk && col < p.dv ? p.s_init[sbase + (size_t)row * p.dv + col] : 0.f;
-    }
-  auto put_state = [&] {
-#pragma unroll
-    for (int j = 0; j < SNT; ++j)
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-        put2<PS>(S, DKP, kTile, sm0 + gr + 8 * r, sn0 + 8 * j + 2 * tq, st[j][2 * r], st[j][2 * r + 1]);
-  };
-  auto load = [&](int c, int stage) {
-    unsigned char* d = sm + stage * L::kStage;
-    const size_t qk = ((size_t)(slot0 + c) * p.hk + hk) * L::kK, at = slot_head(p, slot0 + c, h);
-    cp_tile(d, p.kt + qk, L::kK);
-    cp_tile(d + L::kOffQ, p.qt + qk, L::kK);
-    cp_tile(d + L::kOffX, p.xt + at * L::kX, L::kX);
-    cp_tile(d + L::kOffP, p.pt + at * L::kX, L::kX);
-    cp_tile(d + L::kOffG, reinterpret_cast<const unsigned char*>(p.gates + at * 3 * kChunk), L::kGates);
-    cp_commit();
-  };
-  put_state();
-  if (L::kStages == 2 && nc > 0) load(0, 0);
-  for (int c = 0; c < nc; ++c) {
-    const int stage = L::kStages == 2 ? (c & 1) : 0;
-    unsigned char* d = sm + stage * L::kStage;
-    const float* gates = reinterpret_cast<const float*>(d + L::kOffG);
-    const int64_t left = n - (int64_t)c * kChunk;
-    const int len = left < kChunk ? (int)left : kChunk;
-    const int64_t tok = t0 + (int64_t)c * kChunk;
-    // this thread's values: rows m0 + gr (+ 8), columns c0 + 8 j + 2 tq (+ 1)
-    float v[2][4];
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = m0 + gr + 8 * (r >> 1), col = n0 + c0 + 8 * j + 2 * tq + (r & 1);
-        v[j][r] = row < len && col < p.dv
-                      ? to_f(static_cast<const T*>(p.v)[b * p.vs.b + (tok + row) * p.vs.t + h * p.vs.h + col])
-                      : 0.f;
-      }
-    if (L::kStages == 2) {
-      cp_wait_all();
-      __syncthreads();   // this chunk's tiles and the state are in place, the other stage is free
-      if (c + 1 < nc) load(c + 1, stage ^ 1);
-    } else {
-      __syncthreads();
-      load(c, 0);
-      cp_wait_all();
-      __syncthreads();
-    }
-    if (STORE) {
-      unsigned char* to = p.s0p + (slot_head(p, slot0 + c, h) * p.nv + tile) * L::kS;
-      for (int i = tid * 16; i < L::kS; i += 256 * 16)
-        *reinterpret_cast<uint4*>(to + i) = *reinterpret_cast<const uint4*>(S + i);
-    }
-    float e[2][4], o[2][4];
-    zero(e);
-    mma_tile<2, false, true, P, PS, PS>(e, d, kChunk, DKP, m0, S, DKP, kTile, c0, 0, DKP);
-    zero(o);
-    mma_tile<2, false, true, P, PS, PS>(o, d + L::kOffQ, kChunk, DKP, m0, S, DKP, kTile, c0, 0, DKP);
-    float gam[2], tail[2], bet[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int i = m0 + gr + 8 * r;
-      gam[r] = gates[i];
-      tail[r] = gates[kChunk + i];
-      bet[r] = gates[2 * kChunk + i];
-    }
-    const float glast = gates[kChunk - 1];
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        e[j][2 * r] = v[j][2 * r] - gam[r] * e[j][2 * r];
-        e[j][2 * r + 1] = v[j][2 * r + 1] - gam[r] * e[j][2 * r + 1];
-        put2<PS>(F, kChunk, kTile, m0 + gr + 8 * r, c0 + 8 * j + 2 * tq, bet[r] * e[j][2 * r],
-                 bet[r] * e[j][2 * r + 1]);
-      }
-    __syncthreads();
-    // X is lower triangular: nothing right of this warp's rows
-    mma_tile<2, false, true, PS, PS, PS>(e, d + L::kOffX, kChunk, kChunk, m0, F, kChunk, kTile, c0, 0, m0 + 16);
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = m0 + gr + 8 * r, col = c0 + 8 * j + 2 * tq;
-        if (STORE)
-          put2<PS>(p.ep + (slot_head(p, slot0 + c, h) * p.nv + tile) * L::kF, kChunk, kTile, row, col, e[j][2 * r],
-                   e[j][2 * r + 1]);
-        const float u0 = bet[r] * e[j][2 * r], u1 = bet[r] * e[j][2 * r + 1];
-        put2<PS>(U, kChunk, kTile, row, col, u0, u1);
-        put2<PS>(W, kChunk, kTile, row, col, tail[r] * u0, tail[r] * u1);
-      }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < SNT; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) st[j][r] *= glast;
-    mma_tile<SNT, true, true, P, PS, PS>(st, d, kChunk, DKP, sm0, W, kChunk, kTile, sn0, 0, kChunk);
-    put_state();
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) o[j][r] *= p.scale * gam[r >> 1];
-    mma_tile<2, false, true, PS, PS, PS>(o, d + L::kOffP, kChunk, kChunk, m0, U, kChunk, kTile, c0, 0, m0 + 16);
-    float dot[2] = {0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = m0 + gr + 8 * (r >> 1), col = n0 + c0 + 8 * j + 2 * tq + (r & 1);
-        if (row < len && col < p.dv) {
-          if (STORE)
-            dot[r >> 1] += o[j][r] * to_f(static_cast<const T*>(p.d_o)[b * p.dos.b + (tok + row) * p.dos.t +
-                                                                       h * p.dos.h + col]);
-          else
-            static_cast<T*>(p.o)[b * p.os.b + (tok + row) * p.os.t + h * p.os.h + col] = from_f<T>(o[j][r]);
-        }
-      }
-    if (STORE) {   // the two column halves of a row belong to two warps
-      float* sums = p.odo + ((slot_head(p, slot0 + c, h) * p.nv + tile) * 2 + (warp >> 2)) * kChunk;
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], 1);
-        dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], 2);
-        if (tq == 0) sums[m0 + gr + 8 * r] = dot[r];
-      }
-    }
+  if (tid == 0) {
+    mbar_init(&bars.full[0], 1);
+    mbar_init(&bars.full[1], 1);
+    for (uint64_t* x : {&bars.ks, &bars.qs, &bars.xf, &bars.ds, &bars.pu, &bars.drain}) mbar_init(x, 1);
+    for (uint64_t* x : {&bars.sp, &bars.f, &bars.uw, &bars.o}) mbar_init(x, kParts * quarters);
+    for (int i = 0; i < 4; ++i) mbar_init(&bars.share[i], kParts);
+    bars.abort = 0;
+    fence_mbar_init();
   }
-  if (p.s_end != nullptr) {
-#pragma unroll
-    for (int j = 0; j < SNT; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = sm0 + gr + 8 * (r >> 1), col = n0 + sn0 + 8 * j + 2 * tq + (r & 1);
-        if (row < p.dk && col < p.dv) p.s_end[sbase + (size_t)row * p.dv + col] = st[j][r];
+  if (warp == 0) tmem_alloc(&bars.tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+  const int q = warp & 3, part = warp >> 2;
+
+  if (q < quarters) {   // warps without columns have nothing to add
+    // ---- loads and MMAs: warp 0 waits, its first lane issues ----
+    int loaded = 0;
+    auto load = [&] {
+      const int c = loaded++;
+      if (lane != 0) return;
+      unsigned char* d = sm + (c % L::kStages) * L::kStage;
+      uint64_t* bar = &bars.full[c % L::kStages];
+      const size_t qk = ((size_t)(slot0 + c) * p.hk + hk) * L::kK, at = slot_head(p, slot0 + c, h);
+      mbar_arrive_expect_tx(bar, L::kStage + L::kGates);
+      bulk_load(d, p.kt + qk, L::kK, bar);
+      bulk_load(d + L::kOffQ, p.qt + qk, L::kK, bar);
+      bulk_load(d + L::kOffX, p.xt + at * L::kX, L::kX, bar);
+      bulk_load(d + L::kOffP, p.pt + at * L::kX, L::kX, bar);
+      bulk_load(d + L::kOffV, p.vt + (at * nb + vb) * L::kV, L::kV, bar);
+      if (STORE) bulk_load(d + L::kOffD, p.dot + (at * nb + vb) * L::kV, L::kV, bar);
+      bulk_load(sm + L::kOffG + (c % L::kStages) * L::kGates, p.gates + at * 3 * kChunk, L::kGates, bar);
+    };
+    auto tiles = [&](int c) { return smem_u32(sm + (c % L::kStages) * L::kStage); };
+    auto issue_ks = [&](int c) {   // K S0, once all pieces of the state are in place
+      if (!warp_wait(&bars.full[c % L::kStages], (c / L::kStages) & 1, abort, err, 52) ||
+          !warp_wait(&bars.sp, c & 1, abort, err, 53))
+        return;
+      tc_fence_after();
+      if (lane == 0) {
+        mma_pieces<64, DKP, false, PS, P, PS>(tmem + L::tK, tmem + L::tS, DKP / 2, tiles(c), 0);
+        mma_commit(&bars.ks);
       }
+      __syncwarp();
+    };
+    auto issue_qs = [&](int c) {
+      if (lane == 0) {
+        mma_pieces<64, DKP, false, PS, P, PS>(tmem + L::tQ, tmem + L::tS, DKP / 2, tiles(c) + L::kOffQ, 0);
+        mma_commit(&bars.qs);
+      }
+      __syncwarp();
+    };
+    const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
+    const int lcol = 32 * q + lane, col = vb * kLanes + lcol;  // value column in the block, in the head
+    const int tile = vb * 4 + q;                              // its 32-column tile
+    const int tb = kTok * part, kb = HK * part;               // first token, first state row
+    const bool on = col < p.dv;
+    const size_t sbase = ((size_t)seq * p.hv + h) * p.dk * p.dv;
+    constexpr int kWS = tile_bytes(kTile, PS, DKP), kWF = tile_bytes(kTile, PS, kChunk);
+    float st[HK];
+    if (p.s_init != nullptr)
+      load_column(p.s_init + sbase + (size_t)kb * p.dv + min(col, p.dv - 1), p.dv, p.dk - kb, on, st);
+    else
+#pragma unroll
+      for (int j = 0; j < HK; ++j) st[j] = 0.f;
+    auto put_state = [&](int c) {
+      uint32_t w[PS][HK / 2];
+      put_pieces<PS, HK>(tl + L::tS + kb / 2, DKP / 2, st, w);
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&bars.sp);
+      if (STORE) keep_pieces<PS>(p.s0p + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWS, lane, DKP, kb, w);
+    };
+    if (nc > 0) {
+      if (warp == 0)
+        while (loaded < nc && loaded < L::kStages) load();
+      put_state(0);
+      if (warp == 0) {
+        issue_ks(0);
+        issue_qs(0);
+      }
+    }
+    for (int c = 0; c < nc; ++c) {
+      const uint32_t ph = c & 1;
+      const unsigned char* stage = sm + (c % L::kStages) * L::kStage;
+      const Gates gates(sm + L::kOffG + (c % L::kStages) * L::kGates, tb);
+      float e[kTok], x[kTok];
+      if (!warp_wait(&bars.full[c % L::kStages], (c / L::kStages) & 1, abort, err, 61)) break;
+      staged<T>(stage + L::kOffV, tb, lcol, e);
+      if (!warp_wait(&bars.ks, ph, abort, err, 62)) break;
+      tc_fence_after();
+      ld_cols(tl + L::tK + tb, x);
+      with_tokens(gates.gam, [&](int i, float g) { e[i] -= g * x[i]; });
+      with_tokens(gates.bet, [&](int i, float g) { x[i] = g * e[i]; });
+      put_pieces<PS, kTok>(tl + L::tF + tb / 2, 32, x);
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&bars.f);
+      if (warp == 0) {
+        if (!warp_wait(&bars.f, ph, abort, err, 55)) break;
+        tc_fence_after();
+        if (lane == 0) {
+          mma_pieces<64, 64, false, PS, PS, PS>(tmem + L::tK, tmem + L::tF, 32, tiles(c) + L::kOffX, 0);
+          mma_commit(&bars.xf);
+        }
+        __syncwarp();
+      }
+      if (!warp_wait(&bars.qs, ph, abort, err, 63)) break;
+      tc_fence_after();
+      ld_cols(tl + L::tQ + tb, x);   // scale gamma Q S0 goes back, P u is added to it there
+      {
+        uint32_t y[kTok];
+        with_tokens(gates.gam, [&](int i, float g) { y[i] = __float_as_uint(p.scale * g * x[i]); });
+        st_cols(tl + L::tQ + tb, y);
+      }
+      if (!warp_wait(&bars.xf, ph, abort, err, 64)) break;
+      tc_fence_after();
+      ld_cols(tl + L::tK + tb, x);
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) x[i] += e[i];   // x: e
+      with_tokens(gates.bet, [&](int i, float g) { e[i] = g * x[i]; });   // e: u
+      {
+        uint32_t w[PS][kTok / 2];
+        put_pieces<PS, kTok>(tl + L::tU + tb / 2, 32, e, w);
+        with_tokens(gates.tail, [&](int i, float g) { e[i] *= g; });
+        put_pieces<PS, kTok>(tl + L::tF + tb / 2, 32, e, w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&bars.uw);
+      if (warp == 0) {
+        if (!warp_wait(&bars.uw, ph, abort, err, 56)) break;
+        tc_fence_after();
+        if (lane == 0) {
+          mma_pieces<DKP, 64, true, PS, P, PS>(tmem + L::tD, tmem + L::tF, 32, tiles(c), 0);
+          mma_commit(&bars.ds);
+          mma_pieces<64, 64, false, PS, PS, PS>(tmem + L::tQ, tmem + L::tU, 32, tiles(c) + L::kOffP, 1);
+          mma_commit(&bars.pu);
+        }
+        __syncwarp();
+      }
+      if (STORE) {
+        uint32_t w[PS][kTok / 2];
+        split_all<PS, kTok>(x, w);
+        keep_pieces<PS>(p.ep + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWF, lane, kChunk, tb, w);
+      }
+      const float glast = *gates.last;
+      if (!warp_wait(&bars.ds, ph, abort, err, 65)) break;
+      tc_fence_after();
+      {
+        float y[HK];
+        ld_cols(tl + L::tD + kb, y);
+#pragma unroll
+        for (int i = 0; i < HK; ++i) st[i] = glast * st[i] + y[i];
+      }
+      if (c + 1 < nc) {
+        if (L::kOver) {   // the other quarters' columns of K^T W are read too
+          tc_fence_before();
+          warp_arrive(&bars.share[q]);
+          if (!warp_wait(&bars.share[q], ph, abort, err, 66)) break;
+          tc_fence_after();
+        }
+        put_state(c + 1);
+        // with one stage the tiles of the next chunk can only be fetched once P u is through with these
+        if (warp == 0 && L::kStages == 2) issue_ks(c + 1);
+      }
+      if (!warp_wait(&bars.pu, ph, abort, err, 67)) break;
+      tc_fence_after();
+      ld_cols(tl + L::tQ + tb, x);
+      if (STORE) staged<T>(stage + L::kOffD, tb, lcol, e);
+      tc_fence_before();
+      fence_proxy_async();   // what this stage held is read before bulk copies may replace it
+      warp_arrive(&bars.o);
+      if (warp == 0 && c + 1 < nc) {   // all warps are through with this chunk: its tiles may go
+        if (!warp_wait(&bars.o, ph, abort, err, 54)) break;
+        if (loaded < nc) load();
+        if (L::kStages == 1) issue_ks(c + 1);
+        tc_fence_after();
+        issue_qs(c + 1);
+      }
+      if (STORE) {
+#pragma unroll
+        for (int i = 0; i < kTok; ++i) x[i] *= e[i];
+        const float s = sum_columns(x);
+        if ((lane & 1) == 0) p.odo[(slot_head(p, slot0 + c, h) * p.nv + tile) * kChunk + tb + lane / 2] = s;
+      } else if (on) {
+        const int64_t tok = (int64_t)c * kChunk + tb;
+        store_tokens(static_cast<T*>(p.o) + b * p.os.b + (t0 + tok) * p.os.t + h * p.os.h + col, p.os.t,
+                     (int)min(n - tok, (int64_t)kTok), x);
+      }
+    }
+    if (*abort && warp == 0 && lane == 0) {
+      // loads in flight must land, MMAs in flight end, before the block's memory goes
+      for (int s = 0; s < L::kStages; ++s)
+        if (loaded > s) mbar_wait(&bars.full[s], ((loaded - 1 - s) / L::kStages) & 1, 1u << 22);
+      mma_commit(&bars.drain);
+      mbar_wait(&bars.drain, 0, 1u << 22);
+    }
+    if (p.s_end != nullptr && on && !*abort)
+      store_column(p.s_end + sbase + (size_t)kb * p.dv + col, p.dv, p.dk - kb, st);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
 template <int DKP, typename T, int PS, bool STORE>
 cudaError_t run_scan(const Params& p, cudaStream_t s) {
-  constexpr int smem = ScanLayout<DKP, T, PS>::kBytes;
-  const unsigned grid = (unsigned)p.nseq * p.hv * p.nv;
+  constexpr int smem = ScanLayout<DKP, T, PS, STORE>::kBytes;
+  const unsigned grid = (unsigned)p.nseq * p.hv * ((p.dv + kLanes - 1) / kLanes);
   const double rows = (double)p.bound * kChunk * p.hv;
+  int* err = device_error_flag();
+  if (err == nullptr) return cudaErrorInvalidValue;
   LaunchTimer t(STORE ? "delta_scan_store_kernel" : "delta_scan_kernel", s, rows * 2.0 * p.dv * sizeof(T),
                 rows * 6.0 * p.dk * p.dv);
   cudaError_t e = allow_smem(scan_kernel<DKP, T, PS, STORE>, smem);
   if (e != cudaSuccess) return e;
-  scan_kernel<DKP, T, PS, STORE><<<grid, 256, smem, s>>>(p);
+  scan_kernel<DKP, T, PS, STORE><<<grid, kTcThreads, smem, s>>>(p, err);
   return cudaGetLastError();
 }
 
