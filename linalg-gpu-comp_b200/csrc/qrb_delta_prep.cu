@@ -1,13 +1,15 @@
 // Per-chunk factors of the gated delta rule (mathematics in qrb_delta.cuh).
 //
 //   plan_kernel  packed layout: first chunk slot of every sequence (one block, a prefix sum).
-//   prep_kernel  one block per (chunk, value head): the running decays, X and P of the chunk,
-//                and the chunk's q, k, v (and dO) as zero-padded tiles.  These depend on no state,
-//                so all chunks run at once and the sequential kernels are left with products only.
+//   prep_kernel  one block per (chunk, value head): the running decays, X and P of the chunk, and
+//                the chunk's q, k, v (and dO) as zero-padded tiles.  These depend on no state, so all chunks run at once and the
+//                sequential kernels are left with products only.
 //
-// X is solved column by column in fp32: thread j owns column j, the rows of M are broadcast
-// from shared memory, 2016 multiply-adds a thread in four independent sums.  It is a T factor's
-// recurrence, bound by issue, and blocks of other chunks fill the SM beside it.
+// X is a triangular inverse, as T factors are: the four diagonal 16 x 16 blocks by substitution, a
+// column a thread, then two merges X_10 = R + X_11 beta R with R = -(M_10 + M_10 beta X_00), all in
+// fp32.  One substitution over 64 rows (2016 multiply-adds in a row on 64 threads) and an exponential
+// for every entry of M and P took 370 us for 8896 chunks and heads of 128; the merges are a third of
+// that chain, and off the diagonal blocks a decay is a product of two tabled factors.
 #include "qrb_delta.cuh"
 
 namespace qrb {
@@ -50,70 +52,78 @@ __global__ void __launch_bounds__(1024) plan_kernel(Params p) {
   }
 }
 
-template <int DKP, typename T, int PS>
-constexpr int prep_operands() {
-  constexpr int qk = 2 * tile_bytes(kChunk, Pieces<T>::kIn, DKP);
-  constexpr int xp = 2 * tile_bytes(kChunk, PS, kChunk);
-  return qk > xp ? qk : xp;
-}
-constexpr int kMStride = 68;   // floats per row of M: rows stay 16-byte aligned, columns on distinct banks
+constexpr int kPrepThreads = 256;
+constexpr int kMStride = 68;   // floats per row of M and X: rows stay 16-byte aligned, columns on distinct banks
+constexpr int kRStride = 36;
 
 template <int DKP, typename T, int PS>
-constexpr int prep_smem() {
-  return prep_operands<DKP, T, PS>() + kChunk * kMStride * 4 + kChunk * 8 + kChunk * 4;
-}
+struct PrepLayout {
+  static constexpr int P = Pieces<T>::kIn;
+  static constexpr int kQK = tile_bytes(kChunk, P, DKP), kXP = tile_bytes(kChunk, PS, kChunk);
+  // once the products are taken, over k and q: X's two 32 x 32 diagonal blocks (fp32), the right sides
+  // of a merge, and the pieces of P, later those of X.  52 KB with 16-bit operands: four blocks an SM.
+  static constexpr int kOffS = 0, kOffR = 2 * 32 * kRStride * 4, kOffT = 16384;
+  static_assert(kOffR + 32 * kRStride * 4 <= kOffT, "overlay");
+  static constexpr int kOffM = 2 * kQK > kOffT + kXP ? 2 * kQK : kOffT + kXP;   // M, fp32
+  static constexpr int kOffG = kOffM + kChunk * kMStride * 4;                   // G (fp64), beta, decay tables
+  static constexpr int kBytes = kOffG + kChunk * 8 + kChunk * 4 + kChunk * 4 + 4 * kChunk * 4;
+  static_assert(kBytes <= 232448, "shared memory of one block");
+};
 
-// Rows of x (dense last dimension of d <= DKP) as zero-padded pieces.
-template <int DKP, typename T>
-__device__ void load_rows(unsigned char* tile, const T* x, int64_t row_stride, int len, int d, bool vec) {
-  constexpr int P = Pieces<T>::kIn;
-  constexpr int V = 16 / sizeof(T);
-  if (vec) {
-    for (int u = threadIdx.x; u < kChunk * (DKP / V); u += blockDim.x) {
-      const int r = u / (DKP / V), c = (u % (DKP / V)) * V;
-      alignas(16) T e[V];
-      if (r < len && c < d)
-        *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(x + r * row_stride + c);
-      else
-        *reinterpret_cast<uint4*>(e) = make_uint4(0, 0, 0, 0);
-      if (P == 1) {
-        *reinterpret_cast<uint4*>(tile + tile_off(kChunk, r, c)) = *reinterpret_cast<uint4*>(e);
-      } else {
+// kChunk rows of W values, 16-byte units dealt out over the block: every load of a thread is issued
+// before the first is used (a loop of load and store waits for memory once a turn).  Rows and columns
+// that do not exist read existing ones and become zero.
+template <typename T, int W>
+struct Rows {
+  static constexpr int V = 16 / sizeof(T), kUnits = kChunk * (W / V) / kPrepThreads;
+  static_assert(kUnits * kPrepThreads * V == kChunk * W, "whole turns");
+  uint4 r[kUnits];
+  __device__ __forceinline__ static int row(int u) { return (threadIdx.x + u * kPrepThreads) / (W / V); }
+  __device__ __forceinline__ static int col(int u) { return (threadIdx.x + u * kPrepThreads) % (W / V) * V; }
+  __device__ __forceinline__ void load(const T* x, int64_t stride, int len, int d, bool vec) {
 #pragma unroll
-        for (int i = 0; i < V; i += 2) put2<P>(tile, kChunk, DKP, r, c + i, to_f(e[i]), to_f(e[i + 1]));
+    for (int u = 0; u < kUnits; ++u) {
+      const int rr = row(u), c = col(u);
+      const T* from = x + (int64_t)min(rr, len - 1) * stride;
+      if (vec && d % V == 0) {
+        r[u] = __ldg(reinterpret_cast<const uint4*>(from + (c < d ? c : 0)));
+      } else {
+        alignas(16) T e[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) e[i] = __ldg(from + min(c + i, d - 1));
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (c + i >= d) e[i] = from_f<T>(0.f);
+        r[u] = *reinterpret_cast<uint4*>(e);
+      }
+      if (rr >= len || c >= d) r[u] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  // as pieces into an operand tile
+  __device__ __forceinline__ void put(unsigned char* tile) const {
+    constexpr int P = Pieces<T>::kIn;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int rr = row(u), c = col(u);
+      if (P == 1) {
+        *reinterpret_cast<uint4*>(tile + tile_off(kChunk, rr, c)) = r[u];
+      } else {
+        const T* e = reinterpret_cast<const T*>(&r[u]);
+#pragma unroll
+        for (int i = 0; i < V; i += 2) put2<P>(tile, kChunk, W, rr, c + i, to_f(e[i]), to_f(e[i + 1]));
       }
     }
-    return;
   }
-  for (int u = threadIdx.x; u < kChunk * (DKP / 2); u += blockDim.x) {
-    const int r = u / (DKP / 2), c = (u % (DKP / 2)) * 2;
-    const float a = r < len && c < d ? to_f(x[r * row_stride + c]) : 0.f;
-    const float b = r < len && c + 1 < d ? to_f(x[r * row_stride + c + 1]) : 0.f;
-    put2<P>(tile, kChunk, DKP, r, c, a, b);
-  }
-}
-
-// v or dO of the chunk as kChunk x 128 tiles (one per 128 value columns), zero-padded: what the
-// recurrences then read needs no test of rows, columns or alignment.
-template <typename T>
-__device__ void stage_rows(unsigned char* to, const T* x, int64_t row_stride, int len, int dv, bool vec) {
-  constexpr int V = 16 / sizeof(T);
-  const int nb = (dv + 127) / 128;
-  for (int u = threadIdx.x; u < nb * kChunk * (128 / V); u += blockDim.x) {
-    const int r = (u / (128 / V)) % kChunk, c = (u % (128 / V)) * V, col = u / (kChunk * 128 / V) * 128 + c;
-    alignas(16) T e[V];
-    if (r < len && vec && col + V <= dv) {
-      *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(x + r * row_stride + col);
-    } else {
+  // as they are, dense rows
+  __device__ __forceinline__ void keep(unsigned char* to) const {
 #pragma unroll
-      for (int i = 0; i < V; ++i) e[i] = r < len && col + i < dv ? x[r * row_stride + col + i] : from_f<T>(0.f);
-    }
-    *reinterpret_cast<uint4*>(to + (size_t)u * 16) = *reinterpret_cast<uint4*>(e);
+    for (int u = 0; u < kUnits; ++u)
+      *reinterpret_cast<uint4*>(to + (size_t)(threadIdx.x + u * kPrepThreads) * 16) = r[u];
   }
-}
+};
 
 template <typename T>
-__device__ void zero_rows(const Params& p, int idx, int h) {
+__device__ void zero_rows(const Params& p, int idx, int h, int hk) {
   int64_t end = p.offsets[p.nseq];
   end = end < 0 ? 0 : end;
   const int64_t t0 = end + (int64_t)idx * kChunk;
@@ -126,9 +136,9 @@ __device__ void zero_rows(const Params& p, int idx, int h) {
     } else {
       T* dv = static_cast<T*>(p.dv_) + (t * p.hv + h) * p.dv;
       for (int c = threadIdx.x; c < p.dv; c += blockDim.x) dv[c] = from_f<T>(0.f);
-      if (h < p.hk) {
-        T* dq = static_cast<T*>(p.dq) + (t * p.hk + h) * p.dk;
-        T* dk = static_cast<T*>(p.dk_) + (t * p.hk + h) * p.dk;
+      if (h % p.group == 0) {
+        T* dq = static_cast<T*>(p.dq) + (t * p.hk + hk) * p.dk;
+        T* dk = static_cast<T*>(p.dk_) + (t * p.hk + hk) * p.dk;
         for (int c = threadIdx.x; c < p.dk; c += blockDim.x) dq[c] = dk[c] = from_f<T>(0.f);
       }
       if (threadIdx.x == 0) p.dg[t * p.hv + h] = p.dbeta[t * p.hv + h] = 0.f;
@@ -136,66 +146,102 @@ __device__ void zero_rows(const Params& p, int idx, int h) {
   }
 }
 
+// R -= (M diag(beta)) X over l in [l0, l0 + N): two rows and four columns a thread.
+template <int N>
+__device__ __forceinline__ void block_product(float (&r)[2][4], const float* m0, const float* m1, const float* beta,
+                                              const float* x, int stride) {
+#pragma unroll 8
+  for (int l = 0; l < N; ++l) {
+    const float4 y = *reinterpret_cast<const float4*>(x + l * stride);
+    const float b = beta[l], a0 = m0[l] * b, a1 = m1[l] * b;
+    r[0][0] += a0 * y.x;
+    r[0][1] += a0 * y.y;
+    r[0][2] += a0 * y.z;
+    r[0][3] += a0 * y.w;
+    r[1][0] += a1 * y.x;
+    r[1][1] += a1 * y.y;
+    r[1][2] += a1 * y.z;
+    r[1][3] += a1 * y.w;
+  }
+}
+
 template <int DKP, typename T, int PS>
-__global__ void __launch_bounds__(128) prep_kernel(Params p, int vec) {
-  constexpr int P = Pieces<T>::kIn;
-  constexpr int kQK = tile_bytes(kChunk, P, DKP), kXP = tile_bytes(kChunk, PS, kChunk);
+__global__ void __launch_bounds__(kPrepThreads, PS == 3 ? 2 : 4) prep_kernel(Params p, int vec) {
+  using L = PrepLayout<DKP, T, PS>;
+  constexpr int P = L::P;
   extern __shared__ __align__(128) unsigned char sm[];
-  unsigned char *kt = sm, *qt = sm + kQK, *xt = sm, *pt = sm + kXP;
-  float* M = reinterpret_cast<float*>(sm + prep_operands<DKP, T, PS>());
-  double* G = reinterpret_cast<double*>(M + kChunk * kMStride);
+  unsigned char *kt = sm, *qt = sm + L::kQK, *xp = sm + L::kOffT;
+  float* M = reinterpret_cast<float*>(sm + L::kOffM);
+  float* X = reinterpret_cast<float*>(sm + L::kOffS);
+  float* R = reinterpret_cast<float*>(sm + L::kOffR);
+  double* G = reinterpret_cast<double*>(sm + L::kOffG);
   float* beta = reinterpret_cast<float*>(G + kChunk);
+  float* down = beta + kChunk;     // exp(G_i - G before i's block of 16)
+  float* across = down + kChunk;   // [block][j]: exp(G before the block - G_j)
   const int c = blockIdx.x, h = blockIdx.y, hk = h / p.group, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Chunk ch = chunk_at(p, c);
   if (ch.seq < 0) {
-    if (p.zero_tail) zero_rows<T>(p, ch.idx, h);
+    if (p.zero_tail) zero_rows<T>(p, ch.idx, h, hk);
     return;
   }
-  load_rows<DKP, T>(kt, static_cast<const T*>(p.k) + ch.b * p.ks.b + ch.t0 * p.ks.t + hk * p.ks.h, p.ks.t, ch.len,
-                    p.dk, vec & 1);
-  load_rows<DKP, T>(qt, static_cast<const T*>(p.q) + ch.b * p.qs.b + ch.t0 * p.qs.t + hk * p.qs.h, p.qs.t, ch.len,
-                    p.dk, vec & 2);
   const size_t sh = slot_head(p, c, h);
-  const size_t vat = sh * ((p.dv + 127) / 128) * kChunk * 128 * sizeof(T);
-  stage_rows<T>(p.vt + vat, static_cast<const T*>(p.v) + ch.b * p.vs.b + ch.t0 * p.vs.t + h * p.vs.h, p.vs.t, ch.len,
-                p.dv, vec & 4);
-  if (p.backward)
-    stage_rows<T>(p.dot + vat, static_cast<const T*>(p.d_o) + ch.b * p.dos.b + ch.t0 * p.dos.t + h * p.dos.h, p.dos.t,
-                  ch.len, p.dv, vec & 8);
+  float g[2] = {0.f, 0.f}, bt[2] = {0.f, 0.f};
   if (warp == 0) {
-    // Running sums of g in fp64: differences of far apart sums keep their low bits.
     const int64_t gbase = ch.b * p.gs.b + ch.t0 * p.gs.t + h * p.gs.h;
     const int64_t bbase = ch.b * p.bs.b + ch.t0 * p.bs.t + h * p.bs.h;
-    double g[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int i = 2 * lane + e;
-      float x = 0.f, b = 0.f;
-      if (i < ch.len) {
-        x = p.g[gbase + i * p.gs.t];
-        b = p.beta[bbase + i * p.bs.t];
-        if (x < kMinLog) x = kMinLog;
-      }
-      g[e] = x;
-      beta[i] = b;
+      const int i = min(2 * lane + e, ch.len - 1);
+      g[e] = __ldg(p.g + gbase + i * p.gs.t);
+      bt[e] = __ldg(p.beta + bbase + i * p.bs.t);
     }
-    double s = g[0] + g[1];
+  }
+  {
+    Rows<T, DKP> k, q;
+    k.load(static_cast<const T*>(p.k) + ch.b * p.ks.b + ch.t0 * p.ks.t + hk * p.ks.h, p.ks.t, ch.len, p.dk, vec & 1);
+    q.load(static_cast<const T*>(p.q) + ch.b * p.qs.b + ch.t0 * p.qs.t + hk * p.qs.h, p.qs.t, ch.len, p.dk, vec & 2);
+    k.put(kt);
+    q.put(qt);
+  }
+  if (warp == 0) {
+    // Running sums of g in fp64: differences of far apart sums keep their low bits.
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (2 * lane + e >= ch.len) g[e] = bt[e] = 0.f;
+      if (g[e] < kMinLog) g[e] = kMinLog;
+    }
+    double s = (double)g[0] + (double)g[1];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double y = __shfl_up_sync(0xffffffffu, s, o);
       if (lane >= o) s += y;
     }
     const double last = __shfl_sync(0xffffffffu, s, 31);
-    const double g1 = s, g0 = s - g[1];
+    const double g1 = s, g0 = s - (double)g[1];
+    // G before this lane's block of 16 (8 lanes)
+    double before = __shfl_sync(0xffffffffu, s, (lane & ~7) == 0 ? 0 : (lane & ~7) - 1);
+    if (lane < 8) before = 0.;
     G[2 * lane] = g0;
     G[2 * lane + 1] = g1;
+    beta[2 * lane] = bt[0];
+    beta[2 * lane + 1] = bt[1];
+    down[2 * lane] = expf((float)(g0 - before));
+    down[2 * lane + 1] = expf((float)(g1 - before));
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      const double ref = __shfl_sync(0xffffffffu, s, 8 * i - 1);
+      if (lane < 8 * i) {
+        across[i * kChunk + 2 * lane] = expf((float)(ref - g0));
+        across[i * kChunk + 2 * lane + 1] = expf((float)(ref - g1));
+      }
+    }
     float* gt = p.gates + sh * 3 * kChunk;
     gt[2 * lane] = expf((float)g0);
     gt[2 * lane + 1] = expf((float)g1);
     gt[kChunk + 2 * lane] = expf((float)(last - g0));
     gt[kChunk + 2 * lane + 1] = expf((float)(last - g1));
-    gt[2 * kChunk + 2 * lane] = beta[2 * lane];
-    gt[2 * kChunk + 2 * lane + 1] = beta[2 * lane + 1];
+    gt[2 * kChunk + 2 * lane] = bt[0];
+    gt[2 * kChunk + 2 * lane + 1] = bt[1];
     if (p.backward) {
       p.gsum[sh * kChunk + 2 * lane] = g0;
       p.gsum[sh * kChunk + 2 * lane + 1] = g1;
@@ -203,63 +249,161 @@ __global__ void __launch_bounds__(128) prep_kernel(Params p, int vec) {
   }
   __syncthreads();
   if (h % p.group == 0) {   // one of the heads that share these q, k stores their tiles
-    const size_t at = ((size_t)c * p.hk + hk) * kQK;
-    for (int i = tid * 16; i < kQK; i += 128 * 16) {
+    const size_t at = ((size_t)c * p.hk + hk) * L::kQK;
+    for (int i = tid * 16; i < L::kQK; i += kPrepThreads * 16) {
       *reinterpret_cast<uint4*>(p.kt + at + i) = *reinterpret_cast<const uint4*>(kt + i);
       *reinterpret_cast<uint4*>(p.qt + at + i) = *reinterpret_cast<const uint4*>(qt + i);
     }
   }
-  float am[8][4], ap[8][4];
-  zero(am);
-  zero(ap);
-  mma_tile<8, false, false, P, P, PS>(am, kt, kChunk, DKP, 16 * warp, kt, kChunk, DKP, 0, 0, DKP);
-  mma_tile<8, false, false, P, P, PS>(ap, qt, kChunk, DKP, 16 * warp, kt, kChunk, DKP, 0, 0, DKP);
-  __syncthreads();
+  {
+    // warps 0-3: K K^T, warps 4-7: Q K^T, 16 rows each
+    const int blk = warp & 3, m0 = 16 * blk;
+    float acc[8][4];
+    zero(acc);
+    mma_tile<8, false, false, P, P, PS>(acc, warp < 4 ? kt : qt, kChunk, DKP, m0, kt, kChunk, DKP, 0, 0, DKP);
+    __syncthreads();   // k and q are read: their memory changes hands
+    // decays: exact in the diagonal block, the product of two factors <= 1 (for g <= 0) before it
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < 8; ++j) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int i = 16 * warp + (lane >> 2) + 8 * r, cl = 8 * j + 2 * (lane & 3);
-      const float d0 = cl <= i ? expf((float)(G[i] - G[cl])) : 0.f;
-      const float d1 = cl + 1 <= i ? expf((float)(G[i] - G[cl + 1])) : 0.f;
-      M[i * kMStride + cl] = cl < i ? am[j][2 * r] * d0 : 0.f;
-      M[i * kMStride + cl + 1] = cl + 1 < i ? am[j][2 * r + 1] * d1 : 0.f;
-      put2<PS>(pt, kChunk, kChunk, i, cl, cl <= i ? p.scale * ap[j][2 * r] * d0 : 0.f,
-               cl + 1 <= i ? p.scale * ap[j][2 * r + 1] * d1 : 0.f);
-    }
-  __syncthreads();
-  if (tid < kChunk) {
-    float y[kChunk];   // beta_l X_lj
-#pragma unroll
-    for (int i = 0; i < kChunk; ++i) {
-      float s0 = M[i * kMStride + tid], s1 = 0.f, s2 = 0.f, s3 = 0.f;
-#pragma unroll
-      for (int l = 0; l < (i & ~3); l += 4) {
-        const float4 m = *reinterpret_cast<const float4*>(M + i * kMStride + l);
-        s0 += m.x * y[l];
-        s1 += m.y * y[l + 1];
-        s2 += m.z * y[l + 2];
-        s3 += m.w * y[l + 3];
-      }
-#pragma unroll
-      for (int l = i & ~3; l < i; ++l) s1 += M[i * kMStride + l] * y[l];
-      float x = -((s0 + s1) + (s2 + s3));
-      y[i] = beta[i] * x;
-#pragma unroll
-      for (int q = 0; q < PS; ++q) {
-        const __nv_bfloat16 hx = __float2bfloat16_rn(x);
-        *reinterpret_cast<__nv_bfloat16*>(xt + tile_off(kChunk, i, q * kChunk + tid)) = hx;
-        x -= __bfloat162float(hx);
-        if (q == 0 && !(fabsf(x) <= 3.4e38f)) x = 0.f;
+      for (int r = 0; r < 2; ++r) {
+        const int i = m0 + (lane >> 2) + 8 * r, cl = 8 * j + 2 * (lane & 3);
+        float d0 = 0.f, d1 = 0.f;
+        if (j < 2 * blk) {
+          const float a = down[i];
+          const float2 x = *reinterpret_cast<const float2*>(across + blk * kChunk + cl);
+          d0 = a * x.x;
+          d1 = a * x.y;
+        } else if (j < 2 * blk + 2) {
+          if (cl <= i) d0 = expf((float)(G[i] - G[cl]));
+          if (cl + 1 <= i) d1 = expf((float)(G[i] - G[cl + 1]));
+        }
+        if (warp < 4) {
+          *reinterpret_cast<float2*>(M + i * kMStride + cl) =
+              make_float2(cl < i ? acc[j][2 * r] * d0 : 0.f, cl + 1 < i ? acc[j][2 * r + 1] * d1 : 0.f);
+        } else {
+          put2<PS>(xp, kChunk, kChunk, i, cl, cl <= i ? p.scale * acc[j][2 * r] * d0 : 0.f,
+                   cl + 1 <= i ? p.scale * acc[j][2 * r + 1] * d1 : 0.f);
+        }
       }
     }
-  } else {
-    for (int i = (tid - kChunk) * 16; i < kXP; i += kChunk * 16)
-      *reinterpret_cast<uint4*>(p.pt + sh * kXP + i) = *reinterpret_cast<const uint4*>(pt + i);
   }
   __syncthreads();
-  for (int i = tid * 16; i < kXP; i += 128 * 16)
-    *reinterpret_cast<uint4*>(p.xt + sh * kXP + i) = *reinterpret_cast<const uint4*>(xt + i);
+  if (tid < kChunk) {
+    // the four diagonal 16 x 16 blocks of X, a column a thread
+    const int o = tid & ~15, j = tid & 15;
+    float* to = X + (o >> 5) * 32 * kRStride + (o & 16) * (kRStride + 1);
+    float y[16];   // beta x
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float* m = M + (o + i) * kMStride + o;
+      float s0 = m[j], s1 = 0.f;
+#pragma unroll
+      for (int l = 0; l < i; ++l) {
+        if (l & 1) s1 += m[l] * y[l];
+        else s0 += m[l] * y[l];
+      }
+      const float x = -(s0 + s1);
+      y[i] = beta[o + i] * x;
+      to[i * kRStride + j] = x;
+    }
+  } else {
+    for (int i = (tid - kChunk) * 16; i < L::kXP; i += (kPrepThreads - kChunk) * 16)
+      *reinterpret_cast<uint4*>(p.pt + sh * L::kXP + i) = *reinterpret_cast<const uint4*>(xp + i);
+  }
+  __syncthreads();
+  // v and dO as kChunk x 128 tiles, one per 128 value columns: what the recurrences then read needs no
+  // test of rows, columns or alignment.  Two warps merge meanwhile; the blocks of X above the diagonal
+  // are zeroed here too.
+  float r[2][4];
+  const int half = tid >> 5 & 1, t16 = tid & 31;   // threads 0 .. 63: 8 x 4 tiles of 2 x 4
+  const int i16 = (t16 >> 2) * 2, j16 = (t16 & 3) * 4;
+  float* X32 = X + half * 32 * kRStride;
+  // 16 -> 32: X_10 = R + X_11 beta R, R = -(M_10 + M_10 beta X_00), in both halves of the chunk
+  if (tid < 64) {
+    const float *ma = M + (32 * half + 16 + i16) * kMStride + 32 * half, *mb = ma + kMStride;
+    const float4 a = *reinterpret_cast<const float4*>(ma + j16), b = *reinterpret_cast<const float4*>(mb + j16);
+    r[0][0] = a.x, r[0][1] = a.y, r[0][2] = a.z, r[0][3] = a.w;
+    r[1][0] = b.x, r[1][1] = b.y, r[1][2] = b.z, r[1][3] = b.w;
+    block_product<16>(r, ma, mb, beta + 32 * half, X32 + j16, kRStride);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      *reinterpret_cast<float4*>(R + (16 * half + i16 + e) * kRStride + j16) =
+          make_float4(-r[e][0], -r[e][1], -r[e][2], -r[e][3]);
+    __syncwarp();   // each half is one warp's
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) r[e][q] = -r[e][q];
+    const float* xa = X32 + (16 + i16) * kRStride + 16;
+    block_product<16>(r, xa, xa + kRStride, beta + 32 * half + 16, R + 16 * half * kRStride + j16, kRStride);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      *reinterpret_cast<float4*>(X32 + (16 + i16 + e) * kRStride + j16) =
+          make_float4(r[e][0], r[e][1], r[e][2], r[e][3]);
+  } else {
+    for (int i = (tid - 64) * 16; i < L::kXP; i += (kPrepThreads - 64) * 16)
+      *reinterpret_cast<uint4*>(xp + i) = make_uint4(0, 0, 0, 0);
+  }
+  for (int vb = 0; vb * 128 < p.dv; ++vb) {
+    const size_t vat = (sh * ((p.dv + 127) / 128) + vb) * kChunk * 128 * sizeof(T);
+    Rows<T, 128> v;
+    v.load(static_cast<const T*>(p.v) + ch.b * p.vs.b + ch.t0 * p.vs.t + h * p.vs.h + vb * 128, p.vs.t, ch.len,
+           min(128, p.dv - vb * 128), vec & 4);
+    v.keep(p.vt + vat);
+    if (p.backward) {
+      v.load(static_cast<const T*>(p.d_o) + ch.b * p.dos.b + ch.t0 * p.dos.t + h * p.dos.h + vb * 128, p.dos.t, ch.len,
+             min(128, p.dv - vb * 128), vec & 8);
+      v.keep(p.dot + vat);
+    }
+  }
+  __syncthreads();
+  // 32 -> 64 the same way: 16 x 8 tiles of 2 x 4, the first 128 threads
+  const int i32 = ((tid & 127) >> 3) * 2, j32 = (tid & 7) * 4;
+  if (tid < 128) {
+    const float *ma = M + (32 + i32) * kMStride, *mb = ma + kMStride;
+    const float4 a = *reinterpret_cast<const float4*>(ma + j32), b = *reinterpret_cast<const float4*>(mb + j32);
+    r[0][0] = a.x, r[0][1] = a.y, r[0][2] = a.z, r[0][3] = a.w;
+    r[1][0] = b.x, r[1][1] = b.y, r[1][2] = b.z, r[1][3] = b.w;
+    // X_00's columns 16 .. 31 begin at row 16
+    if (j32 < 16)
+      block_product<32>(r, ma, mb, beta, X + j32, kRStride);
+    else
+      block_product<16>(r, ma + 16, mb + 16, beta + 16, X + 16 * kRStride + j32, kRStride);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      *reinterpret_cast<float4*>(R + (i32 + e) * kRStride + j32) = make_float4(-r[e][0], -r[e][1], -r[e][2], -r[e][3]);
+  } else {
+    // meanwhile: pieces of the two diagonal 32 x 32 blocks
+    for (int u = tid - 128; u < 2 * 32 * 16; u += 128) {
+      const int o = u >> 9, i = (u >> 4) & 31, j = (u & 15) * 2;
+      if (j < i) {
+        const float* x = X + (o * 32 + i) * kRStride + j;
+        put2<PS>(xp, kChunk, kChunk, 32 * o + i, 32 * o + j, x[0], j + 1 < i ? x[1] : 0.f);
+      }
+    }
+  }
+  __syncthreads();
+  if (tid < 128) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) r[e][q] = -r[e][q];
+    const float* xa = X + (32 + i32) * kRStride;
+    // X_11's rows 0 .. 15 have nothing in its second half's columns
+    if (i32 < 16)
+      block_product<16>(r, xa, xa + kRStride, beta + 32, R + j32, kRStride);
+    else
+      block_product<32>(r, xa, xa + kRStride, beta + 32, R + j32, kRStride);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      put2<PS>(xp, kChunk, kChunk, 32 + i32 + e, j32, r[e][0], r[e][1]);
+      put2<PS>(xp, kChunk, kChunk, 32 + i32 + e, j32 + 2, r[e][2], r[e][3]);
+    }
+  }
+  __syncthreads();
+  for (int i = tid * 16; i < L::kXP; i += kPrepThreads * 16)
+    *reinterpret_cast<uint4*>(p.xt + sh * L::kXP + i) = *reinterpret_cast<const uint4*>(xp + i);
 }
 
 template <int DKP, typename T, int PS>
@@ -271,13 +415,13 @@ cudaError_t run_prep(const Params& p, cudaStream_t s) {
   const bool dk_ok = p.dk % (16 / (int)sizeof(T)) == 0;
   const int vec = (dk_ok && fits(p.k, p.ks) ? 1 : 0) | (dk_ok && fits(p.q, p.qs) ? 2 : 0) | (fits(p.v, p.vs) ? 4 : 0) |
                   (fits(p.d_o, p.dos) ? 8 : 0);
-  constexpr int smem = prep_smem<DKP, T, PS>();
+  constexpr int smem = PrepLayout<DKP, T, PS>::kBytes;
   cudaError_t e = allow_smem(prep_kernel<DKP, T, PS>, smem);
   if (e != cudaSuccess) return e;
   const double tokens = (double)p.bound * kChunk;
-  LaunchTimer t("delta_prep_kernel", s, tokens * p.hv * (2.0 * p.dk * sizeof(T) + 4.0 * kChunk * PS),
+  LaunchTimer t("delta_prep_kernel", s, tokens * (2.0 * p.hk * p.dk * sizeof(T) + p.hv * (4.0 * kChunk * PS + p.dv * sizeof(T))),
                 tokens * p.hv * 4.0 * kChunk * p.dk);
-  prep_kernel<DKP, T, PS><<<dim3((unsigned)p.bound, (unsigned)p.hv), 128, smem, s>>>(p, vec);
+  prep_kernel<DKP, T, PS><<<dim3((unsigned)p.bound, (unsigned)p.hv), kPrepThreads, smem, s>>>(p, vec);
   return cudaGetLastError();
 }
 
