@@ -197,31 +197,45 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 // (PM is the piece count of the fp32 operands: what is dropped is below their own rounding).
 // One warp; k0, k1 multiples of 16, NT even.  Fragment layout of m16n8k16: lane 4 g + t holds
 // rows g and g + 8, columns 2 t and 2 t + 1 of each 16 x 8 block of acc.
+// A lane's ldmatrix address is a constant part and a part that the step of k (or the piece and the column
+// group) moves: 16-byte units of a swizzled row are XORed, everything else is added.
+template <bool U>
+struct LaneAddr {
+  uint32_t base;   // of the lane's row and unit
+  int rows;
+  __device__ __forceinline__ LaneAddr(const unsigned char* tile, int rows_, int row, int unit) : rows(rows_) {
+    base = s_addr(tile) + (U ? unit * rows * 16 + row * 16 : row * 128 + ((unit ^ (row & 7)) << 4));
+  }
+  // `col` more columns (a multiple of 8 that shares no bit with the unit), `row` more rows (of 8)
+  __device__ __forceinline__ uint32_t at(int row, int col) const {
+    if (U) return base + (col >> 3) * rows * 16 + row * 16;
+    return ((base + (col >> 6) * rows * 128 + row * 128) ^ ((col & 63) << 1));
+  }
+};
+
 template <int NT, bool AT, bool BT, int PA, int PB, int PM, bool AU = false, bool BU = false>
 __device__ __forceinline__ void mma_tile(float (&acc)[NT][4], const unsigned char* A, int arows, int apc, int m0,
                                          const unsigned char* B, int brows, int bpc, int n0, int k0, int k1) {
   const int lane = threadIdx.x & 31;
-  const uint32_t ab = s_addr(A), bb = s_addr(B);
+  const LaneAddr<AU> a_at(A, arows, AT ? (lane & 7) + ((lane >> 4) & 1) * 8 : m0 + (lane & 15),
+                          AT ? (lane >> 3) & 1 : lane >> 4);
+  const LaneAddr<BU> b_at(B, brows, BT ? lane & 15 : n0 + (lane & 7) + ((lane >> 4) & 1) * 8,
+                          BT ? lane >> 4 : (lane >> 3) & 1);
+#pragma unroll 2
   for (int k = k0; k < k1; k += 16) {
     uint32_t a[PA][4];
 #pragma unroll
     for (int p = 0; p < PA; ++p) {
-      if (AT)
-        ldsm4t(a[p], ab + any_off<AU>(arows, k + (lane & 7) + ((lane >> 4) & 1) * 8,
-                                   p * apc + m0 + ((lane >> 3) & 1) * 8));
-      else
-        ldsm4(a[p], ab + any_off<AU>(arows, m0 + (lane & 15), p * apc + k + (lane >> 4) * 8));
+      if (AT) ldsm4t(a[p], a_at.at(k, p * apc + m0));
+      else ldsm4(a[p], a_at.at(0, p * apc + k));
     }
 #pragma unroll
     for (int j = 0; j < NT; j += 2) {
 #pragma unroll
       for (int q = 0; q < PB; ++q) {
         uint32_t b[4];
-        if (BT)
-          ldsm4t(b, bb + any_off<BU>(brows, k + (lane & 15), q * bpc + n0 + 8 * j + (lane >> 4) * 8));
-        else
-          ldsm4(b, bb + any_off<BU>(brows, n0 + 8 * j + (lane & 7) + ((lane >> 4) & 1) * 8,
-                                 q * bpc + k + ((lane >> 3) & 1) * 8));
+        if (BT) ldsm4t(b, b_at.at(k, q * bpc + n0 + 8 * j));
+        else ldsm4(b, b_at.at(8 * j, q * bpc + k));
 #pragma unroll
         for (int p = 0; p < PA; ++p) {
           if (p + q < PM) {

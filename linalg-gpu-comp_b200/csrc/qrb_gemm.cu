@@ -3,10 +3,13 @@
 //
 // Persistent warp-specialised blocks, one per SM: a TMA producer fills a ring of 64-deep stages
 // (128-byte swizzle; operands with k along their rows and operands with k across them are both
-// read as they lie, so no backward product transposes anything), one thread issues
-// 128 x BN x 16 MMAs into TMEM, and four warps run the epilogue of one tile while the next one's
-// MMAs fill the other accumulator buffer.  BN = 256 reads 12 KB of shared memory per 128-cycle
-// MMA; narrower tiles serve small outputs.
+// read as they lie, so no backward product transposes anything), one thread issues MMAs 16 deep into
+// TMEM, and eight warps run the epilogue of one tile while the next one's MMAs fill the other
+// accumulator buffer.
+//   * Large outputs: pairs of blocks (cta_group::2) on 256 x 256 tiles, each block loading 128 rows of
+//     A and 128 of B: 32 KB per 512 cycles of MMAs.  One block on 128 x 256 needs 48 KB for the same
+//     time, more than L2 delivers to every SM at once (4096 x 2048 x 8192 took twice its MMA time).
+//   * Smaller ones: single blocks on 128 x 256, 128 or 64 tiles.
 //
 //   * Few rows (m <= 128): the operands change places, so the 128-row side of the MMA is the weight
 //     and its 16 .. 128 column side the rows: no tensor-core row is wasted on padding, and the
@@ -35,7 +38,7 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kBM = 128, kBK = 64, kThreads = 256;   // warps: producer, MMA, 2 idle, 4 epilogue
+constexpr int kBM = 128, kBK = 64, kThreads = 384;   // warps: producer, MMA, 2 idle, 8 epilogue
 constexpr int kMaxTerms = 6;
 constexpr int64_t kMaxSplitK32 = 4096;   // longest k of one fp32 accumulation
 
@@ -53,10 +56,11 @@ struct GemmArgs {
   int* err;
 };
 
-template <int BN>
+template <int BN, bool PAIR>
 struct Cfg {
-  static constexpr uint32_t kA = kBM * kBK * 2, kB = BN * kBK * 2, kStage = kA + kB;
-  static constexpr int kStages = BN == 256 ? 4 : 6;
+  static constexpr int kRowsB = PAIR ? BN / 2 : BN;   // rows of B this block loads
+  static constexpr uint32_t kA = kBM * kBK * 2, kB = kRowsB * kBK * 2, kStage = kA + kB;
+  static constexpr int kStages = kStage > 40960 ? 4 : 6;
   static constexpr uint32_t kBar = kStages * kStage;
   static constexpr uint32_t kSmem = kBar + 256 + 1024;
 };
@@ -74,6 +78,17 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t ad, uint64_t bd, ui
       ".reg .pred p;\n"
       "setp.ne.b32 p, %4, 0;\n"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d),
+      "l"(ad), "l"(bd), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
       "}\n" ::"r"(d),
       "l"(ad), "l"(bd), "r"(idesc), "r"(acc)
       : "memory");
@@ -156,20 +171,22 @@ __device__ __forceinline__ void tile_of(const GemmArgs& g, int u, int& tm, int& 
   tn = r / rows;
 }
 
-template <int BN>
+template <int BN, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
             const __grid_constant__ GemmArgs g) {
-  using C = Cfg<BN>;
+  using C = Cfg<BN, PAIR>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                        ~uintptr_t(1023));
   Bars& bars = *reinterpret_cast<Bars*>(sm + C::kBar);
   volatile int* abort = &bars.abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = PAIR ? (int)cluster_ctarank() : 0;
+  const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
   const int units = g.tiles_m * g.tiles_n * g.splits;
   const int bufs = 2 * g.sets * BN <= 512 ? 2 : 1;
-  const uint32_t cols = (uint32_t)(bufs * g.sets * BN) < 32u ? 32u : (uint32_t)(bufs * g.sets * BN);
+  const uint32_t cols = (uint32_t)(bufs * g.sets * BN);   // a power of two, at least 128
 
   if (tid == 0) {
     for (int i = 0; i < C::kStages; ++i) {
@@ -178,28 +195,33 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.accf[i], 1);
-      mbar_init(&bars.acce[i], 4);
+      mbar_init(&bars.acce[i], PAIR ? 16 : 8);
     }
     mbar_init(&bars.drain, 1);
     bars.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc(&bars.tmem, cols);
+  if (warp == 1) {
+    if (PAIR) tmem_alloc_pair(&bars.tmem, cols);
+    else tmem_alloc(&bars.tmem, cols);
+  }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync_all();   // the peer's barriers exist
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
 
   if (warp == 0) {
-    // ---------------- TMA producer ----------------
+    // ---------------- TMA producer (both blocks of a pair, for the leader's barriers) ----------------
     if (lane == 0) {
       prefetch_tensormap(&map_a);
       prefetch_tensormap(&map_b);
       int64_t it = 0;
       bool ok = true;
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      for (int u = first; u < units && ok; u += step) {
         int tm, tn, sp;
         tile_of(g, u, tm, tn, sp);
+        const int row = (PAIR ? 2 * tm + rank : tm) * kBM, col = tn * BN + rank * C::kRowsB;
         const int kb0 = sp * g.per_split, kb1 = min(g.kblocks, kb0 + g.per_split);
         for (int t = 0; t < g.terms && ok; ++t)
           for (int kb = kb0; kb < kb1; ++kb, ++it) {
@@ -211,35 +233,43 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             }
             unsigned char* sa = sm + st * C::kStage;
             unsigned char* sb = sa + C::kA;
-            mbar_arrive_expect_tx(&bars.full[st], C::kStage);
+            if (rank == 0) mbar_arrive_expect_tx(&bars.full[st], (PAIR ? 2 : 1) * C::kStage);
+            const uint32_t bar = PAIR ? mapa_shared(smem_u32(&bars.full[st]), 0) : 0;
+            auto load = [&](void* dst, const CUtensorMap* map, int x, int y, int z) {
+              if (PAIR) tma_load_3d_pair(dst, map, x, y, z, bar);
+              else tma_load_3d(dst, map, x, y, z, &bars.full[st]);
+            };
             if (g.a_mn) {
-              tma_load_3d(sa, &map_a, tm * kBM, kb * kBK, g.pa[t], &bars.full[st]);
-              tma_load_3d(sa + 8192, &map_a, tm * kBM + 64, kb * kBK, g.pa[t], &bars.full[st]);
+              load(sa, &map_a, row, kb * kBK, g.pa[t]);
+              load(sa + 8192, &map_a, row + 64, kb * kBK, g.pa[t]);
             } else {
-              tma_load_3d(sa, &map_a, kb * kBK, tm * kBM, g.pa[t], &bars.full[st]);
+              load(sa, &map_a, kb * kBK, row, g.pa[t]);
             }
             if (g.b_mn) {
-              for (int j = 0; j < BN / 64; ++j)
-                tma_load_3d(sb + j * 8192, &map_b, tn * BN + 64 * j, kb * kBK, g.pb[t], &bars.full[st]);
+              for (int j = 0; j < C::kRowsB / 64; ++j) load(sb + j * 8192, &map_b, col + 64 * j, kb * kBK, g.pb[t]);
             } else {
-              tma_load_3d(sb, &map_b, kb * kBK, tn * BN, g.pb[t], &bars.full[st]);
+              load(sb, &map_b, kb * kBK, col, g.pb[t]);
             }
           }
       }
-      if (*abort) {   // let every load this block issued land before its shared memory goes away
+      if (*abort && rank == 0) {   // every load issued must land before the shared memory goes away
         for (int st = 0; st < C::kStages; ++st)
           if (it > st) mbar_wait(&bars.full[st], (uint32_t)(((it - 1 - st) / C::kStages) & 1), 1u << 22);
       }
     }
   } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
+    // ---------------- MMA issuer (the leader of a pair) ----------------
+    if (lane == 0 && rank == 0) {
       int64_t it = 0;
       int n = 0;
       bool ok = true, issued = false;
+      auto commit = [&](uint64_t* bar) {
+        if (PAIR) mma_commit_pair(bar);
+        else mma_commit(bar);
+      };
       const uint32_t a_lbo = g.a_mn ? 8192 : 16, a_step = g.a_mn ? 2048 : 32;
       const uint32_t b_lbo = g.b_mn ? 8192 : 16, b_step = g.b_mn ? 2048 : 32;
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++n) {
+      for (int u = first; u < units && ok; u += step, ++n) {
         int tm, tn, sp;
         tile_of(g, u, tm, tn, sp);
         const int kb0 = sp * g.per_split, kb1 = min(g.kblocks, kb0 + g.per_split);
@@ -259,15 +289,17 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             const uint32_t sa = smem_u32(sm + st * C::kStage), sb = sa + C::kA;
 #pragma unroll
             for (int kk = 0; kk < kBK / 16; ++kk) {
-              mma_f16(d, sdesc_sw128(sa + kk * a_step, a_lbo, 1024), sdesc_sw128(sb + kk * b_step, b_lbo, 1024),
-                      g.idesc, ((seen >> g.set[t]) & 1) | (kk > 0));
+              const uint64_t ad = sdesc_sw128(sa + kk * a_step, a_lbo, 1024), bd = sdesc_sw128(sb + kk * b_step, b_lbo, 1024);
+              const uint32_t acc = ((seen >> g.set[t]) & 1) | (kk > 0);
+              if (PAIR) mma_f16_pair(d, ad, bd, g.idesc, acc);
+              else mma_f16(d, ad, bd, g.idesc, acc);
             }
             seen |= 1 << g.set[t];
-            mma_commit(&bars.empty[st]);
+            commit(&bars.empty[st]);
             issued = true;
           }
         }
-        if (ok) mma_commit(&bars.accf[buf]);
+        if (ok) commit(&bars.accf[buf]);
       }
       if (*abort && issued) {   // tensor memory must not be released under running MMAs
         mma_commit(&bars.drain);
@@ -275,26 +307,25 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       }
     }
   } else if (warp >= 4) {
-    // ---------------- epilogue: TMEM lane = A's row ----------------
-    const int q = warp & 3;
+    // ---------------- epilogue: TMEM lane = A's row, half of the columns a warp ----------------
+    const int q = warp & 3, c_first = ((warp - 4) >> 2) * (BN / 2), c_last = c_first + BN / 2;
     const uint32_t tl = (uint32_t)(32 * q) << 16;
     const Epilogue& e = g.e;
     const bool vec = (e.y == nullptr || aligned_rows(e.y, e.ldy, e.dtype)) &&
                      (e.residual == nullptr || aligned_rows(e.residual, e.ldr, e.dtype)) &&
                      (e.pre == nullptr || aligned_rows(e.pre, e.ldpre, e.dtype));
     int n = 0;
-    for (int u = blockIdx.x; u < units; u += gridDim.x, ++n) {
+    for (int u = first; u < units; u += step, ++n) {
       int tm, tn, sp;
       tile_of(g, u, tm, tn, sp);
       const int buf = n % bufs, use = n / bufs;
-      const int64_t r = (int64_t)tm * kBM + 32 * q + lane, c0 = (int64_t)tn * BN;
+      const int64_t r = (int64_t)(PAIR ? 2 * tm + rank : tm) * kBM + 32 * q + lane, c0 = (int64_t)tn * BN;
       const float rb = g.swap && e.bias != nullptr && r < g.M ? load1(e.bias, r, e.dtype) : 0.f;
       // the whole warp goes on or leaves: tensor memory loads are collective
       if (!__all_sync(0xffffffffu, mbar_wait_abort(&bars.accf[buf], (uint32_t)(use & 1), abort, g.err, 44))) break;
       tc_fence_after();
-      constexpr int kCh = 32;
 #pragma unroll 1
-      for (int c = 0; c < BN; c += kCh) {
+      for (int c = c_first; c < c_last; c += 32) {
         float x[32];
         const uint32_t at = tmem + tl + (uint32_t)(buf * g.sets * BN + c);
         tmem_ld32(at, x);
@@ -305,28 +336,31 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           for (int j = 0; j < 32; ++j)
             if (fabsf(x[j]) <= 3.4e38f) x[j] += y[j];   // inf * 0 among the small products is no NaN of the sum
         }
-        if (c + kCh >= BN) {   // this warp's last read of the buffer
+        if (c + 32 >= c_last) {   // this warp's last read of the buffer
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.acce[buf]);
+          if (lane == 0) {
+            if (PAIR) mbar_arrive_cluster(mapa_shared(smem_u32(&bars.acce[buf]), 0));
+            else mbar_arrive(&bars.acce[buf]);
+          }
         }
-        float cb = 0.f;   // lane j: the bias of column c + j
-        if (!g.swap && g.splits == 1 && e.bias != nullptr && c0 + c + lane < g.N) cb = load1(e.bias, c0 + c + lane, e.dtype);
-        if (!g.swap && g.splits == 1) {
+        if (!g.swap && g.splits == 1 && e.bias != nullptr) {
+          // lane j holds the bias of column c + j
+          const float cb = c0 + c + lane < g.N ? load1(e.bias, c0 + c + lane, e.dtype) : 0.f;
 #pragma unroll
-          for (int j = 0; j < kCh; ++j) x[j] += __shfl_sync(0xffffffffu, cb, j);
+          for (int j = 0; j < 32; ++j) x[j] += __shfl_sync(0xffffffffu, cb, j);
         }
         if (r >= g.M) continue;
         if (g.splits > 1) {
           if (g.swap) {
 #pragma unroll
-            for (int j = 0; j < kCh; ++j)
+            for (int j = 0; j < 32; ++j)
               if (c0 + c + j < g.N) g.partial[((int64_t)sp * g.out_m + c0 + c + j) * g.out_n + r] = x[j];
           } else {
             float* to = g.partial + ((int64_t)sp * g.out_m + r) * g.out_n + c0 + c;
             const bool v4 = g.out_n % 4 == 0;
 #pragma unroll
-            for (int j = 0; j < kCh; j += 4) {
+            for (int j = 0; j < 32; j += 4) {
               if (v4 && c0 + c + j + 3 < g.N) *reinterpret_cast<float4*>(to + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
               else
                 for (int i = 0; i < 4; ++i)
@@ -336,49 +370,59 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           continue;
         }
         if (g.swap) {
+          const int count = (int)min((int64_t)32, g.N - (c0 + c));
+          if (count <= 0) continue;
 #pragma unroll
-          for (int j = 0; j < kCh; ++j) {
-            const int64_t m = c0 + c + j;
-            if (m >= g.N) continue;
-            float v = x[j] + rb;
-            if (e.pre != nullptr) store1(e.pre, m * e.ldpre + r, e.dtype, v);
-            v = activate(v, e.act);
-            if (e.residual != nullptr) v += load1(e.residual, m * e.ldr + r, e.dtype);
-            store1(e.y, m * e.ldy + r, e.dtype, v);
-          }
+          for (int j = 0; j < 32; ++j) x[j] += rb;
+          if (e.pre != nullptr)
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < count) store1(e.pre, (c0 + c + j) * e.ldpre + r, e.dtype, x[j]);
+          activate_all(x, e.act);
+          if (e.residual != nullptr)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] += load1(e.residual, (c0 + c + min(j, count - 1)) * e.ldr + r, e.dtype);
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (j < count) store1(e.y, (c0 + c + j) * e.ldy + r, e.dtype, x[j]);
           continue;
         }
+        const int64_t left = g.N - (c0 + c);
+        if (e.pre != nullptr)
 #pragma unroll
-        for (int j = 0; j < kCh; j += 8) {
-          const int64_t left = g.N - (c0 + c + j);
-          const int count = left < 8 ? (left < 0 ? 0 : (int)left) : 8;
-          if (e.pre != nullptr) store8(e.pre, r * e.ldpre + c0 + c + j, e.dtype, x + j, count, vec);
-          if (e.act != QRB_ACT_NONE) {
+          for (int j = 0; j < 32; j += 8)
+            store8(e.pre, r * e.ldpre + c0 + c + j, e.dtype, x + j, (int)max((int64_t)0, min((int64_t)8, left - j)), vec);
+        activate_all(x, e.act);
+        if (e.residual != nullptr)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[j + i] = activate(x[j + i], e.act);
-          }
-          if (e.residual != nullptr) add8(e.residual, r * e.ldr + c0 + c + j, e.dtype, x + j, count, vec);
-          store8(e.y, r * e.ldy + c0 + c + j, e.dtype, x + j, count, vec);
-        }
+          for (int j = 0; j < 32; j += 8)
+            add8(e.residual, r * e.ldr + c0 + c + j, e.dtype, x + j, (int)max((int64_t)0, min((int64_t)8, left - j)), vec);
+#pragma unroll
+        for (int j = 0; j < 32; j += 8)
+          store8(e.y, r * e.ldy + c0 + c + j, e.dtype, x + j, (int)max((int64_t)0, min((int64_t)8, left - j)), vec);
       }
     }
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync_all();   // neither block leaves while the other may still reach its memory
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, cols);
+    if (PAIR) tmem_dealloc_pair(tmem, cols);
+    else tmem_dealloc(tmem, cols);
   }
 }
 
 // y = epilogue(sum of the splits' partials, in order).
 __global__ void __launch_bounds__(256) reduce_kernel(const float* part, int splits, int64_t m, int64_t n, Epilogue e) {
-  const int64_t total = m * n;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+  const int64_t total = m * n, c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= n) return;
+  const float b = e.bias != nullptr ? load1(e.bias, c, e.dtype) : 0.f;
+  for (int64_t r = blockIdx.y; r < m; r += gridDim.y) {
     float x = 0.f;
-    for (int s = 0; s < splits; ++s) x += part[s * total + i];
-    const int64_t r = i / n, c = i - r * n;
-    if (e.bias != nullptr) x += load1(e.bias, c, e.dtype);
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) x += part[s * total + r * n + c];
+    x += b;
     if (e.pre != nullptr) store1(e.pre, r * e.ldpre + c, e.dtype, x);
     x = activate(x, e.act);
     if (e.residual != nullptr) x += load1(e.residual, r * e.ldr + c, e.dtype);
@@ -414,34 +458,36 @@ bool make_map(CUtensorMap* map, const Operand& o, int64_t mn, int64_t k, bool ha
 }
 
 struct Plan {
-  int bn, swap, tiles_m, tiles_n, splits, kblocks, per_split;
+  int bn, swap, pair, tiles_m, tiles_n, splits, kblocks, per_split;
 };
 
-// Tile width and split of an m x n x k product.  Up to 128 rows: swapped, the narrowest tile that
-// holds them.  Otherwise the widest of 256, 128, 64 columns whose tiles still fill two thirds of the
-// SMs (a wide tile reads the least shared memory per MMA, an idle SM costs more), and where even 64
-// does not, k is split.
+// Tile shape and split of an m x n x k product.  Up to 128 rows: swapped, the narrowest tile that
+// holds them.  Otherwise pairs on 256 x 256 where these fill two thirds of the SMs (or nearly: the
+// last, partly filled wave counts), then the widest single tile that does (a wide tile reads the least
+// shared memory per MMA, an idle SM costs more), and where even 64 columns do not, k is split.
 Plan plan(int64_t m, int64_t n, int64_t k, int pieces) {
   Plan p{};
   const int sms = sm_count();
   p.kblocks = (int)((k + kBK - 1) / kBK);
   p.swap = m <= 128;
-  auto tiles = [&](int bn) {
+  auto tiles = [&](int bn, int pair) {
     p.bn = bn;
-    p.tiles_m = (int)(((p.swap ? n : m) + kBM - 1) / kBM);
+    p.pair = pair;
+    p.tiles_m = (int)(((p.swap ? n : m) + kBM * (1 + pair) - 1) / (kBM * (1 + pair)));
     p.tiles_n = (int)(((p.swap ? m : n) + bn - 1) / bn);
     return (int64_t)p.tiles_m * p.tiles_n;
   };
   int64_t t;
   if (p.swap) {
-    t = tiles(m <= 64 ? 64 : 128);
+    t = tiles(m <= 64 ? 64 : 128, 0);
   } else {
-    t = tiles(256);
-    if (t * 3 < sms * 2) t = tiles(128);
-    if (t * 3 < sms * 2) t = tiles(64);
+    t = tiles(256, 1);
+    if (t * 3 < sms) t = tiles(256, 0);
+    if (!p.pair && t * 3 < sms * 2) t = tiles(128, 0);
+    if (!p.pair && t * 3 < sms * 2) t = tiles(64, 0);
   }
   // a split is worth at least four stages of work, and there are 16 at most
-  int64_t splits = t * 2 <= sms ? sms / t : 1;
+  int64_t splits = !p.pair && t * 2 <= sms ? sms / t : 1;
   if (splits > (p.kblocks + 3) / 4) splits = (p.kblocks + 3) / 4;
   if (splits > 16) splits = 16;
   if (splits < 1) splits = 1;
@@ -454,15 +500,25 @@ Plan plan(int64_t m, int64_t n, int64_t k, int pieces) {
   return p;
 }
 
-template <int BN>
+template <int BN, bool PAIR>
 cudaError_t run(const CUtensorMap& ma, const CUtensorMap& mb, const GemmArgs& g, cudaStream_t s) {
-  constexpr int smem = Cfg<BN>::kSmem;
-  cudaError_t e = cudaFuncSetAttribute(gemm_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  constexpr int smem = Cfg<BN, PAIR>::kSmem;
+  cudaError_t e = cudaFuncSetAttribute(gemm_kernel<BN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   const int64_t units = (int64_t)g.tiles_m * g.tiles_n * g.splits;
-  const int sms = sm_count();
-  gemm_kernel<BN><<<(unsigned)(units < sms ? units : sms), kThreads, smem, s>>>(ma, mb, g);
-  return cudaGetLastError();
+  const int sms = PAIR ? sm_count() / 2 : sm_count(), grid = (int)(units < sms ? units : sms);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(PAIR ? 2 * grid : grid));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, gemm_kernel<BN, PAIR>, ma, mb, g);
 }
 
 }  // namespace
@@ -494,7 +550,7 @@ cudaError_t multiply(const Operand& A, const Operand& B, int64_t m, int64_t n, i
   g.swap = p.swap;
   const uint32_t fmt = half ? 0 : 1;
   g.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a.mn_major << 15) | ((uint32_t)b.mn_major << 16) |
-            ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
+            ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)((p.pair ? 2 * kBM : kBM) >> 4) << 24);
   if (a.pieces == 1) {
     g.terms = 1;
     g.sets = 1;
@@ -515,21 +571,19 @@ cudaError_t multiply(const Operand& A, const Operand& B, int64_t m, int64_t n, i
   g.err = device_error_flag();
   if (g.err == nullptr) return cudaErrorInvalidValue;
   CUtensorMap ma, mb;
-  if (!make_map(&ma, a, g.M, k, half, kBM) || !make_map(&mb, b, g.N, k, half, p.bn)) return cudaErrorInvalidValue;
+  if (!make_map(&ma, a, g.M, k, half, kBM) || !make_map(&mb, b, g.N, k, half, p.pair ? p.bn / 2 : p.bn)) return cudaErrorInvalidValue;
   cudaError_t r;
   {
     const double bytes = (double)(m * k + n * k) * 2 * A.pieces + (double)m * n * (e.dtype == QRB_F32 ? 4 : 2);
     LaunchTimer t("linear_gemm_kernel", s, bytes, 2.0 * m * n * k);
-    switch (p.bn) {
-      case 64: r = run<64>(ma, mb, g, s); break;
-      case 128: r = run<128>(ma, mb, g, s); break;
-      default: r = run<256>(ma, mb, g, s); break;
-    }
+    if (p.pair) r = run<256, true>(ma, mb, g, s);
+    else if (p.bn == 64) r = run<64, false>(ma, mb, g, s);
+    else if (p.bn == 128) r = run<128, false>(ma, mb, g, s);
+    else r = run<256, false>(ma, mb, g, s);
   }
   if (r != cudaSuccess || p.splits == 1) return r;
   LaunchTimer t("linear_reduce_kernel", s, 4.0 * p.splits * m * n, (double)p.splits * m * n);
-  const int64_t blocks = (m * n + 255) / 256, most = (int64_t)sm_count() * 8;
-  reduce_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(ws, p.splits, m, n, e);
+  reduce_kernel<<<dim3((unsigned)((n + 255) / 256), (unsigned)(m < 1024 ? m : 1024)), 256, 0, s>>>(ws, p.splits, m, n, e);
   return cudaGetLastError();
 }
 

@@ -40,11 +40,60 @@ cudaError_t multiply(const Operand& A, const Operand& B, int64_t m, int64_t n, i
 int launches(int64_t m, int64_t n, int64_t k, int pieces);
 bool supported();   // the driver's tensor map encoder is there
 
+// Phi(x), the normal distribution function, without a branch: with z = |x| / sqrt 2 and
+// t = 1 / (1 + z / 2), erfc(z) = t exp(-z^2 + q(t)); q is the degree-9 Chebyshev fit of
+// ln(erfc(z) / t) + z^2 on t in [0.05, 1] (below it erfc underflows), computed in 64 bits, within
+// 8e-8 of it, 2.2e-7 evaluated in fp32; the exponential adds its argument's rounding.
+// (erff takes two paths that a warp walks one after the other, which cost a GELU epilogue 215 cycles
+// a value.)
+__device__ __forceinline__ float phi(float x) {
+  const float z = fabsf(x) * 0.70710678118654752f;
+  const float t = __fdividef(1.f, fmaf(0.5f, z, 1.f));
+  float q = 1.744112854e-01f;
+  q = fmaf(q, t, -8.387804970e-01f);
+  q = fmaf(q, t, 1.521343200e+00f);
+  q = fmaf(q, t, -1.170532379e+00f);
+  q = fmaf(q, t, 3.013534328e-01f);
+  q = fmaf(q, t, -1.948683954e-01f);
+  q = fmaf(q, t, 9.867874417e-02f);
+  q = fmaf(q, t, 3.738729275e-01f);
+  q = fmaf(q, t, 1.000034051e+00f);
+  q = fmaf(q, t, -1.265512294e+00f);
+  const float half = 0.5f * t * __expf(fmaf(-z, z, q));   // erfc(z) / 2
+  return x < 0.f ? half : 1.f - half;
+}
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+
 __device__ __forceinline__ float activate(float x, int act) {
   if (act == QRB_ACT_RELU) return x > 0.f ? x : (x != x ? x : 0.f);
-  if (act == QRB_ACT_SILU) return x / (1.f + expf(-x));
-  if (act == QRB_ACT_GELU) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
+  if (act == QRB_ACT_SILU) return x * sigmoid(x);
+  if (act == QRB_ACT_GELU) return x * phi(x);
   return x;
+}
+__device__ __forceinline__ float slope(float x, int act) {
+  if (act == QRB_ACT_RELU) return x > 0.f ? 1.f : (x != x ? x : 0.f);
+  if (act == QRB_ACT_SILU) {
+    const float s = sigmoid(x);
+    return s * (1.f + x * (1.f - s));
+  }
+  if (act == QRB_ACT_GELU) return phi(x) + x * 0.39894228040143268f * __expf(-0.5f * x * x);
+  return 1.f;
+}
+
+// act over N values at once: one test for all of them.
+template <int N>
+__device__ __forceinline__ void activate_all(float (&x)[N], int act) {
+  if (act == QRB_ACT_NONE) return;
+  if (act == QRB_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = activate(x[i], QRB_ACT_RELU);
+  } else if (act == QRB_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = activate(x[i], QRB_ACT_SILU);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = activate(x[i], QRB_ACT_GELU);
+  }
 }
 
 }  // namespace gemm

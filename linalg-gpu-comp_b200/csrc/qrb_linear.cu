@@ -53,26 +53,48 @@ __device__ __forceinline__ void put<float>(void* to, int64_t i, int64_t plane, f
   p[i + 2 * plane] = __float2bfloat16_rn(r - __bfloat162float(b));
 }
 
-// rows x cols of `from` (row stride ld) to rows of `pitch` elements.
+template <typename T>
+__device__ __forceinline__ void put8(void* to, int64_t i, int64_t plane, const T (&e)[8], int count) {
+  constexpr int P = sizeof(T) == 4 ? 3 : 1;
+  uint32_t w[P][4];
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    if (P == 1) {
+      T pair[2] = {j < count ? e[j] : fromf<T>(0.f), j + 1 < count ? e[j + 1] : fromf<T>(0.f)};
+      w[0][j / 2] = *reinterpret_cast<const uint32_t*>(pair);
+    } else {
+      __align__(4) __nv_bfloat16 pc[3][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float x = j + h < count ? tof(e[j + h]) : 0.f;
+        pc[0][h] = __float2bfloat16_rn(x);
+        float r = x - __bfloat162float(pc[0][h]);
+        if (!(fabsf(r) <= 3.4e38f)) r = 0.f;
+        pc[1][h] = __float2bfloat16_rn(r);
+        pc[2][h] = __float2bfloat16_rn(r - __bfloat162float(pc[1][h]));
+      }
+#pragma unroll
+      for (int q = 0; q < P; ++q) w[q][j / 2] = *reinterpret_cast<const uint32_t*>(pc[q]);
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < P; ++q)
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(to) + i + q * plane) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+}
+
+// rows x cols of `from` (row stride ld) to rows of `pitch` elements: eight columns a thread, stored as
+// 16-byte units (the columns that pad a row become zero).
 template <typename T>
 __global__ void __launch_bounds__(256) layout_kernel(const T* from, int64_t ld, int64_t rows, int64_t cols, void* to,
                                                      int64_t pitch) {
-  const int64_t total = rows * cols, plane = rows * pitch;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / cols, c = i - r * cols;
-    put<T>(to, r * pitch + c, plane, tof(from[r * ld + c]));
+  const int64_t c = ((int64_t)blockIdx.x * 32 + (threadIdx.x & 31)) * 8, plane = rows * pitch;
+  if (c >= pitch) return;
+  for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.y * 8) {
+    T e[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e[j] = __ldg(from + r * ld + min(c + j, cols - 1));
+    put8<T>(to, r * pitch + c, plane, e, (int)min((int64_t)8, cols - c));
   }
-}
-
-__device__ __forceinline__ float slope(float x, int act) {
-  if (act == QRB_ACT_RELU) return x > 0.f ? 1.f : (x != x ? x : 0.f);
-  if (act == QRB_ACT_SILU) {
-    const float s = 1.f / (1.f + expf(-x));
-    return s * (1.f + x * (1.f - s));
-  }
-  if (act == QRB_ACT_GELU)
-    return 0.5f * (1.f + erff(x * 0.70710678118654752f)) + x * 0.39894228040143268f * expf(-0.5f * x * x);
-  return 1.f;
 }
 
 constexpr int kSumRows = 128, kSumCols = 64;   // rows and columns a block of dp_kernel covers
@@ -213,15 +235,11 @@ int check_ws(const void* ws, size_t have, size_t need) {
   return QRB_OK;
 }
 
-unsigned elem_grid(int64_t total) {
-  const int64_t blocks = (total + 255) / 256, most = (int64_t)qrb::sm_count() * 16;
-  return (unsigned)(blocks < most ? blocks : most);
-}
-
 template <typename T>
 void layout_t(const void* p, int64_t ld, int64_t rows, int64_t cols, void* to, cudaStream_t s) {
-  qrb::gemm::layout_kernel<T><<<elem_grid(rows * cols), 256, 0, s>>>(static_cast<const T*>(p), ld, rows, cols, to,
-                                                                    pitch_of(cols));
+  const int64_t pitch = pitch_of(cols), by = (rows + 7) / 8;
+  const dim3 grid((unsigned)((pitch + 255) / 256), (unsigned)(by < 4096 ? by : 4096));
+  qrb::gemm::layout_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(p), ld, rows, cols, to, pitch);
 }
 
 // The operand a product reads: x itself, or its copy at `to`.
