@@ -94,17 +94,6 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t ad, uint64_t b
       : "memory");
 }
 
-__device__ __forceinline__ float load1(const void* p, int64_t i, int dtype) {
-  if (dtype == QRB_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  if (dtype == QRB_F16) return __half2float(static_cast<const __half*>(p)[i]);
-  return static_cast<const float*>(p)[i];
-}
-__device__ __forceinline__ void store1(void* p, int64_t i, int dtype, float x) {
-  if (dtype == QRB_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
-  else if (dtype == QRB_F16) static_cast<__half*>(p)[i] = __float2half_rn(x);
-  else static_cast<float*>(p)[i] = x;
-}
-
 __device__ __forceinline__ uint32_t pack16(float a, float b, int dtype) {
   if (dtype == QRB_BF16) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
@@ -150,9 +139,12 @@ __device__ __forceinline__ void add8(const void* p, int64_t i, int dtype, float*
     }
     return;
   }
+  if (count <= 0) return;
+  float y[8];   // all loads first: one under a condition would be waited for before the next
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < count) x[j] += load1(p, i + j, dtype);
+  for (int j = 0; j < 8; ++j) y[j] = load1(p, i + min(j, count - 1), dtype);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] += y[j];
 }
 
 __device__ __forceinline__ bool aligned_rows(const void* p, int64_t ld, int dtype) {

@@ -1,6 +1,8 @@
 // Dense products of the linear layer (qrb_gemm.cu), used by qrb_linear.cu.
 #pragma once
 
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -39,6 +41,17 @@ cudaError_t multiply(const Operand& A, const Operand& B, int64_t m, int64_t n, i
                      float* ws, cudaStream_t s);
 int launches(int64_t m, int64_t n, int64_t k, int pieces);
 bool supported();   // the driver's tensor map encoder is there
+
+__device__ __forceinline__ float load1(const void* p, int64_t i, int dtype) {
+  if (dtype == QRB_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  if (dtype == QRB_F16) return __half2float(static_cast<const __half*>(p)[i]);
+  return static_cast<const float*>(p)[i];
+}
+__device__ __forceinline__ void store1(void* p, int64_t i, int dtype, float x) {
+  if (dtype == QRB_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+  else if (dtype == QRB_F16) static_cast<__half*>(p)[i] = __float2half_rn(x);
+  else static_cast<float*>(p)[i] = x;
+}
 
 // Phi(x), the normal distribution function, without a branch: with z = |x| / sqrt 2 and
 // t = 1 / (1 + z / 2), erfc(z) = t exp(-z^2 + q(t)); q is the degree-9 Chebyshev fit of

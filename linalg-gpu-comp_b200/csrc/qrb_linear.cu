@@ -1,7 +1,7 @@
 // The linear layer y = act(x w^T + b) + r and its backward pass: C ABI (include/qrb200_nn.h), and
 // the elementwise kernels around the products of qrb_gemm.cu.
 //
-//   forward:  [lay out x, w] product with the epilogue
+//   forward:  up to four rows: gemv_kernel; otherwise [lay out x, w] product with the epilogue
 //   backward: dp = dy act'(pre) and the column sums of dp (dbias), then dx = dp w, dw = dp^T x
 // Operands the tensor maps cannot address (rows not 16-byte aligned) are laid out in the workspace
 // first, fp32 ones as three bf16 planes.  dp of the 16-bit types is rounded to the type once: it is
@@ -35,38 +35,23 @@ __device__ __forceinline__ __nv_bfloat16 fromf(float x) { return __float2bfloat1
 template <>
 __device__ __forceinline__ __half fromf(float x) { return __float2half_rn(x); }
 
-// One value of a laid-out operand: the value itself, or the three bf16 planes of an fp32 one.  A
-// value that is not finite keeps its first plane only (inf - inf would put NaN into the others).
+// Eight neighbouring values of a laid-out operand (those behind `count` become zero): the values
+// themselves, or the three bf16 planes of fp32 ones.  A value that is not finite keeps its first plane
+// only (inf - inf would put NaN into the others).
 template <typename T>
-__device__ __forceinline__ void put(void* to, int64_t i, int64_t plane, float x) {
-  static_cast<T*>(to)[i] = fromf<T>(x);
-}
-template <>
-__device__ __forceinline__ void put<float>(void* to, int64_t i, int64_t plane, float x) {
-  __nv_bfloat16* p = static_cast<__nv_bfloat16*>(to);
-  const __nv_bfloat16 a = __float2bfloat16_rn(x);
-  float r = x - __bfloat162float(a);
-  if (!(fabsf(r) <= 3.4e38f)) r = 0.f;
-  const __nv_bfloat16 b = __float2bfloat16_rn(r);
-  p[i] = a;
-  p[i + plane] = b;
-  p[i + 2 * plane] = __float2bfloat16_rn(r - __bfloat162float(b));
-}
-
-template <typename T>
-__device__ __forceinline__ void put8(void* to, int64_t i, int64_t plane, const T (&e)[8], int count) {
+__device__ __forceinline__ void put8f(void* to, int64_t i, int64_t plane, const float (&e)[8], int count) {
   constexpr int P = sizeof(T) == 4 ? 3 : 1;
   uint32_t w[P][4];
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
     if (P == 1) {
-      T pair[2] = {j < count ? e[j] : fromf<T>(0.f), j + 1 < count ? e[j + 1] : fromf<T>(0.f)};
+      T pair[2] = {fromf<T>(j < count ? e[j] : 0.f), fromf<T>(j + 1 < count ? e[j + 1] : 0.f)};
       w[0][j / 2] = *reinterpret_cast<const uint32_t*>(pair);
     } else {
       __align__(4) __nv_bfloat16 pc[3][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float x = j + h < count ? tof(e[j + h]) : 0.f;
+        const float x = j + h < count ? e[j + h] : 0.f;
         pc[0][h] = __float2bfloat16_rn(x);
         float r = x - __bfloat162float(pc[0][h]);
         if (!(fabsf(r) <= 3.4e38f)) r = 0.f;
@@ -90,40 +75,76 @@ __global__ void __launch_bounds__(256) layout_kernel(const T* from, int64_t ld, 
   const int64_t c = ((int64_t)blockIdx.x * 32 + (threadIdx.x & 31)) * 8, plane = rows * pitch;
   if (c >= pitch) return;
   for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.y * 8) {
-    T e[8];
+    float e[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = __ldg(from + r * ld + min(c + j, cols - 1));
-    put8<T>(to, r * pitch + c, plane, e, (int)min((int64_t)8, cols - c));
+    for (int j = 0; j < 8; ++j) e[j] = tof(__ldg(from + r * ld + min(c + j, cols - 1)));
+    put8f<T>(to, r * pitch + c, plane, e, (int)min((int64_t)8, cols - c));
   }
 }
 
-constexpr int kSumRows = 128, kSumCols = 64;   // rows and columns a block of dp_kernel covers
+constexpr int kSumRows = 64, kSumCols = 256;   // rows and columns a block of dp_kernel covers
+
+// Eight neighbouring values; VEC: one or two 16-byte loads, otherwise existing columns only.
+template <typename T, bool VEC>
+__device__ __forceinline__ void get8(const T* p, int count, T (&e)[8]) {
+  if (VEC) {
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T) / 2; ++j)
+      reinterpret_cast<uint4*>(e)[j] = __ldg(reinterpret_cast<const uint4*>(p) + j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e[j] = __ldg(p + min(j, count - 1));
+  }
+}
 
 // dp = dy act'(pre) into a laid-out operand (to, unless null) and its column sums over the block's
-// rows (sums[row block][n], unless null).  Sums are of the fp32 products, before any rounding.
-template <typename T>
+// rows (sums[row block][n], unless null).  Sums are of the fp32 products, before any rounding.  A
+// thread takes eight columns of every eighth row, four rows in flight.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dp_kernel(const T* dy, int64_t ldy, const T* pre, int64_t ldp, int act,
                                                  int64_t m, int64_t n, void* to, int64_t pitch, float* sums) {
-  __shared__ float part[4][kSumCols];
-  const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
-  const int64_t col = (int64_t)blockIdx.x * kSumCols + c, r0 = (int64_t)blockIdx.y * kSumRows;
-  float s = 0.f;
-  if (col < n) {
-#pragma unroll 8
-    for (int i = g; i < kSumRows; i += 4) {
-      const int64_t r = r0 + i;
-      if (r >= m) break;
-      float x = tof(dy[r * ldy + col]);
-      if (act != QRB_ACT_NONE) x *= slope(tof(pre[r * ldp + col]), act);
-      s += x;
-      if (to != nullptr) put<T>(to, r * pitch + col, m * pitch, x);
+  __shared__ float part[8][kSumCols];
+  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int64_t col = (int64_t)blockIdx.x * kSumCols + 8 * lane, r0 = (int64_t)blockIdx.y * kSumRows;
+  const int count = (int)min((int64_t)8, n - col);
+  float s[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s[j] = 0.f;
+  if (count > 0) {
+    for (int i = g; i < kSumRows; i += 32) {
+      alignas(16) T a[4][8], b[4][8];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t r = min(r0 + i + 8 * u, m - 1);
+        get8<T, VEC>(dy + r * ldy + col, count, a[u]);
+        if (act != QRB_ACT_NONE) get8<T, VEC>(pre + r * ldp + col, count, b[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t r = r0 + i + 8 * u;
+        if (r >= m) continue;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[j] = tof(a[u][j]);
+          if (act != QRB_ACT_NONE) x[j] *= slope(tof(b[u][j]), act);
+          s[j] += x[j];
+        }
+        if (to != nullptr) put8f<T>(to, r * pitch + col, m * pitch, x, count);
+      }
     }
   }
   if (sums == nullptr) return;
-  part[g][c] = s;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) part[g][8 * lane + j] = s[j];
   __syncthreads();
-  if (g == 0 && col < n)
-    sums[(int64_t)blockIdx.y * n + col] = (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
+  const int c = threadIdx.x;
+  if ((int64_t)blockIdx.x * kSumCols + c < n) {
+    float t = part[0][c];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) t += part[i][c];
+    sums[(int64_t)blockIdx.y * n + (int64_t)blockIdx.x * kSumCols + c] = t;
+  }
 }
 
 template <typename T>
@@ -140,6 +161,84 @@ __global__ void __launch_bounds__(256) colsum_kernel(const float* sums, int64_t 
     for (int i = 1; i < 8; ++i) s += part[i][c];
     out[col] = fromf<T>(s);
   }
+}
+
+// y = epilogue(x w^T) for up to four rows, which the weight's bytes bound: a warp (SPLIT: the eight
+// warps of a block, for outputs too few to fill the card with warps) takes one row of w, 16 bytes a
+// lane and eight loads in flight; x comes from L1.  fp32 sums in a fixed order.
+template <typename T, int M, bool VEC, bool SPLIT>
+__global__ void __launch_bounds__(256) gemv_kernel(const T* x, int64_t ldx, const T* w, int64_t ldw, int64_t k, int64_t n,
+                                                   Epilogue e) {
+  constexpr int V = 16 / (int)sizeof(T), U = 8;   // elements a lane takes at once, times in flight
+  __shared__ float part[8][M];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = SPLIT ? blockIdx.x : (int64_t)blockIdx.x * 8 + warp;
+  if (!SPLIT && c >= n) return;
+  const T* wr = w + c * ldw;
+  float s[M];
+#pragma unroll
+  for (int i = 0; i < M; ++i) s[i] = 0.f;
+  const int64_t step = (SPLIT ? 8 : 1) * 32 * V, begin = (SPLIT ? threadIdx.x : lane) * V;
+  // the same elements to the same lane whatever the alignment: results do not depend on it
+  auto get = [&](T (&to)[V], const T* from, int64_t at) {
+    if (VEC) {
+      *reinterpret_cast<uint4*>(to) = __ldg(reinterpret_cast<const uint4*>(from + at));
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) to[j] = __ldg(from + min(at + j, k - 1));
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (at + j >= k) to[j] = fromf<T>(0.f);
+    }
+  };
+  auto use = [&](const T (&we)[V], int64_t at) {
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      alignas(16) T xe[V];
+      get(xe, x + i * ldx, at);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[i] = fmaf(tof(we[j]), tof(xe[j]), s[i]);
+    }
+  };
+  int64_t at = begin;
+  for (; at + (U - 1) * step < k; at += U * step) {
+    alignas(16) T we[U][V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) get(we[u], wr, at + u * step);
+#pragma unroll
+    for (int u = 0; u < U; ++u) use(we[u], at + u * step);
+  }
+  for (; at < k; at += step) {
+    alignas(16) T we[V];
+    get(we, wr, at);
+    use(we, at);
+  }
+#pragma unroll
+  for (int i = 0; i < M; ++i) s[i] = warp_sum(s[i]);
+  if (SPLIT) {
+    if (lane == 0)
+#pragma unroll
+      for (int i = 0; i < M; ++i) part[warp][i] = s[i];
+    __syncthreads();
+    if (threadIdx.x >= M) return;
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+      if (i == (int)threadIdx.x) {
+        s[0] = part[0][i];
+        for (int j = 1; j < 8; ++j) s[0] += part[j][i];
+      }
+  } else {
+#pragma unroll
+    for (int i = 1; i < M; ++i)
+      if (lane == i) s[0] = s[i];
+    if (lane >= M) return;
+  }
+  const int64_t r = SPLIT ? threadIdx.x : lane;   // lane r finishes row r
+  float v = s[0] + (e.bias != nullptr ? load1(e.bias, c, e.dtype) : 0.f);
+  if (e.pre != nullptr) store1(e.pre, r * e.ldpre + c, e.dtype, v);
+  v = activate(v, e.act);
+  if (e.residual != nullptr) v += load1(e.residual, r * e.ldr + c, e.dtype);
+  store1(e.y, r * e.ldy + c, e.dtype, v);
 }
 
 }  // namespace
@@ -193,7 +292,7 @@ int check_common(int dtype, int act, int64_t m, int64_t k, int64_t n) {
                 (long long)n);
   const int64_t top = (int64_t)1 << 30;
   if (m > top || n > top || k > top || (m > 0 && m * n / (128 * 64) > top / 16) || k * n / (128 * 64) > top / 16 ||
-      m * k / (128 * 64) > top / 16 || m > (int64_t)128 * 65535)
+      m * k / (128 * 64) > top / 16 || m > (int64_t)64 * 65535)
     return fail(QRB_ERR_UNSUPPORTED, "sizes m = %lld, k = %lld, n = %lld are too large", (long long)m, (long long)k,
                 (long long)n);
   return QRB_OK;
@@ -264,11 +363,45 @@ int operand(Operand& o, int dtype, const void* p, int64_t ld, int64_t rows, int6
   return QRB_OK;
 }
 
+constexpr int64_t kVecRows = 4;   // up to here gemv_kernel: it reads the weight once and lays nothing out
+
+template <typename T, int M>
+cudaError_t run_gemv(const qrb_linear_args& a, const Epilogue& e, cudaStream_t s) {
+  const int64_t v = 16 / (int64_t)sizeof(T);
+  const bool vec = a.k % v == 0 && a.ldx % v == 0 && a.ldw % v == 0 &&
+                   ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w)) & 15u) == 0;
+  // eight warps a column where a warp each would leave most of the card without one
+  const bool split = a.n < 4 * (int64_t)qrb::sm_count() && a.k >= 1024;
+  const T *x = static_cast<const T*>(a.x), *w = static_cast<const T*>(a.w);
+  const unsigned grid = (unsigned)(split ? a.n : (a.n + 7) / 8);
+  qrb::LaunchTimer t("linear_gemv_kernel", s, (double)(a.m + a.n) * a.k * sizeof(T), 2.0 * a.m * a.n * a.k);
+  using namespace qrb::gemm;
+  if (vec) {
+    if (split) gemv_kernel<T, M, true, true><<<grid, 256, 0, s>>>(x, a.ldx, w, a.ldw, a.k, a.n, e);
+    else gemv_kernel<T, M, true, false><<<grid, 256, 0, s>>>(x, a.ldx, w, a.ldw, a.k, a.n, e);
+  } else {
+    if (split) gemv_kernel<T, M, false, true><<<grid, 256, 0, s>>>(x, a.ldx, w, a.ldw, a.k, a.n, e);
+    else gemv_kernel<T, M, false, false><<<grid, 256, 0, s>>>(x, a.ldx, w, a.ldw, a.k, a.n, e);
+  }
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t pick_gemv(const qrb_linear_args& a, const Epilogue& e, cudaStream_t s) {
+  switch (a.m) {
+    case 1: return run_gemv<T, 1>(a, e, s);
+    case 2: return run_gemv<T, 2>(a, e, s);
+    case 3: return run_gemv<T, 3>(a, e, s);
+    default: return run_gemv<T, 4>(a, e, s);
+  }
+}
+
 struct FwdLayout {
   size_t x, w, part, total;
 };
 FwdLayout fwd_layout(const qrb_linear_args& a) {
   FwdLayout l{};
+  if (a.m <= kVecRows) return l;
   size_t at = 0;
   l.x = at;
   if (!direct(a.dtype, a.x, a.ldx, a.k)) at += layout_bytes(a.dtype, a.m, a.k);
@@ -305,7 +438,7 @@ BwdLayout bwd_layout(const qrb_linear_backward_args& a) {
   l.w = at;
   if (!direct(a.dtype, a.w, a.ldw, a.k)) at += layout_bytes(a.dtype, a.n, a.k);
   l.sums = at;
-  at += al((size_t)((a.m + 127) / 128) * a.n * 4);
+  at += al((size_t)((a.m + qrb::gemm::kSumRows - 1) / qrb::gemm::kSumRows) * a.n * 4);
   l.part = at;
   size_t p1 = qrb::gemm::scratch(a.m, a.k, a.n, pieces), p2 = qrb::gemm::scratch(a.n, a.k, a.m, pieces);
   at += al((p1 > p2 ? p1 : p2) * 4);
@@ -329,8 +462,13 @@ int run_dp(const qrb_linear_backward_args& a, void* to, float* sums, cudaStream_
   {
     qrb::LaunchTimer t("linear_dp_kernel", s, (double)a.m * a.n * sizeof(T) * 3, (double)a.m * a.n);
     const dim3 grid((unsigned)((a.n + qrb::gemm::kSumCols - 1) / qrb::gemm::kSumCols), (unsigned)rb);
-    qrb::gemm::dp_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(a.dy), a.lddy, static_cast<const T*>(a.pre),
-                                                 a.ldpre, a.activation, a.m, a.n, to, pitch_of(a.n), sums);
+    const int64_t v = 16 / (int64_t)sizeof(T);
+    const bool vec = a.n % 8 == 0 && a.lddy % v == 0 && (reinterpret_cast<uintptr_t>(a.dy) & 15u) == 0 &&
+                     (a.activation == QRB_ACT_NONE ||
+                      (a.ldpre % v == 0 && (reinterpret_cast<uintptr_t>(a.pre) & 15u) == 0));
+    auto kernel = vec ? qrb::gemm::dp_kernel<T, true> : qrb::gemm::dp_kernel<T, false>;
+    kernel<<<grid, 256, 0, s>>>(static_cast<const T*>(a.dy), a.lddy, static_cast<const T*>(a.pre), a.ldpre, a.activation,
+                                a.m, a.n, to, pitch_of(a.n), sums);
     CUDA(cudaGetLastError(), "linear dp launch");
   }
   if (sums != nullptr) {
@@ -370,11 +508,18 @@ int qrb_linear_forward(const qrb_linear_args* a, void* ws, size_t wsb, void* str
   TRY(check_ws(ws, wsb, l.total));
   TRY(check_device());
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const Epilogue e{a->dtype, a->activation, a->y, a->ldy, a->bias, a->residual, a->ldr, a->pre, a->ldpre};
+  if (a->m <= kVecRows) {
+    CUDA(a->dtype == QRB_F32    ? pick_gemv<float>(*a, e, s)
+         : a->dtype == QRB_BF16 ? pick_gemv<__nv_bfloat16>(*a, e, s)
+                                : pick_gemv<__half>(*a, e, s),
+         "linear few-row launch");
+    return QRB_OK;
+  }
   char* w8 = static_cast<char*>(ws);
   Operand x, w;
   TRY(operand(x, a->dtype, a->x, a->ldx, a->m, a->k, false, w8 + l.x, s));
   TRY(operand(w, a->dtype, a->w, a->ldw, a->n, a->k, false, w8 + l.w, s));
-  const Epilogue e{a->dtype, a->activation, a->y, a->ldy, a->bias, a->residual, a->ldr, a->pre, a->ldpre};
   CUDA(qrb::gemm::multiply(x, w, a->m, a->n, a->k, a->dtype == QRB_F16, e, reinterpret_cast<float*>(w8 + l.part), s),
        "linear product launch");
   return QRB_OK;
