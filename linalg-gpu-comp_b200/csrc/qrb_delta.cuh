@@ -341,11 +341,5 @@ cudaError_t launch_rscan(const Params& p, int dtype, cudaStream_t s);
 cudaError_t launch_grad(const Params& p, int dtype, cudaStream_t s);
 cudaError_t launch_step(const qrb_delta_step_args& a, cudaStream_t s);
 
-// Raises a kernel's dynamic shared memory limit on every device it runs on (the attribute belongs to the device).
-template <typename F>
-cudaError_t allow_smem(F* f, int bytes) {
-  return cudaFuncSetAttribute(reinterpret_cast<const void*>(f), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
 }  // namespace delta
 }  // namespace qrb

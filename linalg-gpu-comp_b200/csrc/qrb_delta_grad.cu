@@ -200,7 +200,7 @@ cudaError_t run_grad(const Params& p, cudaStream_t s) {
   static_assert(smem <= 232448, "shared memory of one block");
   const double rows = (double)p.bound * kChunk * p.hv;
   LaunchTimer t("delta_grad_kernel", s, rows * 4.0 * p.dk * sizeof(T), rows * (6.0 * p.dv + 8.0 * kChunk) * p.dk);
-  cudaError_t e = allow_smem(grad_kernel<DKP, T>, smem);
+  cudaError_t e = allow_smem<grad_kernel<DKP, T>>(smem);
   if (e != cudaSuccess) return e;
   grad_kernel<DKP, T><<<dim3((unsigned)p.bound, (unsigned)p.hk), 512, smem, s>>>(p);
   return cudaGetLastError();

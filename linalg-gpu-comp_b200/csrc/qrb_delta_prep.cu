@@ -416,7 +416,7 @@ cudaError_t run_prep(const Params& p, cudaStream_t s) {
   const int vec = (dk_ok && fits(p.k, p.ks) ? 1 : 0) | (dk_ok && fits(p.q, p.qs) ? 2 : 0) | (fits(p.v, p.vs) ? 4 : 0) |
                   (fits(p.d_o, p.dos) ? 8 : 0);
   constexpr int smem = PrepLayout<DKP, T, PS>::kBytes;
-  cudaError_t e = allow_smem(prep_kernel<DKP, T, PS>, smem);
+  cudaError_t e = allow_smem<prep_kernel<DKP, T, PS>>(smem);
   if (e != cudaSuccess) return e;
   const double tokens = (double)p.bound * kChunk;
   LaunchTimer t("delta_prep_kernel", s, tokens * (2.0 * p.hk * p.dk * sizeof(T) + p.hv * (4.0 * kChunk * PS + p.dv * sizeof(T))),

@@ -294,7 +294,7 @@ cudaError_t run_rscan(const Params& p, cudaStream_t s) {
   int* err = device_error_flag();
   if (err == nullptr) return cudaErrorInvalidValue;
   LaunchTimer t("delta_rscan_kernel", s, rows * 2.0 * p.dv * sizeof(T), rows * 6.0 * p.dk * p.dv);
-  cudaError_t e = allow_smem(rscan_kernel<DKP, T>, smem);
+  cudaError_t e = allow_smem<rscan_kernel<DKP, T>>(smem);
   if (e != cudaSuccess) return e;
   const unsigned grid = (unsigned)p.nseq * p.hv * ((p.dv + kLanes - 1) / kLanes);
   rscan_kernel<DKP, T><<<grid, kTcThreads, smem, s>>>(p, err);

@@ -287,7 +287,7 @@ cudaError_t run_scan(const Params& p, cudaStream_t s) {
   if (err == nullptr) return cudaErrorInvalidValue;
   LaunchTimer t(STORE ? "delta_scan_store_kernel" : "delta_scan_kernel", s, rows * 2.0 * p.dv * sizeof(T),
                 rows * 6.0 * p.dk * p.dv);
-  cudaError_t e = allow_smem(scan_kernel<DKP, T, PS, STORE>, smem);
+  cudaError_t e = allow_smem<scan_kernel<DKP, T, PS, STORE>>(smem);
   if (e != cudaSuccess) return e;
   scan_kernel<DKP, T, PS, STORE><<<grid, kTcThreads, smem, s>>>(p, err);
   return cudaGetLastError();

@@ -495,7 +495,7 @@ Plan plan(int64_t m, int64_t n, int64_t k, int pieces) {
 template <int BN, bool PAIR>
 cudaError_t run(const CUtensorMap& ma, const CUtensorMap& mb, const GemmArgs& g, cudaStream_t s) {
   constexpr int smem = Cfg<BN, PAIR>::kSmem;
-  cudaError_t e = cudaFuncSetAttribute(gemm_kernel<BN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_smem<gemm_kernel<BN, PAIR>>(smem);
   if (e != cudaSuccess) return e;
   const int64_t units = (int64_t)g.tiles_m * g.tiles_n * g.splits;
   const int sms = PAIR ? sm_count() / 2 : sm_count(), grid = (int)(units < sms ? units : sms);

@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace qrb {
 
 // Panel (block reflector) width of the blocked path.  Every panel is factored
@@ -65,6 +67,21 @@ int set_error(int status, const char* msg);
 
 // Streaming multiprocessors of the current device (cached per device).
 int sm_count();
+
+// Raises a kernel's dynamic shared memory limit, once per device (a bit of a per-kernel mask): the
+// runtime call costs microseconds, and the limit belongs to the device.
+template <auto Kernel>
+cudaError_t allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = (uint64_t)1 << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(reinterpret_cast<const void*>(Kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
 
 // Brackets one kernel launch with CUDA events on its stream while kernel timing is
 // enabled (qrb_kernel_timing); `bytes` / `flops` are the launch's algorithmic traffic

@@ -29,13 +29,13 @@ _LIB = ("QRBError", "lib")
 __all__ = [*_OPS, *_DELTA, *_LINEAR, *_LIB]
 
 
+_WHERE = {**dict.fromkeys(_OPS, ".ops"), **dict.fromkeys(_DELTA, ".delta"), **dict.fromkeys(_LINEAR, "._linear"),
+          **dict.fromkeys(_LIB, "._lib")}
+
+
 def __getattr__(name: str):
-    if name in _OPS:
-        return getattr(importlib.import_module(".ops", __name__), name)
-    if name in _DELTA:
-        return getattr(importlib.import_module(".delta", __name__), name)
-    if name in _LINEAR:
-        return getattr(importlib.import_module("._linear", __name__), name)
-    if name in _LIB:
-        return getattr(importlib.import_module("._lib", __name__), name)
-    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    if name not in _WHERE:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    value = getattr(importlib.import_module(_WHERE[name], __name__), name)
+    globals()[name] = value   # the next access finds it without coming here (3 us a call)
+    return value
