@@ -63,6 +63,7 @@ struct Params {
   int64_t time;
   const int32_t* offsets;          // packed layout: nseq + 1 token offsets
   int32_t* cstart;                 // packed layout: first chunk slot of each sequence
+  int32_t* order;                  // packed layout: the sequences, longest first
   float scale;
   const void *q, *k, *v, *d_o;
   const float *g, *beta;

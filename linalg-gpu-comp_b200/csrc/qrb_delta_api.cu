@@ -99,7 +99,7 @@ Layout layout(const qrb_delta_args& a, bool backward) {
     at += al(bytes);
     return o;
   };
-  l.cstart = take(a.seq_offsets != nullptr ? (a.nseq + 1) * 4 : 0);
+  l.cstart = take(a.seq_offsets != nullptr ? (2 * a.nseq + 1) * 4 : 0);
   l.kt = take(n * a.hk * tile_bytes(kChunk, pi, dkp));
   l.qt = take(n * a.hk * tile_bytes(kChunk, pi, dkp));
   l.xt = take(n * a.hv * tile_bytes(kChunk, ps, kChunk));
@@ -187,6 +187,7 @@ int run(const qrb_delta_args* a, void* ws, size_t wsb, void* stream, bool backwa
   p.time = a->time;
   p.offsets = a->seq_offsets;
   p.cstart = reinterpret_cast<int32_t*>(w + l.cstart);
+  p.order = p.cstart + a->nseq + 1;
   p.scale = a->scale;
   p.q = a->q;
   p.k = a->k;

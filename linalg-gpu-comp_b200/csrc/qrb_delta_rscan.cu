@@ -55,7 +55,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
   volatile int* abort = &bars.abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nb = (p.dv + kLanes - 1) / kLanes;
-  const int vb = blockIdx.x % nb, sh = blockIdx.x / nb, h = sh % p.hv, seq = sh / p.hv;
+  const int vb = blockIdx.x % nb, sh = blockIdx.x / nb, h = sh % p.hv, turn = sh / p.hv;
+  const int seq = p.offsets != nullptr ? p.order[turn] : turn;   // the longest sequences start first
   const int hk = h / p.group;
   const int quarters = min(4, (p.dv - vb * kLanes + 31) / 32);
   int64_t b, t0, n;
@@ -72,44 +73,71 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
     bars.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 0) tmem_alloc(&bars.tmem, 512);
+  if (warp == 16) tmem_alloc(&bars.tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
-  const int q = warp & 3, part = warp >> 2;
 
-  if (q < quarters) {
-    // ---- loads and MMAs: warp 0 waits, its first lane issues; step i handles chunk nc - 1 - i ----
-    int loaded = 0;
-    auto load = [&] {
-      const int i = loaded++;
-      if (lane != 0) return;
-      unsigned char* d = sm + (i % L::kStages) * L::kStage;
-      uint64_t* bar = &bars.full[i % L::kStages];
-      const int c = nc - 1 - i;
-      const size_t qk = ((size_t)(slot0 + c) * p.hk + hk) * L::kK, at = slot_head(p, slot0 + c, h);
-      mbar_arrive_expect_tx(bar, L::kStage + L::kGates);
-      bulk_load(d, p.kt + qk, L::kK, bar);
-      bulk_load(d + L::kOffQ, p.qt + qk, L::kK, bar);
-      bulk_load(d + L::kOffX, p.xt + at * L::kX, L::kX, bar);
-      bulk_load(d + L::kOffP, p.pt + at * L::kX, L::kX, bar);
-      bulk_load(d + L::kOffV, p.vt + (at * nb + vb) * L::kV, L::kV, bar);
-      bulk_load(d + L::kOffD, p.dot + (at * nb + vb) * L::kV, L::kV, bar);
-      bulk_load(sm + L::kOffG + (i % L::kStages) * L::kGates, p.gates + at * 3 * kChunk, L::kGates, bar);
-    };
-    auto tiles = [&](int i) { return smem_u32(sm + (i % L::kStages) * L::kStage); };
-    auto issue_ks = [&](int i) {   // K dS', once all pieces of the gradient are in place
-      if (!warp_wait(&bars.full[i % L::kStages], (i / L::kStages) & 1, abort, err, 72) ||
-          !warp_wait(&bars.sp, i & 1, abort, err, 73))
-        return;
-      tc_fence_after();
-      if (lane == 0) {
-        mma_pieces<64, DKP, false, PS, P, PS>(tmem + L::tK, tmem + L::tS, DKP / 2, tiles(i), 0);
+  if (warp == 16) {
+    // ---------------- loads and MMAs: one thread; step i handles chunk nc - 1 - i ----------------
+    if (lane == 0) {
+      int loaded = 0;
+      auto load = [&] {
+        const int i = loaded++;
+        unsigned char* d = sm + (i % L::kStages) * L::kStage;
+        uint64_t* bar = &bars.full[i % L::kStages];
+        const int c = nc - 1 - i;
+        const size_t qk = ((size_t)(slot0 + c) * p.hk + hk) * L::kK, at = slot_head(p, slot0 + c, h);
+        mbar_arrive_expect_tx(bar, L::kStage + L::kGates);
+        bulk_load(d, p.kt + qk, L::kK, bar);
+        bulk_load(d + L::kOffQ, p.qt + qk, L::kK, bar);
+        bulk_load(d + L::kOffX, p.xt + at * L::kX, L::kX, bar);
+        bulk_load(d + L::kOffP, p.pt + at * L::kX, L::kX, bar);
+        bulk_load(d + L::kOffV, p.vt + (at * nb + vb) * L::kV, L::kV, bar);
+        bulk_load(d + L::kOffD, p.dot + (at * nb + vb) * L::kV, L::kV, bar);
+        bulk_load(sm + L::kOffG + (i % L::kStages) * L::kGates, p.gates + at * 3 * kChunk, L::kGates, bar);
+      };
+      while (loaded < nc && loaded < L::kStages) load();
+      for (int i = 0; i < nc; ++i) {
+        const uint32_t ph = i & 1, sb = smem_u32(sm + (i % L::kStages) * L::kStage);
+        if (L::kStages == 1 && i > 0) {
+          if (!mbar_wait_abort(&bars.done, ph ^ 1, abort, err, 71)) break;
+          load();
+        }
+        if (!mbar_wait_abort(&bars.full[i % L::kStages], (i / L::kStages) & 1, abort, err, 72)) break;
+        if (!mbar_wait_abort(&bars.sp, ph, abort, err, 73)) break;
+        tc_fence_after();
+        mma_pieces<64, DKP, false, PS, P, PS>(tmem + L::tK, tmem + L::tS, DKP / 2, sb, 0);
         mma_commit(&bars.ks);
+        if (L::kStages == 2 && i > 0) {
+          if (!mbar_wait_abort(&bars.done, ph ^ 1, abort, err, 74)) break;
+          if (loaded < nc) load();
+        }
+        if (!mbar_wait_abort(&bars.dop, ph, abort, err, 75)) break;
+        tc_fence_after();
+        mma_pieces<64, 64, true, P, PS, PS>(tmem + L::tP, tmem + L::tF, 32, sb + L::kOffP, 0);
+        mma_commit(&bars.pd);
+        if (!mbar_wait_abort(&bars.f, ph, abort, err, 76)) break;
+        tc_fence_after();
+        mma_pieces<64, 64, true, PS, PS, PS>(tmem + L::tK, tmem + L::tF, 32, sb + L::kOffX, 0);
+        mma_commit(&bars.xf);
+        mma_pieces<DKP, 64, true, PS, P, PS>(tmem + L::tD, tmem + L::tO, 32, sb + L::kOffQ, 0);
+        if (!mbar_wait_abort(&bars.uw, ph, abort, err, 77)) break;
+        tc_fence_after();
+        mma_pieces<DKP, 64, true, PS, P, PS>(tmem + L::tD, tmem + L::tF, 32, sb, 1);
+        mma_commit(&bars.ds);
       }
-      __syncwarp();
-    };
+      if (*abort) {   // loads in flight must land, MMAs in flight end, before the block's memory goes
+        for (int s = 0; s < L::kStages; ++s)
+          if (loaded > s) mbar_wait(&bars.full[s], ((loaded - 1 - s) / L::kStages) & 1, 1u << 22);
+        mma_commit(&bars.drain);
+        mbar_wait(&bars.drain, 0, 1u << 22);
+      }
+    }
+  } else {
+    const int q = warp & 3, part = warp >> 2;
+    if (q < quarters) {
     const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
     const int lcol = 32 * q + lane, col = vb * kLanes + lcol;
     const int tile = vb * 4 + q;
@@ -126,23 +154,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
       for (int j = 0; j < HK; ++j) st[j] = 0.f;
     // pieces of dS' for the products, the first PG of them for the gradient kernel too
     auto put_state = [&](int c) {
-      uint32_t w[PS][HK / 2], g[PG][HK / 2];
-      put_pieces<PS, HK>(tl + L::tS + kb / 2, DKP / 2, st, w);
+      float y[HK];
+#pragma unroll
+      for (int i = 0; i < HK; ++i) y[i] = st[i];
+      put_pieces<PS, PG>(tl + L::tS + kb / 2, DKP / 2, y, p.dsp + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWS, lane,
+                         DKP, kb);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&bars.sp);
-#pragma unroll
-      for (int a = 0; a < PG; ++a)
-#pragma unroll
-        for (int i = 0; i < HK / 2; ++i) g[a][i] = w[a][i];
-      keep_pieces<PG>(p.dsp + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWS, lane, DKP, kb, g);
     };
-    if (nc > 0) {
-      if (warp == 0)
-        while (loaded < nc && loaded < L::kStages) load();
-      put_state(nc - 1);
-      if (warp == 0) issue_ks(0);
-    }
+    if (nc > 0) put_state(nc - 1);
     for (int i = 0; i < nc; ++i) {
       const uint32_t ph = i & 1;
       const int c = nc - 1 - i;
@@ -152,21 +173,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
       float x[kTok], u[kTok];
       if (!warp_wait(&bars.full[i % L::kStages], (i / L::kStages) & 1, abort, err, 81)) break;
       staged<T>(stage + L::kOffD, tb, lcol, x);
-      put_pieces<P, kTok>(tl + L::tF + tb / 2, 32, x);
-      with_tokens(gates.gam, [&](int j, float g) { x[j] *= p.scale * g; });
-      put_pieces<PS, kTok>(tl + L::tO + tb / 2, 32, x);
+      with_tokens(gates.gam, [&](int j, float g) { u[j] = x[j] * (p.scale * g); });
+      put_pieces<P, 0>(tl + L::tF + tb / 2, 32, x);
+      put_pieces<PS, 0>(tl + L::tO + tb / 2, 32, u);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&bars.dop);
-      if (warp == 0) {
-        if (!warp_wait(&bars.dop, ph, abort, err, 75)) break;
-        tc_fence_after();
-        if (lane == 0) {
-          mma_pieces<64, 64, true, P, PS, PS>(tmem + L::tP, tmem + L::tF, 32, tiles(i) + L::kOffP, 0);
-          mma_commit(&bars.pd);
-        }
-        __syncwarp();
-      }
       {
         // <S', dS'>: S' is the next chunk's first state, behind the last chunk the final state
         float y[HK], sds = 0.f;
@@ -189,20 +201,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
 #pragma unroll
       for (int j = 0; j < kTok; ++j) u[j] += x[j];
       with_tokens(gates.bet, [&](int j, float g) { x[j] = g * u[j]; });
-      put_pieces<PS, kTok>(tl + L::tF + tb / 2, 32, x);
+      put_pieces<PS, 0>(tl + L::tF + tb / 2, 32, x);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&bars.f);
-      if (warp == 0) {
-        if (!warp_wait(&bars.f, ph, abort, err, 76)) break;
-        tc_fence_after();
-        if (lane == 0) {
-          mma_pieces<64, 64, true, PS, PS, PS>(tmem + L::tK, tmem + L::tF, 32, tiles(i) + L::kOffX, 0);
-          mma_commit(&bars.xf);
-          mma_pieces<DKP, 64, true, PS, P, PS>(tmem + L::tD, tmem + L::tO, 32, tiles(i) + L::kOffQ, 0);
-        }
-        __syncwarp();
-      }
       if (!warp_wait(&bars.xf, ph, abort, err, 84)) break;
       tc_fence_after();
       ld_cols(tl + L::tK + tb, x);
@@ -211,24 +213,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
       float y[kTok];   // dV
       with_tokens(gates.bet, [&](int j, float g) { y[j] = g * u[j]; });
       with_tokens(gates.gam, [&](int j, float g) { x[j] = -g * y[j]; });
-      put_pieces<PS, kTok>(tl + L::tF + tb / 2, 32, x);
+      put_pieces<PS, 0>(tl + L::tF + tb / 2, 32, x);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&bars.uw);
-      if (warp == 0) {
-        if (!warp_wait(&bars.uw, ph, abort, err, 77)) break;
-        tc_fence_after();
-        if (lane == 0) {
-          mma_pieces<DKP, 64, true, PS, P, PS>(tmem + L::tD, tmem + L::tF, 32, tiles(i), 1);
-          mma_commit(&bars.ds);
-        }
-        __syncwarp();
-      }
       const float glast = *gates.last;
       {
-        uint32_t g[PG][kTok / 2];
-        split_all<PG, kTok>(u, g);
-        keep_pieces<PG>(p.dup + at * kWF, lane, kChunk, tb, g);
+#pragma unroll
+        for (int j = 0; j < kTok; ++j) x[j] = u[j];
+        put_pieces<PG, PG>(kNoTmem, 0, x, p.dup + at * kWF, lane, kChunk, tb);
         fetch_pieces<PS, kTok>(p.ep + at * kWF, lane, kChunk, tb, x);
 #pragma unroll
         for (int j = 0; j < kTok; ++j) x[j] *= u[j];
@@ -262,26 +255,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
         if (!warp_wait(&bars.share[q], ph, abort, err, 86)) break;
         tc_fence_after();
         put_state(c - 1);
-        if (warp == 0) {
-          if (!warp_wait(&bars.done, ph, abort, err, 74)) break;
-          if (loaded < nc) load();
-          issue_ks(i + 1);
-        }
       }
-    }
-    if (*abort && warp == 0 && lane == 0) {
-      // loads in flight must land, MMAs in flight end, before the block's memory goes
-      for (int s = 0; s < L::kStages; ++s)
-        if (loaded > s) mbar_wait(&bars.full[s], ((loaded - 1 - s) / L::kStages) & 1, 1u << 22);
-      mma_commit(&bars.drain);
-      mbar_wait(&bars.drain, 0, 1u << 22);
     }
     if (p.ds_init != nullptr && on && !*abort)
       store_column(p.ds_init + sbase + (size_t)kb * p.dv + col, p.dv, p.dk - kb, st);
+    }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }

@@ -9,8 +9,9 @@
 // a chain of three products with register work between them.  Q S0 and P u, which o is made of, run
 // in the shadow of that work (the first is scaled in place and the second added to it), and o is stored
 // in the shadow of the next chunk's K S0.  Sixteen warps, because the register work between two
-// products is bound by latency; the first thread also loads the chunk tiles by bulk copies (two chunks
-// in flight where they fit) and issues the MMAs.
+// products is bound by latency.  A thread beside them loads the chunk tiles by bulk copies (two chunks
+// in flight where they fit) and issues the MMAs: it is held up while the tensor cores' queue is full,
+// which in a computing warp made every other one wait for it.
 #include "qrb_delta_tc.cuh"
 
 namespace qrb {
@@ -60,7 +61,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
   volatile int* abort = &bars.abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nb = (p.dv + kLanes - 1) / kLanes;
-  const int vb = blockIdx.x % nb, sh = blockIdx.x / nb, h = sh % p.hv, seq = sh / p.hv;
+  const int vb = blockIdx.x % nb, sh = blockIdx.x / nb, h = sh % p.hv, turn = sh / p.hv;
+  const int seq = p.offsets != nullptr ? p.order[turn] : turn;   // the longest sequences start first
   const int hk = h / p.group;
   const int quarters = min(4, (p.dv - vb * kLanes + 31) / 32);   // 32-column groups that hold columns
   int64_t b, t0, n;
@@ -77,50 +79,70 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
     bars.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 0) tmem_alloc(&bars.tmem, 512);
+  if (warp == 16) tmem_alloc(&bars.tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
-  const int q = warp & 3, part = warp >> 2;
 
-  if (q < quarters) {   // warps without columns have nothing to add
-    // ---- loads and MMAs: warp 0 waits, its first lane issues ----
-    int loaded = 0;
-    auto load = [&] {
-      const int c = loaded++;
-      if (lane != 0) return;
-      unsigned char* d = sm + (c % L::kStages) * L::kStage;
-      uint64_t* bar = &bars.full[c % L::kStages];
-      const size_t qk = ((size_t)(slot0 + c) * p.hk + hk) * L::kK, at = slot_head(p, slot0 + c, h);
-      mbar_arrive_expect_tx(bar, L::kStage + L::kGates);
-      bulk_load(d, p.kt + qk, L::kK, bar);
-      bulk_load(d + L::kOffQ, p.qt + qk, L::kK, bar);
-      bulk_load(d + L::kOffX, p.xt + at * L::kX, L::kX, bar);
-      bulk_load(d + L::kOffP, p.pt + at * L::kX, L::kX, bar);
-      bulk_load(d + L::kOffV, p.vt + (at * nb + vb) * L::kV, L::kV, bar);
-      if (STORE) bulk_load(d + L::kOffD, p.dot + (at * nb + vb) * L::kV, L::kV, bar);
-      bulk_load(sm + L::kOffG + (c % L::kStages) * L::kGates, p.gates + at * 3 * kChunk, L::kGates, bar);
-    };
-    auto tiles = [&](int c) { return smem_u32(sm + (c % L::kStages) * L::kStage); };
-    auto issue_ks = [&](int c) {   // K S0, once all pieces of the state are in place
-      if (!warp_wait(&bars.full[c % L::kStages], (c / L::kStages) & 1, abort, err, 52) ||
-          !warp_wait(&bars.sp, c & 1, abort, err, 53))
-        return;
-      tc_fence_after();
-      if (lane == 0) {
-        mma_pieces<64, DKP, false, PS, P, PS>(tmem + L::tK, tmem + L::tS, DKP / 2, tiles(c), 0);
+  if (warp == 16) {
+    // ---------------- loads and MMAs: one thread ----------------
+    if (lane == 0) {
+      int loaded = 0;
+      auto load = [&] {
+        const int c = loaded++;
+        unsigned char* d = sm + (c % L::kStages) * L::kStage;
+        uint64_t* bar = &bars.full[c % L::kStages];
+        const size_t qk = ((size_t)(slot0 + c) * p.hk + hk) * L::kK, at = slot_head(p, slot0 + c, h);
+        mbar_arrive_expect_tx(bar, L::kStage + L::kGates);
+        bulk_load(d, p.kt + qk, L::kK, bar);
+        bulk_load(d + L::kOffQ, p.qt + qk, L::kK, bar);
+        bulk_load(d + L::kOffX, p.xt + at * L::kX, L::kX, bar);
+        bulk_load(d + L::kOffP, p.pt + at * L::kX, L::kX, bar);
+        bulk_load(d + L::kOffV, p.vt + (at * nb + vb) * L::kV, L::kV, bar);
+        if (STORE) bulk_load(d + L::kOffD, p.dot + (at * nb + vb) * L::kV, L::kV, bar);
+        bulk_load(sm + L::kOffG + (c % L::kStages) * L::kGates, p.gates + at * 3 * kChunk, L::kGates, bar);
+      };
+      while (loaded < nc && loaded < L::kStages) load();
+      for (int c = 0; c < nc; ++c) {
+        const uint32_t ph = c & 1, sb = smem_u32(sm + (c % L::kStages) * L::kStage);
+        if (L::kStages == 1 && c > 0) {   // the one stage is free once all are through with the last chunk
+          if (!mbar_wait_abort(&bars.o, ph ^ 1, abort, err, 51)) break;
+          load();
+        }
+        if (!mbar_wait_abort(&bars.full[c % L::kStages], (c / L::kStages) & 1, abort, err, 52)) break;
+        if (!mbar_wait_abort(&bars.sp, ph, abort, err, 53)) break;
+        tc_fence_after();
+        mma_pieces<64, DKP, false, PS, P, PS>(tmem + L::tK, tmem + L::tS, DKP / 2, sb, 0);
         mma_commit(&bars.ks);
-      }
-      __syncwarp();
-    };
-    auto issue_qs = [&](int c) {
-      if (lane == 0) {
-        mma_pieces<64, DKP, false, PS, P, PS>(tmem + L::tQ, tmem + L::tS, DKP / 2, tiles(c) + L::kOffQ, 0);
+        if (L::kStages == 2 && c > 0) {   // o of the last chunk is read: Q S0 may land, its stage may go
+          if (!mbar_wait_abort(&bars.o, ph ^ 1, abort, err, 54)) break;
+          if (loaded < nc) load();
+          tc_fence_after();
+        }
+        mma_pieces<64, DKP, false, PS, P, PS>(tmem + L::tQ, tmem + L::tS, DKP / 2, sb + L::kOffQ, 0);
         mma_commit(&bars.qs);
+        if (!mbar_wait_abort(&bars.f, ph, abort, err, 55)) break;
+        tc_fence_after();
+        mma_pieces<64, 64, false, PS, PS, PS>(tmem + L::tK, tmem + L::tF, 32, sb + L::kOffX, 0);
+        mma_commit(&bars.xf);
+        if (!mbar_wait_abort(&bars.uw, ph, abort, err, 56)) break;
+        tc_fence_after();
+        mma_pieces<DKP, 64, true, PS, P, PS>(tmem + L::tD, tmem + L::tF, 32, sb, 0);
+        mma_commit(&bars.ds);
+        mma_pieces<64, 64, false, PS, PS, PS>(tmem + L::tQ, tmem + L::tU, 32, sb + L::kOffP, 1);
+        mma_commit(&bars.pu);
       }
-      __syncwarp();
-    };
+      if (*abort) {   // loads in flight must land, MMAs in flight end, before the block's memory goes
+        for (int s = 0; s < L::kStages; ++s)
+          if (loaded > s) mbar_wait(&bars.full[s], ((loaded - 1 - s) / L::kStages) & 1, 1u << 22);
+        mma_commit(&bars.drain);
+        mbar_wait(&bars.drain, 0, 1u << 22);
+      }
+    }
+  } else {
+    const int q = warp & 3, part = warp >> 2;
+    if (q < quarters) {   // warps without columns have nothing to add
     const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
     const int lcol = 32 * q + lane, col = vb * kLanes + lcol;  // value column in the block, in the head
     const int tile = vb * 4 + q;                              // its 32-column tile
@@ -135,22 +157,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
 #pragma unroll
       for (int j = 0; j < HK; ++j) st[j] = 0.f;
     auto put_state = [&](int c) {
-      uint32_t w[PS][HK / 2];
-      put_pieces<PS, HK>(tl + L::tS + kb / 2, DKP / 2, st, w);
+      float y[HK];
+#pragma unroll
+      for (int i = 0; i < HK; ++i) y[i] = st[i];
+      put_pieces<PS, STORE ? PS : 0>(tl + L::tS + kb / 2, DKP / 2, y,
+                                     p.s0p + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWS, lane, DKP, kb);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&bars.sp);
-      if (STORE) keep_pieces<PS>(p.s0p + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWS, lane, DKP, kb, w);
     };
-    if (nc > 0) {
-      if (warp == 0)
-        while (loaded < nc && loaded < L::kStages) load();
-      put_state(0);
-      if (warp == 0) {
-        issue_ks(0);
-        issue_qs(0);
-      }
-    }
+    if (nc > 0) put_state(0);
     for (int c = 0; c < nc; ++c) {
       const uint32_t ph = c & 1;
       const unsigned char* stage = sm + (c % L::kStages) * L::kStage;
@@ -163,19 +179,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
       ld_cols(tl + L::tK + tb, x);
       with_tokens(gates.gam, [&](int i, float g) { e[i] -= g * x[i]; });
       with_tokens(gates.bet, [&](int i, float g) { x[i] = g * e[i]; });
-      put_pieces<PS, kTok>(tl + L::tF + tb / 2, 32, x);
+      put_pieces<PS, 0>(tl + L::tF + tb / 2, 32, x);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&bars.f);
-      if (warp == 0) {
-        if (!warp_wait(&bars.f, ph, abort, err, 55)) break;
-        tc_fence_after();
-        if (lane == 0) {
-          mma_pieces<64, 64, false, PS, PS, PS>(tmem + L::tK, tmem + L::tF, 32, tiles(c) + L::kOffX, 0);
-          mma_commit(&bars.xf);
-        }
-        __syncwarp();
-      }
       if (!warp_wait(&bars.qs, ph, abort, err, 63)) break;
       tc_fence_after();
       ld_cols(tl + L::tQ + tb, x);   // scale gamma Q S0 goes back, P u is added to it there
@@ -191,30 +198,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
       for (int i = 0; i < kTok; ++i) x[i] += e[i];   // x: e
       with_tokens(gates.bet, [&](int i, float g) { e[i] = g * x[i]; });   // e: u
       {
-        uint32_t w[PS][kTok / 2];
-        put_pieces<PS, kTok>(tl + L::tU + tb / 2, 32, e, w);
-        with_tokens(gates.tail, [&](int i, float g) { e[i] *= g; });
-        put_pieces<PS, kTok>(tl + L::tF + tb / 2, 32, e, w);
+        float y[kTok];
+        with_tokens(gates.tail, [&](int i, float g) { y[i] = g * e[i]; });
+        put_pieces<PS, 0>(tl + L::tU + tb / 2, 32, e);
+        put_pieces<PS, 0>(tl + L::tF + tb / 2, 32, y);
       }
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&bars.uw);
-      if (warp == 0) {
-        if (!warp_wait(&bars.uw, ph, abort, err, 56)) break;
-        tc_fence_after();
-        if (lane == 0) {
-          mma_pieces<DKP, 64, true, PS, P, PS>(tmem + L::tD, tmem + L::tF, 32, tiles(c), 0);
-          mma_commit(&bars.ds);
-          mma_pieces<64, 64, false, PS, PS, PS>(tmem + L::tQ, tmem + L::tU, 32, tiles(c) + L::kOffP, 1);
-          mma_commit(&bars.pu);
-        }
-        __syncwarp();
-      }
-      if (STORE) {
-        uint32_t w[PS][kTok / 2];
-        split_all<PS, kTok>(x, w);
-        keep_pieces<PS>(p.ep + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWF, lane, kChunk, tb, w);
-      }
+      if (STORE)
+        put_pieces<PS, PS>(kNoTmem, 0, x, p.ep + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWF, lane, kChunk, tb);
       const float glast = *gates.last;
       if (!warp_wait(&bars.ds, ph, abort, err, 65)) break;
       tc_fence_after();
@@ -232,8 +225,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
           tc_fence_after();
         }
         put_state(c + 1);
-        // with one stage the tiles of the next chunk can only be fetched once P u is through with these
-        if (warp == 0 && L::kStages == 2) issue_ks(c + 1);
       }
       if (!warp_wait(&bars.pu, ph, abort, err, 67)) break;
       tc_fence_after();
@@ -242,13 +233,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
       tc_fence_before();
       fence_proxy_async();   // what this stage held is read before bulk copies may replace it
       warp_arrive(&bars.o);
-      if (warp == 0 && c + 1 < nc) {   // all warps are through with this chunk: its tiles may go
-        if (!warp_wait(&bars.o, ph, abort, err, 54)) break;
-        if (loaded < nc) load();
-        if (L::kStages == 1) issue_ks(c + 1);
-        tc_fence_after();
-        issue_qs(c + 1);
-      }
       if (STORE) {
 #pragma unroll
         for (int i = 0; i < kTok; ++i) x[i] *= e[i];
@@ -260,19 +244,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
                      (int)min(n - tok, (int64_t)kTok), x);
       }
     }
-    if (*abort && warp == 0 && lane == 0) {
-      // loads in flight must land, MMAs in flight end, before the block's memory goes
-      for (int s = 0; s < L::kStages; ++s)
-        if (loaded > s) mbar_wait(&bars.full[s], ((loaded - 1 - s) / L::kStages) & 1, 1u << 22);
-      mma_commit(&bars.drain);
-      mbar_wait(&bars.drain, 0, 1u << 22);
-    }
     if (p.s_end != nullptr && on && !*abort)
       store_column(p.s_end + sbase + (size_t)kb * p.dv + col, p.dv, p.dk - kb, st);
+    }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }

@@ -20,7 +20,7 @@ using namespace sm100;
 constexpr int kLanes = 128;                 // value columns per block of the recurrences
 constexpr int kParts = 4;                   // threads that share a value column
 constexpr int kTok = kChunk / kParts;       // tokens of a thread
-constexpr int kTcThreads = kLanes * kParts;
+constexpr int kTcThreads = kLanes * kParts + 32;   // sixteen warps compute, one issues loads and MMAs
 constexpr int kSmemLimit = 232448;
 
 // kind::f16, bf16 operands, fp32 accumulation, M = 128, A in tensor memory.
@@ -106,54 +106,33 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// The pieces of two values, packed as an A operand wants them (the first in the low half).
-template <int PS>
-__device__ __forceinline__ void split2(float a, float b, uint32_t (&p)[PS]) {
+constexpr uint32_t kNoTmem = 0xffffffffu;
+
+// N values of this lane as PS pieces of N / 2 columns each, piece_cols apart.  KEEP > 0: the first KEEP
+// pieces also go to a tile of the gradient kernel (32 value columns as rows, pieces of `cols` columns,
+// written in units of 8).  One piece at a time: x becomes what is left.
+template <int PS, int KEEP, int N>
+__device__ __forceinline__ void put_pieces(uint32_t taddr, uint32_t piece_cols, float (&x)[N], unsigned char* tile = nullptr,
+                                           int row = 0, int cols = 0, int col = 0) {
 #pragma unroll
   for (int i = 0; i < PS; ++i) {
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p[i]) : "f"(b), "f"(a));
-    if (i + 1 < PS) {
-      a -= __uint_as_float(p[i] << 16);
-      b -= __uint_as_float(p[i] & 0xffff0000u);
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(x[2 * j + 1]), "f"(x[2 * j]));
+      if (i + 1 < PS) {
+        x[2 * j] -= __uint_as_float(w[j] << 16);
+        x[2 * j + 1] -= __uint_as_float(w[j] & 0xffff0000u);
+      }
+    }
+    if (taddr != kNoTmem) st_cols(taddr + i * piece_cols, w);
+    if (i < KEEP) {
+#pragma unroll
+      for (int j = 0; j < N / 2; j += 4)
+        *reinterpret_cast<uint4*>(tile + unit_off(kTile, row, i * cols + col + 2 * j)) =
+            make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
     }
   }
-}
-
-template <int PS, int N>
-__device__ __forceinline__ void split_all(const float (&x)[N], uint32_t (&w)[PS][N / 2]) {
-#pragma unroll
-  for (int j = 0; j < N / 2; ++j) {
-    uint32_t p[PS];
-    split2<PS>(x[2 * j], x[2 * j + 1], p);
-#pragma unroll
-    for (int i = 0; i < PS; ++i) w[i][j] = p[i];
-  }
-}
-
-// N values of this lane as PS pieces of N / 2 columns each, piece_cols apart; w keeps them.
-template <int PS, int N>
-__device__ __forceinline__ void put_pieces(uint32_t taddr, uint32_t piece_cols, const float (&x)[N],
-                                           uint32_t (&w)[PS][N / 2]) {
-  split_all<PS, N>(x, w);
-#pragma unroll
-  for (int i = 0; i < PS; ++i) st_cols(taddr + i * piece_cols, w[i]);
-}
-template <int PS, int N>
-__device__ __forceinline__ void put_pieces(uint32_t taddr, uint32_t piece_cols, const float (&x)[N]) {
-  uint32_t w[PS][N / 2];
-  put_pieces<PS, N>(taddr, piece_cols, x, w);
-}
-
-// Tiles the recurrences leave for the gradient kernel: 32 value columns as rows, pieces of `cols`
-// columns, written in units of 8 columns.
-template <int PS, int W>
-__device__ __forceinline__ void keep_pieces(unsigned char* tile, int row, int cols, int col, const uint32_t (&w)[PS][W]) {
-#pragma unroll
-  for (int i = 0; i < PS; ++i)
-#pragma unroll
-    for (int j = 0; j < W; j += 4)
-      *reinterpret_cast<uint4*>(tile + unit_off(kTile, row, i * cols + col + 2 * j)) =
-          make_uint4(w[i][j], w[i][j + 1], w[i][j + 2], w[i][j + 3]);
 }
 
 template <int PS, int N>
