@@ -29,7 +29,7 @@
 // (the fp32 final state is then within about 3e-6), three for fp32.  The backward recurrences take
 // three for every type, because dg is the small difference of the sums above: with two it was
 // 2e-5 off, four to eight times the error of its terms.  dq and dk, rounded to their type in the
-// end, take two pieces of the 16-bit types.
+// end, take two pieces of the 16-bit types, and so does e in dbeta.
 //
 // Operand tiles are bf16 in blocks of 64 columns (128 bytes a row), the 16-byte units of a row
 // XORed with row % 8, both in shared memory (where ldmatrix then reads without bank conflicts)
@@ -98,6 +98,15 @@ struct Pieces<float> {
   static constexpr int kIn = 3, kS = 3;
 };
 constexpr int kBackPieces = 3;   // of the backward recurrences
+// Pieces of S0, P and u in o (one bf16 piece was tried for bf16 calls: its two products cancel in part, and
+// o was 3.6e-3 off in place of 1.7e-3).
+template <typename T>
+struct OutPieces {
+  static constexpr int k = Pieces<T>::kS;
+};
+// Backward: every kAnchor-th chunk from a sequence's end takes <S', dS'> from the states themselves, the
+// others from the next chunk's by the same identity as dg within a chunk (see qrb_delta_rscan.cu).
+constexpr int kAnchor = 8;
 
 
 __device__ __forceinline__ float to_f(float x) { return x; }

@@ -75,10 +75,11 @@ constexpr int kPrepThreads = 256;
 constexpr int kMStride = 68;   // floats per row of M and X: rows stay 16-byte aligned, columns on distinct banks
 constexpr int kRStride = 36;
 
-template <int DKP, typename T, int PS>
+template <int DKP, typename T, int PS, int PO>
 struct PrepLayout {
   static constexpr int P = Pieces<T>::kIn;
-  static constexpr int kQK = tile_bytes(kChunk, P, DKP), kXP = tile_bytes(kChunk, PS, kChunk);
+  static constexpr int kQK = tile_bytes(kChunk, P, DKP), kXP = tile_bytes(kChunk, PS, kChunk), kPP = tile_bytes(kChunk, PO, kChunk);
+  static_assert(PO <= PS, "overlay");
   // once the products are taken, over k and q: X's two 32 x 32 diagonal blocks (fp32), the right sides
   // of a merge, and the pieces of P, later those of X.  52 KB with 16-bit operands: four blocks an SM.
   static constexpr int kOffS = 0, kOffR = 2 * 32 * kRStride * 4, kOffT = 16384;
@@ -184,9 +185,9 @@ __device__ __forceinline__ void block_product(float (&r)[2][4], const float* m0,
   }
 }
 
-template <int DKP, typename T, int PS>
+template <int DKP, typename T, int PS, int PO>
 __global__ void __launch_bounds__(kPrepThreads, PS == 3 ? 2 : 4) prep_kernel(Params p, int vec) {
-  using L = PrepLayout<DKP, T, PS>;
+  using L = PrepLayout<DKP, T, PS, PO>;
   constexpr int P = L::P;
   extern __shared__ __align__(128) unsigned char sm[];
   unsigned char *kt = sm, *qt = sm + L::kQK, *xp = sm + L::kOffT;
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(kPrepThreads, PS == 3 ? 2 : 4) prep_kernel(Par
           *reinterpret_cast<float2*>(M + i * kMStride + cl) =
               make_float2(cl < i ? acc[j][2 * r] * d0 : 0.f, cl + 1 < i ? acc[j][2 * r + 1] * d1 : 0.f);
         } else {
-          put2<PS>(xp, kChunk, kChunk, i, cl, cl <= i ? p.scale * acc[j][2 * r] * d0 : 0.f,
+          put2<PO>(xp, kChunk, kChunk, i, cl, cl <= i ? p.scale * acc[j][2 * r] * d0 : 0.f,
                    cl + 1 <= i ? p.scale * acc[j][2 * r + 1] * d1 : 0.f);
         }
       }
@@ -327,8 +328,8 @@ __global__ void __launch_bounds__(kPrepThreads, PS == 3 ? 2 : 4) prep_kernel(Par
       to[i * kRStride + j] = x;
     }
   } else {
-    for (int i = (tid - kChunk) * 16; i < L::kXP; i += (kPrepThreads - kChunk) * 16)
-      *reinterpret_cast<uint4*>(p.pt + sh * L::kXP + i) = *reinterpret_cast<const uint4*>(xp + i);
+    for (int i = (tid - kChunk) * 16; i < L::kPP; i += (kPrepThreads - kChunk) * 16)
+      *reinterpret_cast<uint4*>(p.pt + sh * L::kPP + i) = *reinterpret_cast<const uint4*>(xp + i);
   }
   __syncthreads();
   // v and dO as kChunk x 128 tiles, one per 128 value columns: what the recurrences then read needs no
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(kPrepThreads, PS == 3 ? 2 : 4) prep_kernel(Par
     *reinterpret_cast<uint4*>(p.xt + sh * L::kXP + i) = *reinterpret_cast<const uint4*>(xp + i);
 }
 
-template <int DKP, typename T, int PS>
+template <int DKP, typename T, int PS, int PO>
 cudaError_t run_prep(const Params& p, cudaStream_t s) {
   const auto fits = [&](const void* x, const Strides& st) {
     const int64_t v = 16 / (int64_t)sizeof(T);
@@ -434,13 +435,13 @@ cudaError_t run_prep(const Params& p, cudaStream_t s) {
   const bool dk_ok = p.dk % (16 / (int)sizeof(T)) == 0;
   const int vec = (dk_ok && fits(p.k, p.ks) ? 1 : 0) | (dk_ok && fits(p.q, p.qs) ? 2 : 0) | (fits(p.v, p.vs) ? 4 : 0) |
                   (fits(p.d_o, p.dos) ? 8 : 0);
-  constexpr int smem = PrepLayout<DKP, T, PS>::kBytes;
-  cudaError_t e = allow_smem<prep_kernel<DKP, T, PS>>(smem);
+  constexpr int smem = PrepLayout<DKP, T, PS, PO>::kBytes;
+  cudaError_t e = allow_smem<prep_kernel<DKP, T, PS, PO>>(smem);
   if (e != cudaSuccess) return e;
   const double tokens = (double)p.bound * kChunk;
-  LaunchTimer t("delta_prep_kernel", s, tokens * (2.0 * p.hk * p.dk * sizeof(T) + p.hv * (4.0 * kChunk * PS + p.dv * sizeof(T))),
+  LaunchTimer t("delta_prep_kernel", s, tokens * (2.0 * p.hk * p.dk * sizeof(T) + p.hv * (2.0 * kChunk * (PS + PO) + p.dv * sizeof(T))),
                 tokens * p.hv * 4.0 * kChunk * p.dk);
-  prep_kernel<DKP, T, PS><<<dim3((unsigned)p.bound, (unsigned)p.hv), kPrepThreads, smem, s>>>(p, vec);
+  prep_kernel<DKP, T, PS, PO><<<dim3((unsigned)p.bound, (unsigned)p.hv), kPrepThreads, smem, s>>>(p, vec);
   return cudaGetLastError();
 }
 
@@ -452,16 +453,18 @@ cudaError_t launch_plan(const Params& p, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-template <typename T, int PS>
+template <typename T, int PS, int PO>
 static cudaError_t pick_prep(const Params& p, cudaStream_t s) {
-  return p.dk <= 64 ? run_prep<64, T, PS>(p, s) : run_prep<128, T, PS>(p, s);
+  return p.dk <= 64 ? run_prep<64, T, PS, PO>(p, s) : run_prep<128, T, PS, PO>(p, s);
 }
 
 cudaError_t launch_prep(const Params& p, int dtype, cudaStream_t s) {
   constexpr int B = kBackPieces;
-  if (dtype == 1) return p.backward ? pick_prep<__nv_bfloat16, B>(p, s) : pick_prep<__nv_bfloat16, 2>(p, s);
-  if (dtype == 2) return p.backward ? pick_prep<__half, B>(p, s) : pick_prep<__half, 2>(p, s);
-  return pick_prep<float, 3>(p, s);
+  if (dtype == 1)
+    return p.backward ? pick_prep<__nv_bfloat16, B, B>(p, s)
+                      : pick_prep<__nv_bfloat16, 2, OutPieces<__nv_bfloat16>::k>(p, s);
+  if (dtype == 2) return p.backward ? pick_prep<__half, B, B>(p, s) : pick_prep<__half, 2, OutPieces<__half>::k>(p, s);
+  return pick_prep<float, 3, 3>(p, s);
 }
 
 }  // namespace delta

@@ -73,47 +73,45 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
     bars.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 16) tmem_alloc(&bars.tmem, 512);
+  if (warp == kIssuer) tmem_alloc(&bars.tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
 
-  if (warp == 16) {
-    // ---------------- loads and MMAs: one thread; step i handles chunk nc - 1 - i ----------------
+  if (warp == kLoader) {
+    // ---------------- loads: one thread; step i handles chunk nc - 1 - i ----------------
     if (lane == 0) {
-      int loaded = 0;
-      auto load = [&] {
-        const int i = loaded++;
-        unsigned char* d = sm + (i % L::kStages) * L::kStage;
-        uint64_t* bar = &bars.full[i % L::kStages];
-        const int c = nc - 1 - i;
+      int i = 0;
+      for (; i < nc; ++i) {
+        const int stage = i % L::kStages, c = nc - 1 - i;
+        if (i >= L::kStages && !mbar_wait_abort(&bars.done, (i - L::kStages) & 1, abort, err, 71)) break;
+        unsigned char* d = sm + stage * L::kStage;
+        uint64_t* bar = &bars.full[stage];
         const size_t qk = ((size_t)(slot0 + c) * p.hk + hk) * L::kK, at = slot_head(p, slot0 + c, h);
         mbar_arrive_expect_tx(bar, L::kStage + L::kGates);
         bulk_load(d, p.kt + qk, L::kK, bar);
-        bulk_load(d + L::kOffQ, p.qt + qk, L::kK, bar);
-        bulk_load(d + L::kOffX, p.xt + at * L::kX, L::kX, bar);
-        bulk_load(d + L::kOffP, p.pt + at * L::kX, L::kX, bar);
-        bulk_load(d + L::kOffV, p.vt + (at * nb + vb) * L::kV, L::kV, bar);
+        bulk_load(sm + L::kOffG + stage * L::kGates, p.gates + at * 3 * kChunk, L::kGates, bar);
         bulk_load(d + L::kOffD, p.dot + (at * nb + vb) * L::kV, L::kV, bar);
-        bulk_load(sm + L::kOffG + (i % L::kStages) * L::kGates, p.gates + at * 3 * kChunk, L::kGates, bar);
-      };
-      while (loaded < nc && loaded < L::kStages) load();
+        bulk_load(d + L::kOffP, p.pt + at * L::kX, L::kX, bar);
+        bulk_load(d + L::kOffX, p.xt + at * L::kX, L::kX, bar);
+        bulk_load(d + L::kOffQ, p.qt + qk, L::kK, bar);
+        bulk_load(d + L::kOffV, p.vt + (at * nb + vb) * L::kV, L::kV, bar);
+      }
+      if (*abort)   // loads in flight must land before the block's memory goes
+        for (int s = 0; s < L::kStages; ++s)
+          if (i > s) mbar_wait(&bars.full[s], ((i - 1 - s) / L::kStages) & 1, 1u << 22);
+    }
+  } else if (warp == kIssuer) {
+    // ---------------- MMAs: one thread ----------------
+    if (lane == 0) {
       for (int i = 0; i < nc; ++i) {
         const uint32_t ph = i & 1, sb = smem_u32(sm + (i % L::kStages) * L::kStage);
-        if (L::kStages == 1 && i > 0) {
-          if (!mbar_wait_abort(&bars.done, ph ^ 1, abort, err, 71)) break;
-          load();
-        }
         if (!mbar_wait_abort(&bars.full[i % L::kStages], (i / L::kStages) & 1, abort, err, 72)) break;
         if (!mbar_wait_abort(&bars.sp, ph, abort, err, 73)) break;
         tc_fence_after();
         mma_pieces<64, DKP, false, PS, P, PS>(tmem + L::tK, tmem + L::tS, DKP / 2, sb, 0);
         mma_commit(&bars.ks);
-        if (L::kStages == 2 && i > 0) {
-          if (!mbar_wait_abort(&bars.done, ph ^ 1, abort, err, 74)) break;
-          if (loaded < nc) load();
-        }
         if (!mbar_wait_abort(&bars.dop, ph, abort, err, 75)) break;
         tc_fence_after();
         mma_pieces<64, 64, true, P, PS, PS>(tmem + L::tP, tmem + L::tF, 32, sb + L::kOffP, 0);
@@ -128,9 +126,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
         mma_pieces<DKP, 64, true, PS, P, PS>(tmem + L::tD, tmem + L::tF, 32, sb, 1);
         mma_commit(&bars.ds);
       }
-      if (*abort) {   // loads in flight must land, MMAs in flight end, before the block's memory goes
-        for (int s = 0; s < L::kStages; ++s)
-          if (loaded > s) mbar_wait(&bars.full[s], ((loaded - 1 - s) / L::kStages) & 1, 1u << 22);
+      if (*abort) {   // MMAs in flight must end before tensor memory goes
         mma_commit(&bars.drain);
         mbar_wait(&bars.drain, 0, 1u << 22);
       }
@@ -163,6 +159,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
       tc_fence_before();
       warp_arrive(&bars.sp);
     };
+    float sds = 0.f;
     if (nc > 0) put_state(nc - 1);
     for (int i = 0; i < nc; ++i) {
       const uint32_t ph = i & 1;
@@ -180,15 +177,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
       tc_fence_before();
       warp_arrive(&bars.dop);
       {
-        // <S', dS'>: S' is the next chunk's first state, behind the last chunk the final state
-        float y[HK], sds = 0.f;
-        if (c + 1 < nc)
-          fetch_pieces<PS, HK>(p.s0p + (slot_head(p, slot0 + c + 1, h) * p.nv + tile) * kWS, lane, DKP, kb, y);
-        else
-          load_column(p.s_last + scol, p.dv, p.dk - kb, on, y);
+        // This warp's share of <S', dS'>: behind the last chunk from the final state, at every kAnchor-th
+        // chunk before it from the next chunk's first state, and between from the next chunk's share, as
+        // <S0, dS0> = <S', dS'> + sum (o.do - v.dV) over a chunk's tokens.
+        if (i % kAnchor == 0) {
+          float y[HK];
+          if (i > 0)
+            fetch_pieces<PS, HK>(p.s0p + (slot_head(p, slot0 + c + 1, h) * p.nv + tile) * kWS, lane, DKP, kb, y);
+          else
+            load_column(p.s_last + scol, p.dv, p.dk - kb, on, y);
+          sds = 0.f;
 #pragma unroll
-        for (int a = 0; a < HK; ++a) sds += y[a] * st[a];
-        sds = warp_sum(sds);
+          for (int a = 0; a < HK; ++a) sds += y[a] * st[a];
+          sds = warp_sum(sds);
+        }
         if (lane == 0) p.sds[at * kParts + part] = sds;
       }
       if (!warp_wait(&bars.ks, ph, abort, err, 82)) break;
@@ -222,7 +224,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
 #pragma unroll
         for (int j = 0; j < kTok; ++j) x[j] = u[j];
         put_pieces<PG, PG>(kNoTmem, 0, x, p.dup + at * kWF, lane, kChunk, tb);
-        fetch_pieces<PS, kTok>(p.ep + at * kWF, lane, kChunk, tb, x);
+        fetch_pieces<PG, kTok>(p.ep + at * kWF, lane, kChunk, tb, x);
 #pragma unroll
         for (int j = 0; j < kTok; ++j) x[j] *= u[j];
         const float s = sum_columns(x);
@@ -234,6 +236,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
         for (int j = 0; j < kTok; ++j) x[j] *= y[j];
         const float s = sum_columns(x);
         if ((lane & 1) == 0) p.vdv[at * kChunk + tb + lane / 2] = s;
+        // on to the chunk before: the tokens' sums, each in two lanes
+        sds += warp_sum((lane & 1) == 0 ? p.odo[at * kChunk + tb + lane / 2] - s : 0.f);
         const int64_t tok = (int64_t)c * kChunk + tb;
         if (on)
           store_tokens(static_cast<T*>(p.dv_) + ((b * p.time + t0 + tok) * p.hv + h) * p.dv + col,
@@ -263,7 +267,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == kIssuer) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }

@@ -9,9 +9,10 @@
 // a chain of three products with register work between them.  Q S0 and P u, which o is made of, run
 // in the shadow of that work (the first is scaled in place and the second added to it), and o is stored
 // in the shadow of the next chunk's K S0.  Sixteen warps, because the register work between two
-// products is bound by latency.  A thread beside them loads the chunk tiles by bulk copies (two chunks
-// in flight where they fit) and issues the MMAs: it is held up while the tensor cores' queue is full,
-// which in a computing warp made every other one wait for it.
+// products is bound by latency; a thread beside them issues the MMAs (it is held up while the tensor
+// cores' queue is full, which in a computing warp made every other one wait for it) and another loads
+// the chunk tiles by bulk copies, two chunks in flight where they fit (issuing those takes 800 cycles a
+// chunk).  An N = 64 MMA takes 47 cycles by itself, 60 to 120 while the warps use tensor memory.
 #include "qrb_delta_tc.cuh"
 
 namespace qrb {
@@ -20,12 +21,13 @@ namespace {
 
 template <int DKP, typename T, int PS, bool STORE>
 struct ScanLayout {
+  static constexpr int PO = STORE ? PS : OutPieces<T>::k;   // pieces of S0, P and u in o
   static constexpr int P = Pieces<T>::kIn;
   static constexpr int kK = tile_bytes(kChunk, P, DKP);
-  static constexpr int kX = tile_bytes(kChunk, PS, kChunk);
+  static constexpr int kX = tile_bytes(kChunk, PS, kChunk), kP = tile_bytes(kChunk, PO, kChunk);
   static constexpr int kV = kChunk * kLanes * (int)sizeof(T);
   static constexpr int kGates = 3 * kChunk * 4;
-  static constexpr int kOffQ = kK, kOffX = 2 * kK, kOffP = kOffX + kX, kOffV = kOffP + kX, kOffD = kOffV + kV;
+  static constexpr int kOffQ = kK, kOffX = 2 * kK, kOffP = kOffX + kX, kOffV = kOffP + kP, kOffD = kOffV + kV;
   static constexpr int kStage = kOffD + (STORE ? kV : 0);   // a multiple of 1024; gates apart
   static constexpr int kStages = 2 * (kStage + kGates) + 256 + 1024 <= kSmemLimit ? 2 : 1;
   static constexpr int kOffG = kStages * kStage;
@@ -39,11 +41,11 @@ struct ScanLayout {
   static constexpr bool kOver = PS == 3;
   static constexpr uint32_t tS = 0, tD = kOver ? 0 : kSp, tK = kOver ? (kSp > (uint32_t)DKP ? kSp : DKP) : kSp + DKP,
                             tQ = tK + 64, tF = tQ + 64, tU = tF + 32 * PS;
-  static_assert(tU + 32 * PS <= 512, "tensor memory");
+  static_assert(tU + 32 * PO <= 512, "tensor memory");
 };
 
 struct ScanBars {
-  uint64_t full[2], sp, ks, qs, f, xf, uw, ds, pu, o, share[4], drain;
+  uint64_t full[2], sp, ks, qs, f, xf, uw, sq, ds, pu, o, share[4], drain;
   uint32_t tmem;
   int abort;
 };
@@ -53,7 +55,8 @@ static_assert(sizeof(ScanBars) <= 256, "barrier block");
 template <int DKP, typename T, int PS, bool STORE>
 __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_constant__ Params p, int* err) {
   using L = ScanLayout<DKP, T, PS, STORE>;
-  constexpr int P = L::P, HK = DKP / kParts;   // HK: state rows of one thread
+  constexpr int PG = Pieces<T>::kS;   // pieces kept for dq, dk and dbeta
+  constexpr int P = L::P, PO = L::PO, HK = DKP / kParts;   // HK: state rows of one thread
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                        ~uintptr_t(1023));
@@ -74,68 +77,70 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
     mbar_init(&bars.full[0], 1);
     mbar_init(&bars.full[1], 1);
     for (uint64_t* x : {&bars.ks, &bars.qs, &bars.xf, &bars.ds, &bars.pu, &bars.drain}) mbar_init(x, 1);
-    for (uint64_t* x : {&bars.sp, &bars.f, &bars.uw, &bars.o}) mbar_init(x, kParts * quarters);
+    for (uint64_t* x : {&bars.sp, &bars.f, &bars.uw, &bars.sq, &bars.o}) mbar_init(x, kParts * quarters);
     for (int i = 0; i < 4; ++i) mbar_init(&bars.share[i], kParts);
     bars.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 16) tmem_alloc(&bars.tmem, 512);
+  if (warp == kIssuer) tmem_alloc(&bars.tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
 
-  if (warp == 16) {
-    // ---------------- loads and MMAs: one thread ----------------
+  if (warp == kLoader) {
+    // ---------------- loads: one thread ----------------
     if (lane == 0) {
-      int loaded = 0;
-      auto load = [&] {
-        const int c = loaded++;
-        unsigned char* d = sm + (c % L::kStages) * L::kStage;
-        uint64_t* bar = &bars.full[c % L::kStages];
+      int c = 0;
+      for (; c < nc; ++c) {
+        const int stage = c % L::kStages;
+        // the chunk that held this stage is done with: all its products and reads
+        if (c >= L::kStages && !mbar_wait_abort(&bars.o, (c - L::kStages) & 1, abort, err, 51)) break;
+        unsigned char* d = sm + stage * L::kStage;
+        uint64_t* bar = &bars.full[stage];
         const size_t qk = ((size_t)(slot0 + c) * p.hk + hk) * L::kK, at = slot_head(p, slot0 + c, h);
         mbar_arrive_expect_tx(bar, L::kStage + L::kGates);
         bulk_load(d, p.kt + qk, L::kK, bar);
-        bulk_load(d + L::kOffQ, p.qt + qk, L::kK, bar);
-        bulk_load(d + L::kOffX, p.xt + at * L::kX, L::kX, bar);
-        bulk_load(d + L::kOffP, p.pt + at * L::kX, L::kX, bar);
+        bulk_load(sm + L::kOffG + stage * L::kGates, p.gates + at * 3 * kChunk, L::kGates, bar);
         bulk_load(d + L::kOffV, p.vt + (at * nb + vb) * L::kV, L::kV, bar);
+        bulk_load(d + L::kOffX, p.xt + at * L::kX, L::kX, bar);
+        bulk_load(d + L::kOffQ, p.qt + qk, L::kK, bar);
+        bulk_load(d + L::kOffP, p.pt + at * L::kP, L::kP, bar);
         if (STORE) bulk_load(d + L::kOffD, p.dot + (at * nb + vb) * L::kV, L::kV, bar);
-        bulk_load(sm + L::kOffG + (c % L::kStages) * L::kGates, p.gates + at * 3 * kChunk, L::kGates, bar);
-      };
-      while (loaded < nc && loaded < L::kStages) load();
+      }
+      if (*abort)   // loads in flight must land before the block's memory goes
+        for (int s = 0; s < L::kStages; ++s)
+          if (c > s) mbar_wait(&bars.full[s], ((c - 1 - s) / L::kStages) & 1, 1u << 22);
+    }
+  } else if (warp == kIssuer) {
+    // ---------------- MMAs: one thread ----------------
+    if (lane == 0) {
       for (int c = 0; c < nc; ++c) {
         const uint32_t ph = c & 1, sb = smem_u32(sm + (c % L::kStages) * L::kStage);
-        if (L::kStages == 1 && c > 0) {   // the one stage is free once all are through with the last chunk
-          if (!mbar_wait_abort(&bars.o, ph ^ 1, abort, err, 51)) break;
-          load();
-        }
         if (!mbar_wait_abort(&bars.full[c % L::kStages], (c / L::kStages) & 1, abort, err, 52)) break;
         if (!mbar_wait_abort(&bars.sp, ph, abort, err, 53)) break;
         tc_fence_after();
         mma_pieces<64, DKP, false, PS, P, PS>(tmem + L::tK, tmem + L::tS, DKP / 2, sb, 0);
         mma_commit(&bars.ks);
-        if (L::kStages == 2 && c > 0) {   // o of the last chunk is read: Q S0 may land, its stage may go
-          if (!mbar_wait_abort(&bars.o, ph ^ 1, abort, err, 54)) break;
-          if (loaded < nc) load();
-          tc_fence_after();
-        }
-        mma_pieces<64, DKP, false, PS, P, PS>(tmem + L::tQ, tmem + L::tS, DKP / 2, sb + L::kOffQ, 0);
-        mma_commit(&bars.qs);
-        if (!mbar_wait_abort(&bars.f, ph, abort, err, 55)) break;
+        if (!mbar_wait_abort(&bars.f, ph, abort, err, 54)) break;
         tc_fence_after();
         mma_pieces<64, 64, false, PS, PS, PS>(tmem + L::tK, tmem + L::tF, 32, sb + L::kOffX, 0);
         mma_commit(&bars.xf);
+        if (c > 0 && !mbar_wait_abort(&bars.o, ph ^ 1, abort, err, 55)) break;   // the last chunk's o is read
+        tc_fence_after();
+        mma_pieces<64, DKP, false, PO, P, PO>(tmem + L::tQ, tmem + L::tS, DKP / 2, sb + L::kOffQ, 0);
+        mma_commit(&bars.qs);
         if (!mbar_wait_abort(&bars.uw, ph, abort, err, 56)) break;
+        if (L::kOver && !mbar_wait_abort(&bars.qs, ph, abort, err, 57)) break;   // pieces of S read
         tc_fence_after();
         mma_pieces<DKP, 64, true, PS, P, PS>(tmem + L::tD, tmem + L::tF, 32, sb, 0);
         mma_commit(&bars.ds);
-        mma_pieces<64, 64, false, PS, PS, PS>(tmem + L::tQ, tmem + L::tU, 32, sb + L::kOffP, 1);
+        if (!mbar_wait_abort(&bars.sq, ph, abort, err, 58)) break;
+        tc_fence_after();
+        mma_pieces<64, 64, false, PO, PO, PO>(tmem + L::tQ, tmem + L::tU, 32, sb + L::kOffP, 1);
         mma_commit(&bars.pu);
       }
-      if (*abort) {   // loads in flight must land, MMAs in flight end, before the block's memory goes
-        for (int s = 0; s < L::kStages; ++s)
-          if (loaded > s) mbar_wait(&bars.full[s], ((loaded - 1 - s) / L::kStages) & 1, 1u << 22);
+      if (*abort) {   // MMAs in flight must end before tensor memory goes
         mma_commit(&bars.drain);
         mbar_wait(&bars.drain, 0, 1u << 22);
       }
@@ -160,8 +165,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
       float y[HK];
 #pragma unroll
       for (int i = 0; i < HK; ++i) y[i] = st[i];
-      put_pieces<PS, STORE ? PS : 0>(tl + L::tS + kb / 2, DKP / 2, y,
-                                     p.s0p + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWS, lane, DKP, kb);
+      unsigned char* to = STORE ? p.s0p + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWS : nullptr;
+      // all pieces where the backward recurrence takes <S', dS'> from them, else those dq and dk need
+      if (STORE && (nc - c) % kAnchor == 0) put_pieces<PS, PS>(tl + L::tS + kb / 2, DKP / 2, y, to, lane, DKP, kb);
+      else put_pieces<PS, STORE ? PG : 0>(tl + L::tS + kb / 2, DKP / 2, y, to, lane, DKP, kb);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&bars.sp);
@@ -183,14 +190,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&bars.f);
-      if (!warp_wait(&bars.qs, ph, abort, err, 63)) break;
-      tc_fence_after();
-      ld_cols(tl + L::tQ + tb, x);   // scale gamma Q S0 goes back, P u is added to it there
-      {
-        uint32_t y[kTok];
-        with_tokens(gates.gam, [&](int i, float g) { y[i] = __float_as_uint(p.scale * g * x[i]); });
-        st_cols(tl + L::tQ + tb, y);
-      }
       if (!warp_wait(&bars.xf, ph, abort, err, 64)) break;
       tc_fence_after();
       ld_cols(tl + L::tK + tb, x);
@@ -200,14 +199,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
       {
         float y[kTok];
         with_tokens(gates.tail, [&](int i, float g) { y[i] = g * e[i]; });
-        put_pieces<PS, 0>(tl + L::tU + tb / 2, 32, e);
+        put_pieces<PO, 0>(tl + L::tU + tb / 2, 32, e);
         put_pieces<PS, 0>(tl + L::tF + tb / 2, 32, y);
       }
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&bars.uw);
       if (STORE)
-        put_pieces<PS, PS>(kNoTmem, 0, x, p.ep + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWF, lane, kChunk, tb);
+        put_pieces<PG, PG>(kNoTmem, 0, x, p.ep + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWF, lane, kChunk, tb);
+      if (!warp_wait(&bars.qs, ph, abort, err, 63)) break;
+      tc_fence_after();
+      ld_cols(tl + L::tQ + tb, x);   // scale gamma Q S0 goes back, P u is added to it there
+      {
+        uint32_t y[kTok];
+        with_tokens(gates.gam, [&](int i, float g) { y[i] = __float_as_uint(p.scale * g * x[i]); });
+        st_cols(tl + L::tQ + tb, y);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&bars.sq);
       const float glast = *gates.last;
       if (!warp_wait(&bars.ds, ph, abort, err, 65)) break;
       tc_fence_after();
@@ -250,7 +260,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == kIssuer) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }

@@ -20,7 +20,8 @@ using namespace sm100;
 constexpr int kLanes = 128;                 // value columns per block of the recurrences
 constexpr int kParts = 4;                   // threads that share a value column
 constexpr int kTok = kChunk / kParts;       // tokens of a thread
-constexpr int kTcThreads = kLanes * kParts + 32;   // sixteen warps compute, one issues loads and MMAs
+constexpr int kIssuer = kLanes * kParts / 32, kLoader = kIssuer + 1;   // sixteen warps compute, one issues MMAs, one loads
+constexpr int kTcThreads = 32 * (kLoader + 1);
 constexpr int kSmemLimit = 232448;
 
 // kind::f16, bf16 operands, fp32 accumulation, M = 128, A in tensor memory.
