@@ -48,7 +48,8 @@ namespace qrb {
 namespace delta {
 
 constexpr int kChunk = 64;   // tokens per chunk
-constexpr int kTile = 32;    // value columns per tile of the sequential kernels
+constexpr int kTile = 32;    // value columns per tile the recurrences leave for the gradient kernel
+constexpr int kLanes = 128;  // value columns per block of the recurrences
 constexpr float kMinLog = -120.f;   // exp(kMinLog) is 0 in fp32: a smaller g (-inf too) is the same decay
 
 struct Strides {

@@ -24,10 +24,10 @@ struct GLayout {
   static constexpr int kD = tile_bytes(kChunk, P, kTile);
   // tiles in the workspace have kBackPieces pieces; the first kS of them are a prefix
   static constexpr int kWS = tile_bytes(kTile, kBackPieces, DKP), kWF = tile_bytes(kTile, kBackPieces, kChunk);
-  static constexpr int kOffE = 0, kOffDU = kF, kOffS0 = 2 * kF, kOffDS = kOffS0 + kS;
-  static constexpr int kStage = kOffDS + kS;
+  static constexpr int kOffE = 0, kOffDU = kF, kOffS0 = 2 * kF, kOffDS = kOffS0 + kS, kOffD = kOffDS + kS;
+  static constexpr int kStage = kOffD + kD;
   static constexpr int kZ = tile_bytes(kChunk, PS, kChunk);
-  static constexpr int kOffQ = kK, kOffD = 2 * kK, kOffT = kOffD + kD;
+  static constexpr int kOffQ = kK, kOffT = 2 * kK;
   // Z and N are formed when the last tile is consumed and lie over the tiles
   static constexpr int kTiles = kStages * kStage > 2 * kZ ? kStages * kStage : 2 * kZ;
   static constexpr int kOffG = kOffT + kTiles;     // G (64 doubles), gates, row sums, reductions
@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(512) grad_kernel(Params p) {
   constexpr int P = L::P, PS = L::PS;
   constexpr int NT = DKP / 32;           // 8-column blocks of q / k columns a warp holds
   extern __shared__ __align__(128) unsigned char sm[];
-  unsigned char *K = sm, *Q = sm + L::kOffQ, *D = sm + L::kOffD, *TT = sm + L::kOffT;
+  unsigned char *K = sm, *Q = sm + L::kOffQ, *TT = sm + L::kOffT;
   unsigned char *Z = TT, *N = TT + L::kZ;
   double* G = reinterpret_cast<double*>(sm + L::kOffG);
   float* gates = reinterpret_cast<float*>(G + 64);
@@ -58,10 +58,12 @@ __global__ void __launch_bounds__(512) grad_kernel(Params p) {
   float tq_[NT][4], tk_[NT][4];          // sums over the heads of the group
   zero(tq_);
   zero(tk_);
-  const int er = tid >> 3, ec = (tid & 7) * 4;   // elementwise work on 64 x 32 tiles: row, first column
   for (int hh = 0; hh < p.group; ++hh) {
     const int h = hk * p.group + hh;
     const size_t at = slot_head(p, c, h);
+    auto dO = [&](int n) {   // the tile's columns of dO, kLanes values a token
+      return reinterpret_cast<const T*>(p.dot) + (at * ((p.dv + kLanes - 1) / kLanes) + n / 4) * kChunk * kLanes + n % 4 * kTile;
+    };
     auto load = [&](int n, int stage) {
       unsigned char* d = TT + stage * L::kStage;
       const size_t t = at * p.nv + n;
@@ -69,6 +71,9 @@ __global__ void __launch_bounds__(512) grad_kernel(Params p) {
       cp_tile(d + L::kOffDU, p.dup + t * L::kWF, L::kF);
       cp_tile(d + L::kOffS0, p.s0p + t * L::kWS, L::kS);
       cp_tile(d + L::kOffDS, p.dsp + t * L::kWS, L::kS);
+      // dO: 32 columns of the staged tile, which bf16 tiles take unit by unit
+      if (P == 1 && tid < 4 * kChunk)
+        cp16(d + L::kOffD + tile_off(kChunk, tid >> 2, (tid & 3) * 8), dO(n) + (size_t)(tid >> 2) * kLanes + (tid & 3) * 8);
       cp_commit();
     };
     __syncthreads();                     // the previous head's Z, N and sums are consumed
@@ -85,12 +90,12 @@ __global__ void __launch_bounds__(512) grad_kernel(Params p) {
       const int stage = L::kStages == 2 ? (n & 1) : 0;
       unsigned char* d = TT + stage * L::kStage;
       const unsigned char *E = d + L::kOffE, *DU = d + L::kOffDU, *S0 = d + L::kOffS0, *DS = d + L::kOffDS;
-      float x[4];
+      unsigned char* D = d + L::kOffD;
+      T x[4];
+      if (P > 1) {
+        const T* from = dO(n) + (size_t)(tid >> 3) * kLanes + (tid & 7) * 4;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int col = n * kTile + ec + i;
-        const bool in = er < ch.len && col < p.dv;
-        x[i] = in ? to_f(static_cast<const T*>(p.d_o)[ch.b * p.dos.b + (ch.t0 + er) * p.dos.t + h * p.dos.h + col]) : 0.f;
+        for (int i = 0; i < 4; ++i) x[i] = __ldg(from + i);
       }
       if (L::kStages == 2) {
         cp_wait_all();
@@ -101,9 +106,11 @@ __global__ void __launch_bounds__(512) grad_kernel(Params p) {
         load(n, 0);
         cp_wait_all();
       }
-      put2<P>(D, kChunk, kTile, er, ec, x[0], x[1]);
-      put2<P>(D, kChunk, kTile, er, ec + 2, x[2], x[3]);
-      __syncthreads();
+      if (P > 1) {
+        put2<P>(D, kChunk, kTile, tid >> 3, (tid & 7) * 4, to_f(x[0]), to_f(x[1]));
+        put2<P>(D, kChunk, kTile, tid >> 3, (tid & 7) * 4 + 2, to_f(x[2]), to_f(x[3]));
+      }
+      if (P > 1 || L::kStages == 1) __syncthreads();
       mma_tile<NT, false, true, P, PS, PS, false, true>(aq, D, kChunk, kTile, m0, S0, kTile, DKP, d0, 0, kTile);
       mma_tile<NT, true, true, PS, PS, PS, true, true>(ay, DU, kTile, kChunk, m0, S0, kTile, DKP, d0, 0, kTile);
       mma_tile<NT, true, true, PS, PS, PS, true, true>(au, E, kTile, kChunk, m0, DS, kTile, DKP, d0, 0, kTile);

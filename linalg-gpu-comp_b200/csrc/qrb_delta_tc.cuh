@@ -17,7 +17,6 @@ namespace delta {
 
 using namespace sm100;
 
-constexpr int kLanes = 128;                 // value columns per block of the recurrences
 constexpr int kParts = 4;                   // threads that share a value column
 constexpr int kTok = kChunk / kParts;       // tokens of a thread
 constexpr int kIssuer = kLanes * kParts / 32, kLoader = kIssuer + 1;   // sixteen warps compute, one issues MMAs, one loads
