@@ -60,9 +60,12 @@ template <int BN, bool PAIR>
 struct Cfg {
   static constexpr int kRowsB = PAIR ? BN / 2 : BN;   // rows of B this block loads
   static constexpr uint32_t kA = kBM * kBK * 2, kB = kRowsB * kBK * 2, kStage = kA + kB;
-  static constexpr int kStages = kStage > 40960 ? 4 : 6;
+  static constexpr uint32_t kTurn = 8 * 32 * 33 * 4;   // a 32 x 32 tile for each epilogue warp to turn
+  static constexpr int kStages = kStage > 40960 ? 3 : (kStage > 24576 ? 5 : 6);
   static constexpr uint32_t kBar = kStages * kStage;
-  static constexpr uint32_t kSmem = kBar + 256 + 1024;
+  static constexpr uint32_t kOffTurn = kBar + 256;
+  static constexpr uint32_t kSmem = kOffTurn + kTurn + 1024;
+  static_assert(kSmem <= 232448, "shared memory of one block");
 };
 
 struct Bars {
@@ -103,9 +106,9 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int dtype) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Eight neighbouring outputs, 16-byte aligned where `vec`.
-__device__ __forceinline__ void store8(void* p, int64_t i, int dtype, const float* x, int count, bool vec) {
-  if (vec && count == 8) {
+// Eight neighbouring outputs of a 16-byte aligned row, the first `count` of which exist.
+__device__ __forceinline__ void store8(void* p, int64_t i, int dtype, const float* x, int count) {
+  if (count == 8) {
     if (dtype == QRB_F32) {
       float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
       q[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -122,8 +125,8 @@ __device__ __forceinline__ void store8(void* p, int64_t i, int dtype, const floa
     if (j < count) store1(p, i + j, dtype, x[j]);
 }
 
-__device__ __forceinline__ void add8(const void* p, int64_t i, int dtype, float* x, int count, bool vec) {
-  if (vec && count == 8 && dtype != QRB_F32) {
+__device__ __forceinline__ void add8(const void* p, int64_t i, int dtype, float* x, int count) {
+  if (count == 8 && dtype != QRB_F32) {
     const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -302,6 +305,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     // ---------------- epilogue: TMEM lane = A's row, half of the columns a warp ----------------
     const int q = warp & 3, c_first = ((warp - 4) >> 2) * (BN / 2), c_last = c_first + BN / 2;
     const uint32_t tl = (uint32_t)(32 * q) << 16;
+    float* turned = reinterpret_cast<float*>(sm + C::kOffTurn) + (warp - 4) * 32 * 33;
     const Epilogue& e = g.e;
     const bool vec = (e.y == nullptr || aligned_rows(e.y, e.ldy, e.dtype)) &&
                      (e.residual == nullptr || aligned_rows(e.residual, e.ldr, e.dtype)) &&
@@ -341,6 +345,38 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           const float cb = c0 + c + lane < g.N ? load1(e.bias, c0 + c + lane, e.dtype) : 0.f;
 #pragma unroll
           for (int j = 0; j < 32; ++j) x[j] += __shfl_sync(0xffffffffu, cb, j);
+        }
+        if (g.splits == 1 && !g.swap && !vec) {
+          // rows that are not 16-byte aligned: a lane's row written value by value would touch 32 rows an
+          // instruction, so the warp turns the tile and writes 32 neighbouring columns of one row at a time
+          const int rows = (int)max((int64_t)0, min((int64_t)32, g.M - (r - lane)));
+          const bool mine = c0 + c + lane < g.N;
+          auto turn = [&] {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) turned[lane * 33 + j] = x[j];
+            __syncwarp();
+          };
+          const int64_t row = r - lane, cc = c0 + c + lane;
+          if (e.pre != nullptr) {
+            turn();
+            if (mine)
+              for (int i = 0; i < rows; ++i) store1(e.pre, (row + i) * e.ldpre + cc, e.dtype, turned[i * 33 + lane]);
+          }
+          activate_all(x, e.act);
+          turn();
+          if (mine) {
+            for (int i = 0; i < rows; i += 8) {
+              float add[8];
+#pragma unroll
+              for (int u = 0; u < 8; ++u)
+                add[u] = e.residual != nullptr ? load1(e.residual, (row + min(i + u, rows - 1)) * e.ldr + cc, e.dtype) : 0.f;
+#pragma unroll
+              for (int u = 0; u < 8; ++u)
+                if (i + u < rows) store1(e.y, (row + i + u) * e.ldy + cc, e.dtype, turned[(i + u) * 33 + lane] + add[u]);
+            }
+          }
+          continue;
         }
         if (r >= g.M) continue;
         if (g.splits > 1) {
@@ -383,15 +419,15 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         if (e.pre != nullptr)
 #pragma unroll
           for (int j = 0; j < 32; j += 8)
-            store8(e.pre, r * e.ldpre + c0 + c + j, e.dtype, x + j, (int)max((int64_t)0, min((int64_t)8, left - j)), vec);
+            store8(e.pre, r * e.ldpre + c0 + c + j, e.dtype, x + j, (int)max((int64_t)0, min((int64_t)8, left - j)));
         activate_all(x, e.act);
         if (e.residual != nullptr)
 #pragma unroll
           for (int j = 0; j < 32; j += 8)
-            add8(e.residual, r * e.ldr + c0 + c + j, e.dtype, x + j, (int)max((int64_t)0, min((int64_t)8, left - j)), vec);
+            add8(e.residual, r * e.ldr + c0 + c + j, e.dtype, x + j, (int)max((int64_t)0, min((int64_t)8, left - j)));
 #pragma unroll
         for (int j = 0; j < 32; j += 8)
-          store8(e.y, r * e.ldy + c0 + c + j, e.dtype, x + j, (int)max((int64_t)0, min((int64_t)8, left - j)), vec);
+          store8(e.y, r * e.ldy + c0 + c + j, e.dtype, x + j, (int)max((int64_t)0, min((int64_t)8, left - j)));
       }
     }
   }

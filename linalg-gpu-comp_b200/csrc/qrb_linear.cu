@@ -68,17 +68,23 @@ __device__ __forceinline__ void put8f(void* to, int64_t i, int64_t plane, const 
 }
 
 // rows x cols of `from` (row stride ld) to rows of `pitch` elements: eight columns a thread, stored as
-// 16-byte units (the columns that pad a row become zero).
+// 16-byte units (the columns that pad a row become zero).  Up to two matrices a launch (blockIdx.z).
 template <typename T>
-__global__ void __launch_bounds__(256) layout_kernel(const T* from, int64_t ld, int64_t rows, int64_t cols, void* to,
-                                                     int64_t pitch) {
-  const int64_t c = ((int64_t)blockIdx.x * 32 + (threadIdx.x & 31)) * 8, plane = rows * pitch;
-  if (c >= pitch) return;
-  for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.y * 8) {
+struct LayoutJob {
+  const T* from;
+  int64_t ld, rows, cols, pitch;
+  void* to;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) layout_kernel(LayoutJob<T> a, LayoutJob<T> b) {
+  const LayoutJob<T>& g = blockIdx.z == 0 ? a : b;
+  const int64_t c = ((int64_t)blockIdx.x * 32 + (threadIdx.x & 31)) * 8, plane = g.rows * g.pitch;
+  if (c >= g.pitch) return;
+  for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < g.rows; r += (int64_t)gridDim.y * 8) {
     float e[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = tof(__ldg(from + r * ld + min(c + j, cols - 1)));
-    put8f<T>(to, r * pitch + c, plane, e, (int)min((int64_t)8, cols - c));
+    for (int j = 0; j < 8; ++j) e[j] = tof(__ldg(g.from + r * g.ld + min(c + j, g.cols - 1)));
+    put8f<T>(g.to, r * g.pitch + c, plane, e, (int)min((int64_t)8, g.cols - c));
   }
 }
 
@@ -334,34 +340,60 @@ int check_ws(const void* ws, size_t have, size_t need) {
   return QRB_OK;
 }
 
-template <typename T>
-void layout_t(const void* p, int64_t ld, int64_t rows, int64_t cols, void* to, cudaStream_t s) {
-  const int64_t pitch = pitch_of(cols), by = (rows + 7) / 8;
-  const dim3 grid((unsigned)((pitch + 255) / 256), (unsigned)(by < 4096 ? by : 4096));
-  qrb::gemm::layout_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(p), ld, rows, cols, to, pitch);
-}
+// The operands a product reads: x (rows x cols, row stride ld) itself, or a copy that a Layouts call makes.
+struct Layouts {
+  int dtype;
+  struct Job {
+    const void* p;
+    int64_t ld, rows, cols;
+    void* to;
+  } job[2];
+  int jobs = 0;
 
-// The operand a product reads: x itself, or its copy at `to`.
-int operand(Operand& o, int dtype, const void* p, int64_t ld, int64_t rows, int64_t cols, bool mn_major, void* to,
-            cudaStream_t s) {
-  o.mn_major = mn_major;
-  o.pieces = dtype == QRB_F32 ? 3 : 1;
-  if (direct(dtype, p, ld, cols)) {
-    o.p = p;
-    o.ld = ld;
-    o.plane = 0;
+  explicit Layouts(int dtype_) : dtype(dtype_) {}
+
+  Operand operand(const void* p, int64_t ld, int64_t rows, int64_t cols, bool mn_major, void* to) {
+    Operand o{};
+    o.mn_major = mn_major;
+    o.pieces = dtype == QRB_F32 ? 3 : 1;
+    if (direct(dtype, p, ld, cols)) {
+      o.p = p;
+      o.ld = ld;
+      return o;
+    }
+    o.p = to;
+    o.ld = pitch_of(cols);
+    o.plane = rows * o.ld;
+    job[jobs++] = {p, ld, rows, cols, to};
+    return o;
+  }
+
+  template <typename T>
+  void go(cudaStream_t s) const {
+    qrb::gemm::LayoutJob<T> j[2]{};
+    int64_t px = 0, py = 0;
+    for (int i = 0; i < jobs; ++i) {
+      j[i] = {static_cast<const T*>(job[i].p), job[i].ld, job[i].rows, job[i].cols, pitch_of(job[i].cols), job[i].to};
+      if (j[i].pitch > px) px = j[i].pitch;
+      if (j[i].rows > py) py = j[i].rows;
+    }
+    py = (py + 7) / 8;
+    const dim3 grid((unsigned)((px + 255) / 256), (unsigned)(py < 4096 ? py : 4096), (unsigned)jobs);
+    qrb::gemm::layout_kernel<T><<<grid, 256, 0, s>>>(j[0], j[1]);
+  }
+
+  int run(cudaStream_t s) const {
+    if (jobs == 0) return QRB_OK;
+    double cells = 0;
+    for (int i = 0; i < jobs; ++i) cells += (double)job[i].rows * job[i].cols;
+    qrb::LaunchTimer t("linear_layout_kernel", s, cells * (dtype == QRB_F32 ? 10 : 4), 0);
+    if (dtype == QRB_F32) go<float>(s);
+    else if (dtype == QRB_BF16) go<__nv_bfloat16>(s);
+    else go<__half>(s);
+    CUDA(cudaGetLastError(), "linear layout launch");
     return QRB_OK;
   }
-  o.p = to;
-  o.ld = pitch_of(cols);
-  o.plane = rows * o.ld;
-  qrb::LaunchTimer t("linear_layout_kernel", s, (double)rows * cols * 2 * esize(dtype), 0);
-  if (dtype == QRB_F32) layout_t<float>(p, ld, rows, cols, to, s);
-  else if (dtype == QRB_BF16) layout_t<__nv_bfloat16>(p, ld, rows, cols, to, s);
-  else layout_t<__half>(p, ld, rows, cols, to, s);
-  CUDA(cudaGetLastError(), "linear layout launch");
-  return QRB_OK;
-}
+};
 
 constexpr int64_t kVecRows = 4;   // up to here gemv_kernel: it reads the weight once and lays nothing out
 
@@ -517,9 +549,10 @@ int qrb_linear_forward(const qrb_linear_args* a, void* ws, size_t wsb, void* str
     return QRB_OK;
   }
   char* w8 = static_cast<char*>(ws);
-  Operand x, w;
-  TRY(operand(x, a->dtype, a->x, a->ldx, a->m, a->k, false, w8 + l.x, s));
-  TRY(operand(w, a->dtype, a->w, a->ldw, a->n, a->k, false, w8 + l.w, s));
+  Layouts lay(a->dtype);
+  const Operand x = lay.operand(a->x, a->ldx, a->m, a->k, false, w8 + l.x);
+  const Operand w = lay.operand(a->w, a->ldw, a->n, a->k, false, w8 + l.w);
+  TRY(lay.run(s));
   CUDA(qrb::gemm::multiply(x, w, a->m, a->n, a->k, a->dtype == QRB_F16, e, reinterpret_cast<float*>(w8 + l.part), s),
        "linear product launch");
   return QRB_OK;
@@ -574,16 +607,17 @@ int qrb_linear_backward(const qrb_linear_backward_args* a, void* ws, size_t wsb,
   Epilogue e{};
   e.dtype = a->dtype;
   e.ldy = a->k;
+  Layouts lay(a->dtype);
+  Operand x{}, w{};
+  if (a->dx != nullptr) w = lay.operand(a->w, a->ldw, a->n, a->k, true, w8 + l.w);
+  if (a->dw != nullptr) x = lay.operand(a->x, a->ldx, a->m, a->k, true, w8 + l.x);
+  TRY(lay.run(s));
   if (a->dx != nullptr) {
-    Operand w;
-    TRY(operand(w, a->dtype, a->w, a->ldw, a->n, a->k, true, w8 + l.w, s));
     p.mn_major = 0;
     e.y = a->dx;
     CUDA(qrb::gemm::multiply(p, w, a->m, a->k, a->n, half, e, part, s), "linear dx launch");
   }
   if (a->dw != nullptr) {
-    Operand x;
-    TRY(operand(x, a->dtype, a->x, a->ldx, a->m, a->k, true, w8 + l.x, s));
     p.mn_major = 1;
     e.y = a->dw;
     CUDA(qrb::gemm::multiply(p, x, a->n, a->k, a->m, half, e, part, s), "linear dw launch");
