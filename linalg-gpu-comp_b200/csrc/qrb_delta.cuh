@@ -25,11 +25,12 @@
 // Precision: states, accumulators and gates are fp32 (G fp64).  Products run on the tensor cores
 // with every fp32 operand split into bf16 pieces, x = x0 + x1 (+ x2): two pieces keep 2^-18 of x,
 // three 2^-27; bf16 inputs are one piece and exact, fp16 inputs two and exact.  Products of pieces
-// i, j with i + j below the piece count are added.  Forward takes two pieces for the 16-bit types
-// (the fp32 final state is then within about 3e-6), three for fp32.  The backward recurrences take
-// three for every type, because dg is the small difference of the sums above: with two it was
-// 2e-5 off, four to eight times the error of its terms.  dq and dk, rounded to their type in the
-// end, take two pieces of the 16-bit types, and so does e in dbeta.
+// i, j with i + j below the piece count are added.  X, F = beta e0 and W = tail u, whose
+// errors the state keeps, take three pieces; S0, P and u, which enter e and o once, two for the 16-bit
+// types (with two everywhere the fp32 final state was 3e-6 off, so it is below 1e-6).  fp32 and the
+// backward recurrences take three throughout: dg is the small difference of the sums above, and with two
+// it was 2e-5 off, four to eight times the error of its terms.  dq and dk, rounded to their type in the
+// end, take two pieces of the 16-bit types.
 //
 // Operand tiles are bf16 in blocks of 64 columns (128 bytes a row), the 16-byte units of a row
 // XORed with row % 8, both in shared memory (where ldmatrix then reads without bank conflicts)
@@ -85,7 +86,7 @@ struct Params {
 };
 
 template <typename T>
-struct Pieces;   // kIn: pieces of an input, kS: of an fp32 operand of the forward pass and of dq, dk
+struct Pieces;   // kIn: pieces of an input, kS: of S0, P and u in the forward pass, and in dq, dk
 template <>
 struct Pieces<__nv_bfloat16> {
   static constexpr int kIn = 1, kS = 2;
@@ -99,15 +100,13 @@ struct Pieces<float> {
   static constexpr int kIn = 3, kS = 3;
 };
 constexpr int kBackPieces = 3;   // of the backward recurrences
-// Pieces of S0, P and u in o (one bf16 piece was tried for bf16 calls: its two products cancel in part, and
-// o was 3.6e-3 off in place of 1.7e-3).
-template <typename T>
-struct OutPieces {
-  static constexpr int k = Pieces<T>::kS;
-};
+constexpr int kChainPieces = 3;  // of X, F and W
+// (One bf16 piece of S0, P and u in o was tried for bf16 calls: its two products cancel in part, and o was
+// 3.6e-3 off in place of 1.7e-3.)
 // Backward: every kAnchor-th chunk from a sequence's end takes <S', dS'> from the states themselves, the
-// others from the next chunk's by the same identity as dg within a chunk (see qrb_delta_rscan.cu).
-constexpr int kAnchor = 8;
+// others from the next chunk's by the same identity as dg within a chunk (see qrb_delta_rscan.cu).  The
+// states' third pieces are then kept and read half as often; at every eighth dg was 1.8e-6 off.
+constexpr int kAnchor = 2;
 
 
 __device__ __forceinline__ float to_f(float x) { return x; }
@@ -232,8 +231,18 @@ __device__ __forceinline__ void mma_tile(float (&acc)[NT][4], const unsigned cha
                           AT ? (lane >> 3) & 1 : lane >> 4);
   const LaneAddr<BU> b_at(B, brows, BT ? lane & 15 : n0 + (lane & 7) + ((lane >> 4) & 1) * 8,
                           BT ? lane >> 4 : (lane >> 3) & 1);
+  // Tensor-core sums truncate: where three pieces promise fp32 accuracy, two steps of k are summed
+  // apart and added in fp32 (48 truncating additions to one sum left dk 1.7e-6 off).
+  constexpr bool kApart = PM == 3;
+  float part[kApart ? NT : 1][4];
 #pragma unroll 2
   for (int k = k0; k < k1; k += 16) {
+    if (kApart && ((k - k0) & 16) == 0) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[kApart ? j : 0][i] = 0.f;
+    }
     uint32_t a[PA][4];
 #pragma unroll
     for (int p = 0; p < PA; ++p) {
@@ -250,11 +259,17 @@ __device__ __forceinline__ void mma_tile(float (&acc)[NT][4], const unsigned cha
 #pragma unroll
         for (int p = 0; p < PA; ++p) {
           if (p + q < PM) {
-            mma16816(acc[j], a[p], b[0], b[1]);
-            mma16816(acc[j + 1], a[p], b[2], b[3]);
+            mma16816(kApart ? part[kApart ? j : 0] : acc[j], a[p], b[0], b[1]);
+            mma16816(kApart ? part[kApart ? j + 1 : 0] : acc[j + 1], a[p], b[2], b[3]);
           }
         }
       }
+    }
+    if (kApart && (((k - k0) & 16) != 0 || k + 16 >= k1)) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][i] += part[kApart ? j : 0][i];
     }
   }
 }

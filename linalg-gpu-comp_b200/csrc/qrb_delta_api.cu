@@ -102,7 +102,7 @@ Layout layout(const qrb_delta_args& a, bool backward) {
   l.cstart = take(a.seq_offsets != nullptr ? (2 * a.nseq + 1) * 4 : 0);
   l.kt = take(n * a.hk * tile_bytes(kChunk, pi, dkp));
   l.qt = take(n * a.hk * tile_bytes(kChunk, pi, dkp));
-  l.xt = take(n * a.hv * tile_bytes(kChunk, ps, kChunk));
+  l.xt = take(n * a.hv * tile_bytes(kChunk, kChainPieces, kChunk));
   l.pt = take(n * a.hv * tile_bytes(kChunk, ps, kChunk));
   l.gates = take(n * a.hv * 3 * kChunk * 4);
   const size_t staged = n * a.hv * ((a.dv + 127) / 128) * kChunk * 128 * (a.dtype == QRB_F32 ? 4 : 2);

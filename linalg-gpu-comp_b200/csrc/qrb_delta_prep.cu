@@ -81,7 +81,7 @@ struct PrepLayout {
   static constexpr int kQK = tile_bytes(kChunk, P, DKP), kXP = tile_bytes(kChunk, PS, kChunk), kPP = tile_bytes(kChunk, PO, kChunk);
   static_assert(PO <= PS, "overlay");
   // once the products are taken, over k and q: X's two 32 x 32 diagonal blocks (fp32), the right sides
-  // of a merge, and the pieces of P, later those of X.  52 KB with 16-bit operands: four blocks an SM.
+  // of a merge, and the pieces of P, later those of X.  60 KB with bf16 operands: three blocks an SM.
   static constexpr int kOffS = 0, kOffR = 2 * 32 * kRStride * 4, kOffT = 16384;
   static_assert(kOffR + 32 * kRStride * 4 <= kOffT, "overlay");
   static constexpr int kOffM = 2 * kQK > kOffT + kXP ? 2 * kQK : kOffT + kXP;   // M, fp32
@@ -186,7 +186,7 @@ __device__ __forceinline__ void block_product(float (&r)[2][4], const float* m0,
 }
 
 template <int DKP, typename T, int PS, int PO>
-__global__ void __launch_bounds__(kPrepThreads, PS == 3 ? 2 : 4) prep_kernel(Params p, int vec) {
+__global__ void __launch_bounds__(kPrepThreads, Pieces<T>::kIn == 1 ? 3 : 2) prep_kernel(Params p, int vec) {
   using L = PrepLayout<DKP, T, PS, PO>;
   constexpr int P = L::P;
   extern __shared__ __align__(128) unsigned char sm[];
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kPrepThreads, PS == 3 ? 2 : 4) prep_kernel(Par
     const int blk = warp & 3, m0 = 16 * blk;
     float acc[8][4];
     zero(acc);
-    mma_tile<8, false, false, P, P, PS>(acc, warp < 4 ? kt : qt, kChunk, DKP, m0, kt, kChunk, DKP, 0, 0, DKP);
+    mma_tile<8, false, false, P, P, P == 1 ? 1 : 3>(acc, warp < 4 ? kt : qt, kChunk, DKP, m0, kt, kChunk, DKP, 0, 0, DKP);
     __syncthreads();   // k and q are read: their memory changes hands
     // decays: exact in the diagonal block, the product of two factors <= 1 (for g <= 0) before it
 #pragma unroll
@@ -460,10 +460,9 @@ static cudaError_t pick_prep(const Params& p, cudaStream_t s) {
 
 cudaError_t launch_prep(const Params& p, int dtype, cudaStream_t s) {
   constexpr int B = kBackPieces;
-  if (dtype == 1)
-    return p.backward ? pick_prep<__nv_bfloat16, B, B>(p, s)
-                      : pick_prep<__nv_bfloat16, 2, OutPieces<__nv_bfloat16>::k>(p, s);
-  if (dtype == 2) return p.backward ? pick_prep<__half, B, B>(p, s) : pick_prep<__half, 2, OutPieces<__half>::k>(p, s);
+  constexpr int C = kChainPieces;
+  if (dtype == 1) return p.backward ? pick_prep<__nv_bfloat16, C, B>(p, s) : pick_prep<__nv_bfloat16, C, 2>(p, s);
+  if (dtype == 2) return p.backward ? pick_prep<__half, C, B>(p, s) : pick_prep<__half, C, 2>(p, s);
   return pick_prep<float, 3, 3>(p, s);
 }
 

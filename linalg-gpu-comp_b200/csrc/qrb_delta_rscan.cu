@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
 #pragma unroll
         for (int j = 0; j < kTok; ++j) x[j] = u[j];
         put_pieces<PG, PG>(kNoTmem, 0, x, p.dup + at * kWF, lane, kChunk, tb);
-        fetch_pieces<PG, kTok>(p.ep + at * kWF, lane, kChunk, tb, x);
+        fetch_pieces<PS, kTok>(p.ep + at * kWF, lane, kChunk, tb, x);
 #pragma unroll
         for (int j = 0; j < kTok; ++j) x[j] *= u[j];
         const float s = sum_columns(x);

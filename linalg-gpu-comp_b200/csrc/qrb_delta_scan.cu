@@ -21,10 +21,10 @@ namespace {
 
 template <int DKP, typename T, int PS, bool STORE>
 struct ScanLayout {
-  static constexpr int PO = STORE ? PS : OutPieces<T>::k;   // pieces of S0, P and u in o
+  static constexpr int PX = kChainPieces;
   static constexpr int P = Pieces<T>::kIn;
   static constexpr int kK = tile_bytes(kChunk, P, DKP);
-  static constexpr int kX = tile_bytes(kChunk, PS, kChunk), kP = tile_bytes(kChunk, PO, kChunk);
+  static constexpr int kX = tile_bytes(kChunk, PX, kChunk), kP = tile_bytes(kChunk, PS, kChunk);
   static constexpr int kV = kChunk * kLanes * (int)sizeof(T);
   static constexpr int kGates = 3 * kChunk * 4;
   static constexpr int kOffQ = kK, kOffX = 2 * kK, kOffP = kOffX + kX, kOffV = kOffP + kP, kOffD = kOffV + kV;
@@ -34,14 +34,12 @@ struct ScanLayout {
   static constexpr int kBar = kOffG + kStages * kGates;
   static constexpr int kBytes = kBar + 256 + 1024;   // 1024: alignment
   static_assert(kBytes <= kSmemLimit, "shared memory of one block");
-  // tensor memory columns: pieces of S | K^T W | K S0, then X F | Q S0, then P u | F, then W | U.
-  // Three pieces: K^T W lies over the pieces of S (read by then), rewritten behind a barrier of the
-  // warps that share lanes.
+  // tensor memory columns: pieces of S, then K^T W over them (they are read by then; the warps that share
+  // lanes meet before they are written again) | K S0, then X F | Q S0, then P u | F, then W | U
   static constexpr uint32_t kSp = PS * (DKP / 2);
-  static constexpr bool kOver = PS == 3;
-  static constexpr uint32_t tS = 0, tD = kOver ? 0 : kSp, tK = kOver ? (kSp > (uint32_t)DKP ? kSp : DKP) : kSp + DKP,
-                            tQ = tK + 64, tF = tQ + 64, tU = tF + 32 * PS;
-  static_assert(tU + 32 * PO <= 512, "tensor memory");
+  static constexpr uint32_t tS = 0, tD = 0, tK = kSp > (uint32_t)DKP ? kSp : DKP, tQ = tK + 64, tF = tQ + 64,
+                            tU = tF + 32 * PX;
+  static_assert(tU + 32 * PS <= 512, "tensor memory");
 };
 
 struct ScanBars {
@@ -55,8 +53,8 @@ static_assert(sizeof(ScanBars) <= 256, "barrier block");
 template <int DKP, typename T, int PS, bool STORE>
 __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_constant__ Params p, int* err) {
   using L = ScanLayout<DKP, T, PS, STORE>;
-  constexpr int PG = Pieces<T>::kS;   // pieces kept for dq, dk and dbeta
-  constexpr int P = L::P, PO = L::PO, HK = DKP / kParts;   // HK: state rows of one thread
+  constexpr int PG = Pieces<T>::kS;   // pieces of S0 kept for dq and dk
+  constexpr int P = L::P, PX = L::PX, HK = DKP / kParts;   // HK: state rows of one thread
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                        ~uintptr_t(1023));
@@ -124,20 +122,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
         mma_commit(&bars.ks);
         if (!mbar_wait_abort(&bars.f, ph, abort, err, 54)) break;
         tc_fence_after();
-        mma_pieces<64, 64, false, PS, PS, PS>(tmem + L::tK, tmem + L::tF, 32, sb + L::kOffX, 0);
+        mma_pieces<64, 64, false, PX, PX, PX>(tmem + L::tK, tmem + L::tF, 32, sb + L::kOffX, 0);
         mma_commit(&bars.xf);
         if (c > 0 && !mbar_wait_abort(&bars.o, ph ^ 1, abort, err, 55)) break;   // the last chunk's o is read
         tc_fence_after();
-        mma_pieces<64, DKP, false, PO, P, PO>(tmem + L::tQ, tmem + L::tS, DKP / 2, sb + L::kOffQ, 0);
+        mma_pieces<64, DKP, false, PS, P, PS>(tmem + L::tQ, tmem + L::tS, DKP / 2, sb + L::kOffQ, 0);
         mma_commit(&bars.qs);
         if (!mbar_wait_abort(&bars.uw, ph, abort, err, 56)) break;
-        if (L::kOver && !mbar_wait_abort(&bars.qs, ph, abort, err, 57)) break;   // pieces of S read
+        if (!mbar_wait_abort(&bars.qs, ph, abort, err, 57)) break;   // the pieces of S are read
         tc_fence_after();
-        mma_pieces<DKP, 64, true, PS, P, PS>(tmem + L::tD, tmem + L::tF, 32, sb, 0);
+        mma_pieces<DKP, 64, true, PX, P, PX>(tmem + L::tD, tmem + L::tF, 32, sb, 0);
         mma_commit(&bars.ds);
         if (!mbar_wait_abort(&bars.sq, ph, abort, err, 58)) break;
         tc_fence_after();
-        mma_pieces<64, 64, false, PO, PO, PO>(tmem + L::tQ, tmem + L::tU, 32, sb + L::kOffP, 1);
+        mma_pieces<64, 64, false, PS, PS, PS>(tmem + L::tQ, tmem + L::tU, 32, sb + L::kOffP, 1);
         mma_commit(&bars.pu);
       }
       if (*abort) {   // MMAs in flight must end before tensor memory goes
@@ -186,7 +184,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
       ld_cols(tl + L::tK + tb, x);
       with_tokens(gates.gam, [&](int i, float g) { e[i] -= g * x[i]; });
       with_tokens(gates.bet, [&](int i, float g) { x[i] = g * e[i]; });
-      put_pieces<PS, 0>(tl + L::tF + tb / 2, 32, x);
+      put_pieces<PX, 0>(tl + L::tF + tb / 2, 32, x);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&bars.f);
@@ -199,14 +197,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
       {
         float y[kTok];
         with_tokens(gates.tail, [&](int i, float g) { y[i] = g * e[i]; });
-        put_pieces<PO, 0>(tl + L::tU + tb / 2, 32, e);
-        put_pieces<PS, 0>(tl + L::tF + tb / 2, 32, y);
+        put_pieces<PS, 0>(tl + L::tU + tb / 2, 32, e);
+        put_pieces<PX, 0>(tl + L::tF + tb / 2, 32, y);
       }
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&bars.uw);
       if (STORE)
-        put_pieces<PG, PG>(kNoTmem, 0, x, p.ep + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWF, lane, kChunk, tb);
+        put_pieces<PS, PS>(kNoTmem, 0, x, p.ep + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWF, lane, kChunk, tb);
       if (!warp_wait(&bars.qs, ph, abort, err, 63)) break;
       tc_fence_after();
       ld_cols(tl + L::tQ + tb, x);   // scale gamma Q S0 goes back, P u is added to it there
@@ -228,12 +226,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
         for (int i = 0; i < HK; ++i) st[i] = glast * st[i] + y[i];
       }
       if (c + 1 < nc) {
-        if (L::kOver) {   // the other quarters' columns of K^T W are read too
-          tc_fence_before();
-          warp_arrive(&bars.share[q]);
-          if (!warp_wait(&bars.share[q], ph, abort, err, 66)) break;
-          tc_fence_after();
-        }
+        tc_fence_before();
+        warp_arrive(&bars.share[q]);   // the other quarters' columns of K^T W are read too
+        if (!warp_wait(&bars.share[q], ph, abort, err, 66)) break;
+        tc_fence_after();
         put_state(c + 1);
       }
       if (!warp_wait(&bars.pu, ph, abort, err, 67)) break;

@@ -17,9 +17,9 @@
 //   * Few tiles: the blocks divide k; fp32 partials are added in order by reduce_kernel, which
 //     then runs the epilogue, so results repeat.
 //   * fp32: three bf16 planes per operand, x = x0 + x1 + x2 to 2^-27; the six products x_i w_j with
-//     i + j < 3.  The five small ones have an accumulator of their own, and k is cut at 4096 (fp32
+//     i + j < 3.  The five small ones have an accumulator of their own, and k is cut at 512 (fp32
 //     partials beyond): the tensor cores' accumulation truncates, and its bias grows with the
-//     number of additions to the large sum.
+//     number of additions to the large sum (k = 1432 in one piece was 1.5e-6 off).
 //
 // Every wait is bounded (mbar_wait_abort); see qrb_wide.cu.  No TMA load uses cluster multicast.
 #include "qrb_gemm.cuh"
@@ -40,7 +40,7 @@ using namespace sm100;
 
 constexpr int kBM = 128, kBK = 64, kThreads = 384;   // warps: producer, MMA, 2 idle, 8 epilogue
 constexpr int kMaxTerms = 6;
-constexpr int64_t kMaxSplitK32 = 4096;   // longest k of one fp32 accumulation
+constexpr int64_t kMaxSplitK32 = 512;    // longest k of one fp32 accumulation
 
 struct GemmArgs {
   int64_t M, N;                 // MMA orientation: A's rows, B's rows
