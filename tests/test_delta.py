@@ -389,6 +389,115 @@ def test_streams_and_graphs():
 
 
 @gpu
+def test_two_streams_at_once():
+    """Calls that overlap on the device do not meet: each has its own workspace, and blocks that want the
+    same tensor memory wait for it."""
+    calls = [make(1, 700, 2, 8, 128, 128, BF, seed=i) for i in range(4)]
+    want = [(*api().gated_delta_rule(*x), *api().gated_delta_rule_backward(x[2], *x)[:5]) for x in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for s, x in zip(streams, calls):
+            with torch.cuda.stream(s):
+                got.append((*api().gated_delta_rule(*x), *api().gated_delta_rule_backward(x[2], *x)[:5]))
+    torch.cuda.synchronize()
+    for i, res in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(res, want[i % 4])), i
+    from qr_b200 import _lib
+    assert _lib.lib().qrb_device_error() == 0
+
+
+FIRST_CALL = """
+import sys
+sys.path.insert(0, {pkg!r})
+import torch, qr_b200
+r = lambda *s: torch.randn(*s, device="cuda")
+q, k, v = (r(1, 100, 2, 64).bfloat16() for _ in range(3))
+g, b = -r(1, 100, 2).abs(), r(1, 100, 2).sigmoid()
+state, x, w = r(2, 2, 64, 64), r(200, 72).bfloat16(), r(96, 72).bfloat16()
+dy = r(200, 96).bfloat16()
+k = torch.nn.functional.normalize(k.float(), dim=-1).bfloat16()
+torch.cuda.synchronize()
+def run():
+    return [*qr_b200.gated_delta_rule(q, k, v, g, b), *qr_b200.gated_delta_rule_backward(v, q, k, v, g, b)[:5],
+            qr_b200.gated_delta_step(q[0, :2], k[0, :2], v[0, :2], g[0, :2], b[0, :2], state, state_out=state.clone()),
+            qr_b200.linear(x, w), *qr_b200.linear_backward(dy, x, w)[:2], qr_b200.linear(x[:1], w)]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = run()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, c) for a, c in zip(out, run()))
+print("same")
+"""
+
+
+@gpu
+def test_first_call_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+
+    from conftest import PKG
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL.format(pkg=str(PKG))], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+@gpu
+def test_final_state_over_initial_state():
+    x = make(2, 90, 1, 2, 64, 96, BF)
+    init = states(2, 2, 64, 96)
+    want = api().gated_delta_rule(*x, initial_state=init)
+    o = torch.empty_like(x[2])
+    api().gated_delta_rule(*x, initial_state=init, out=(o, init))
+    assert torch.equal(o, want[0]) and torch.equal(init, want[1])
+
+
+@gpu
+def test_far_strides():
+    """Batch strides past 2^31 elements."""
+    far = 2 ** 31 + 64
+    x = make(2, 70, 1, 1, 64, 64, BF)
+    want = api().gated_delta_rule(*x)
+    wb = api().gated_delta_rule_backward(x[2], *x)
+    big = torch.empty(far + 70 * 192 + 64, dtype=BF, device="cuda")
+    views = []
+    for i in range(3):
+        v = big.as_strided((2, 70, 1, 64), (far, 192, 64, 1), 64 * i)
+        v.copy_(x[i])
+        views.append(v)
+    got = api().gated_delta_rule(*views, *x[3:])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert all(torch.equal(a, b) for a, b in zip(api().gated_delta_rule_backward(views[2], *views, *x[3:])[:5], wb[:5]))
+
+
+@gpu
+def test_long_sequence_in_parts():
+    """100,001 tokens in one call and in two with the state carried over: chunks lie differently, so values
+    agree to the kernels' accuracy, not bit for bit."""
+    x = make(1, 100001, 1, 1, 64, 64, BF)
+    o, s = api().gated_delta_rule(*x)
+    cut = 33333
+    o1, s1 = api().gated_delta_rule(*[t[:, :cut] for t in x])
+    o2, s2 = api().gated_delta_rule(*[t[:, cut:] for t in x], initial_state=s1)
+    assert rel(torch.cat([o1, o2], 1), o) <= 2 * tol(BF, STATE_TOL[BF]) and rel(s2, s) <= 2 * STATE_TOL[BF]
+
+
+@gpu
+def test_many_short_sequences():
+    n = 3000
+    lens = [(i * 7) % 4 for i in range(n)]
+    offs = [0]
+    for m in lens:
+        offs.append(offs[-1] + m)
+    x = make(1, offs[-1], 1, 1, 16, 16, F32)
+    o, s = api().gated_delta_rule(*x, seq_offsets=torch.tensor(offs, device="cuda"))
+    for i in (0, 1, 2, 3, 1500, 2998, 2999):
+        ro, rs, _ = D.forward(*[t[0, offs[i]:offs[i + 1]] for t in x], 0.25, torch.zeros(1, 16, 16, device="cuda"))
+        assert rel(o[0, offs[i]:offs[i + 1]], ro) <= STATE_TOL[F32] and rel(s[i], rs) <= STATE_TOL[F32]
+
+
+@gpu
 def test_gradients_are_refused_under_capture():
     x = [t.requires_grad_() for t in make(1, 10, 1, 1, 64, 64, BF)]
     gr = torch.cuda.CUDAGraph()

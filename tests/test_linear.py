@@ -9,7 +9,7 @@ Tolerances, relative 2-norms of a whole output, derived:
     k <= 4096 to the large sum before fp32 addition takes over: 256 * 2^-23 = 2^-15; activations at
     most double a relative error (their slope stays below 1.13, cancellation against the residual
     the same);
-  * backward, 16-bit types: dp is rounded once more, another eps / 2 of each term.
+  * backward, 16-bit types: dp is rounded once more, another eps / 2 of each term (check_sum).
 """
 import math
 
@@ -52,6 +52,19 @@ def make(m, k, n, dtype, seed=0):
             r(m, n).to(dtype))
 
 
+def check_sum(got, a, b, dtype, what):
+    """got = a b, where a was rounded to the type first.  That changes each term a_ij b_jk by at most eps / 2 of
+    itself, with independent signs: the sum by (eps / 2) sqrt(sum_j a_ij^2 b_jk^2 / 3) in the mean square, and
+    twice the root without the 3 is 3.5 standard deviations for a single output; of whole outputs it is about
+    twice their norm, unless the terms cancel (one output of 300 terms may be a twentieth of its root).  fp32
+    operands are not rounded; their sums' 2^-14 takes eps / 2's place."""
+    ref = a @ b
+    term = tol(dtype, 0) if dtype == F32 else torch.finfo(dtype).eps / 2
+    off = (got.double() - ref).norm().item()
+    room = tol(dtype) * ref.norm().item() + 2 * term * (a.square() @ b.square()).sum().sqrt().item()
+    assert off <= room, (*what, off, room)
+
+
 def reference(x, w, b, act, res):
     p = torch.nn.functional.linear(x.double(), w.double(), None if b is None else b.double())
     y = ACTS[act](p)
@@ -59,7 +72,7 @@ def reference(x, w, b, act, res):
 
 
 SIZES = [(1, 1, 1), (1, 64, 128), (1, 2048, 1111), (3, 65, 257), (16, 512, 512), (64, 100, 40), (65, 130, 66),
-         (128, 8192, 64), (129, 64, 128), (130, 1001, 250), (255, 256, 256), (300, 72, 1032), (512, 352, 176),
+         (128, 8192, 64), (129, 64, 128), (130, 1001, 250), (255, 256, 256), (300, 72, 1032), (512, 352, 176), (300, 1, 1), (257, 3, 2), (140, 5, 300),
          (1000, 4100, 72), (2049, 128, 136)]
 
 
@@ -86,8 +99,8 @@ def test_backward(size, dtype):
         p = pre.double().requires_grad_()
         dp = torch.autograd.grad(ACTS[act](p), p, dy.double())[0]
         dx, dw, db = api().linear_backward(dy, x, w, activation=act, pre=pre, with_bias=True)
-        assert rel(dx, dp @ w.double()) <= tol(dtype, 2), (act, "dx")
-        assert rel(dw, dp.T @ x.double()) <= tol(dtype, 2), (act, "dw")
+        check_sum(dx, dp, w.double(), dtype, (act, "dx"))
+        check_sum(dw, dp.T, x.double(), dtype, (act, "dw"))
         # sums over m of terms of both signs: m additions of 2^-24 of their absolute sum
         room = tol(dtype) + 2.0 ** -24 * size[0] * dp.abs().sum(0).norm() / dp.sum(0).norm().clamp_min(1e-30)
         assert rel(db, dp.sum(0)) <= room, (act, "dbias")
@@ -204,6 +217,21 @@ def test_streams_and_graphs():
             assert all(torch.equal(a, c) for a, c in zip(r, want))
     from qr_b200 import _lib
     assert _lib.lib().qrb_device_error() == 0
+
+
+@gpu
+def test_far_strides():
+    """Rows past 2^31 elements."""
+    m, k, n = 200, 64, 96
+    x, w, b, res, dy = make(m, k, n, BF)
+    ld = 2 ** 31 // (m - 8) // 8 * 8
+    big = torch.empty(ld * m, dtype=BF, device="cuda")
+    xv = big.as_strided((m, k), (ld, 1))
+    xv.copy_(x)
+    out = big.as_strided((m, n), (ld, 1), 512)
+    assert torch.equal(api().linear(xv, w, b, out=out), api().linear(x, w, b))
+    assert all(torch.equal(p, q) for p, q in zip(api().linear_backward(dy, xv, w)[:2], api().linear_backward(dy, x, w)[:2]))
+    assert torch.equal(api().linear(xv[-3:], w), api().linear(x[-3:], w))
 
 
 @gpu
