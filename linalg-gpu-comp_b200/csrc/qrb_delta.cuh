@@ -66,6 +66,13 @@ struct Params {
   const int32_t* offsets;          // packed layout: nseq + 1 token offsets
   int32_t* cstart;                 // packed layout: first chunk slot of each sequence
   int32_t* order;                  // packed layout: the sequences, longest first
+  // Long sequences on few heads: segments of `seg` chunks run side by side (0: whole sequences; see
+  // qrb_delta_join.cu).  segstart: packed layout, first segment of each sequence; nsegs: an upper bound.
+  int seg, nsegs;
+  int32_t* segstart;
+  // [segment][hv]: S before it (dkp x nb*128), its transition (dkp x dkp), dS before it (for a first
+  // segment: dS behind the sequence, which like S before it is copied since the caller's may be written over)
+  float *seg_s, *seg_a, *seg_ds;
   float scale;
   const void *q, *k, *v, *d_o;
   const float *g, *beta;
@@ -357,13 +364,63 @@ __device__ __forceinline__ Chunk chunk_at(const Params& p, int c) {
   return r;
 }
 
+// The stretch of a sequence that a block of the recurrences walks: all of it, or one segment.
+struct Span {
+  int seq, g, g0, slot0, nc;   // g: segment; g0: the sequence's first; slot0, nc: chunks (nc < 0: no such segment)
+  int64_t b, t0, n;
+  bool first, last;
+};
+
+template <bool CUT = true>
+__device__ __forceinline__ Span span_at(const Params& p, int turn) {
+  Span s;
+  int j = 0, ns = 1, total;
+  s.g = turn;
+  if (!CUT || p.seg == 0) {
+    s.seq = p.offsets != nullptr ? p.order[turn] : turn;   // the longest sequences start first
+  } else if (p.offsets == nullptr) {
+    ns = max(1, (p.nchunk + p.seg - 1) / p.seg);
+    s.seq = turn / ns;
+    j = turn - s.seq * ns;
+  } else {
+    if (turn >= p.segstart[p.nseq]) {
+      s.nc = -1;
+      return s;
+    }
+    int lo = 0, hi = p.nseq;   // the last sequence whose first segment is not behind turn
+    while (hi - lo > 1) {
+      const int m = (lo + hi) >> 1;
+      if (p.segstart[m] <= turn) lo = m;
+      else hi = m;
+    }
+    s.seq = lo;
+    j = turn - p.segstart[lo];
+    ns = p.segstart[lo + 1] - p.segstart[lo];
+  }
+  seq_range(p, s.seq, s.b, s.t0, s.n);
+  seq_slots(p, s.seq, s.slot0, total);
+  s.first = j == 0;
+  s.last = j == ns - 1;
+  s.g0 = turn - j;
+  s.nc = total;
+  if (CUT && p.seg > 0) {
+    const int c0 = j * p.seg;
+    s.slot0 += c0;
+    s.t0 += (int64_t)c0 * kChunk;
+    s.nc = min(p.seg, total - c0);
+    s.n = min(s.n - (int64_t)c0 * kChunk, (int64_t)s.nc * kChunk);
+  }
+  return s;
+}
+
 __device__ __forceinline__ size_t slot_head(const Params& p, int c, int h) { return (size_t)c * p.hv + h; }
 
 // ---- launchers ----
 cudaError_t launch_plan(const Params& p, cudaStream_t s);
 cudaError_t launch_prep(const Params& p, int dtype, cudaStream_t s);
-cudaError_t launch_scan(const Params& p, int dtype, cudaStream_t s);
-cudaError_t launch_rscan(const Params& p, int dtype, cudaStream_t s);
+cudaError_t launch_scan(const Params& p, int dtype, bool state_only, cudaStream_t s);
+cudaError_t launch_rscan(const Params& p, int dtype, bool state_only, cudaStream_t s);
+cudaError_t launch_join(const Params& p, bool backward, cudaStream_t s);
 cudaError_t launch_grad(const Params& p, int dtype, cudaStream_t s);
 cudaError_t launch_step(const qrb_delta_step_args& a, cudaStream_t s);
 

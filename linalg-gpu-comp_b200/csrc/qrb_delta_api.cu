@@ -2,6 +2,7 @@
 // the launch sequence.
 //   forward:  [plan] prep, scan
 //   backward: [plan] prep, scan (keeping every chunk's state and e), rscan, grad
+// with a state-only pass and a join before scan and rscan where long sequences are cut into segments.
 // Backward repeats the forward recurrence instead of asking the caller to keep 4 dk dv bytes per
 // 64 tokens and head between the passes.
 #include <cstdarg>
@@ -84,8 +85,45 @@ int check_args(const qrb_delta_args* a) {
   return QRB_OK;
 }
 
+// Segments of `seg` chunks (0: whole sequences) and how many there may be at most.  With one chunk of the
+// full recurrence as the unit (5.5 us at dk = dv = 128 in bf16), one of the state-only pass takes about
+// as much (0.6 in fp32), a join's step 1/4 and the two launches 3.5: a sequence of nc chunks costs
+// 2 seg + ns / 4 + 3.5 in ns segments, which is least at seg = sqrt(nc / 8) where there are SMs for so
+// many.  One sequence, 16 heads of 128 x 128, bf16: 512 tokens 57 us whole, 65 in four; 1024 tokens 99
+// and 79; 4096 tokens 373 and 234; backward, whose chunks take longer, 512 tokens 171 us whole, 135 in
+// four, 4096 tokens 1320 and 723.  The state-only pass has one more block per head, for the transition.
+// Packed lengths are not known on the host: segments are cut as if one sequence held most of the tokens,
+// which costs little where it does not (a sequence of one segment has no first pass), unless the
+// sequences alone nearly fill the card.  7 packed sequences, 6 heads of 64 x 64, 3001 tokens, backward:
+// 605 us whole, 218 cut.
+struct Segments {
+  int seg, nsegs;
+};
+Segments segments(const qrb_delta_args& a, bool backward) {
+  const int64_t nb = (a.dv + 127) / 128;
+  const int64_t room = qrb::sm_count() / (a.hv * (nb + 1));   // segments with an SM for each of their blocks
+  const bool packed = a.seq_offsets != nullptr;
+  Segments s{0, 0};
+  if (a.nseq < 1 || (packed ? 2 * room < 3 * a.nseq : room < 2 * a.nseq)) return s;
+  const int64_t nc = packed ? chunk_slots(a) : (a.time + kChunk - 1) / kChunk, each = packed ? room : room / a.nseq;
+  if (nc < (packed ? 16 : 6)) return s;
+  int64_t seg = (nc + each - 1) / each;
+  while (8 * seg * seg < nc) ++seg;
+  if (packed) {
+    if (seg < 3) seg = 3;
+    s.nsegs = (int)(nc / seg + a.nseq);
+  } else {
+    const int64_t ns = (nc + seg - 1) / seg;
+    if (8 * seg + ns + (backward ? 6 : 14) > 4 * nc) return s;
+    s.nsegs = (int)(ns * a.nseq);
+  }
+  s.seg = (int)seg;
+  return s;
+}
+
 struct Layout {
   size_t cstart, kt, qt, xt, pt, gates, gsum, s0p, dsp, ep, dup, odo, vdv, edu, sds, s_last, vt, dot, total;
+  size_t seg_s, seg_a, seg_ds;
 };
 
 Layout layout(const qrb_delta_args& a, bool backward) {
@@ -99,7 +137,7 @@ Layout layout(const qrb_delta_args& a, bool backward) {
     at += al(bytes);
     return o;
   };
-  l.cstart = take(a.seq_offsets != nullptr ? (2 * a.nseq + 1) * 4 : 0);
+  l.cstart = take(a.seq_offsets != nullptr ? (3 * a.nseq + 2) * 4 : 0);
   l.kt = take(n * a.hk * tile_bytes(kChunk, pi, dkp));
   l.qt = take(n * a.hk * tile_bytes(kChunk, pi, dkp));
   l.xt = take(n * a.hv * tile_bytes(kChunk, kChainPieces, kChunk));
@@ -107,6 +145,11 @@ Layout layout(const qrb_delta_args& a, bool backward) {
   l.gates = take(n * a.hv * 3 * kChunk * 4);
   const size_t staged = n * a.hv * ((a.dv + 127) / 128) * kChunk * 128 * (a.dtype == QRB_F32 ? 4 : 2);
   l.vt = take(staged);
+  const Segments g = segments(a, backward);
+  const size_t cells = (size_t)g.nsegs * a.hv * dkp * 4;   // of one column of every border
+  l.seg_s = take(cells * ((a.dv + 127) / 128) * 128);
+  l.seg_a = take(cells * dkp);
+  if (backward) l.seg_ds = take(cells * ((a.dv + 127) / 128) * 128);
   if (backward) {
     l.dot = take(staged);
     l.gsum = take(n * a.hv * kChunk * 8);
@@ -188,6 +231,13 @@ int run(const qrb_delta_args* a, void* ws, size_t wsb, void* stream, bool backwa
   p.offsets = a->seq_offsets;
   p.cstart = reinterpret_cast<int32_t*>(w + l.cstart);
   p.order = p.cstart + a->nseq + 1;
+  p.segstart = p.order + a->nseq;
+  const Segments g = segments(*a, backward);
+  p.seg = g.seg;
+  p.nsegs = g.nsegs;
+  p.seg_s = reinterpret_cast<float*>(w + l.seg_s);
+  p.seg_a = reinterpret_cast<float*>(w + l.seg_a);
+  p.seg_ds = reinterpret_cast<float*>(w + l.seg_ds);
   p.scale = a->scale;
   p.q = a->q;
   p.k = a->k;
@@ -234,9 +284,17 @@ int run(const qrb_delta_args* a, void* ws, size_t wsb, void* stream, bool backwa
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p.offsets != nullptr) CUDA(qrb::delta::launch_plan(p, s), "delta plan launch");
   if (p.bound > 0) CUDA(qrb::delta::launch_prep(p, a->dtype, s), "delta chunk factor launch");
-  CUDA(qrb::delta::launch_scan(p, a->dtype, s), "delta recurrence launch");
+  if (p.seg > 0) {
+    CUDA(qrb::delta::launch_scan(p, a->dtype, true, s), "delta segment launch");
+    CUDA(qrb::delta::launch_join(p, false, s), "delta join launch");
+  }
+  CUDA(qrb::delta::launch_scan(p, a->dtype, false, s), "delta recurrence launch");
   if (backward) {
-    CUDA(qrb::delta::launch_rscan(p, a->dtype, s), "delta backward recurrence launch");
+    if (p.seg > 0) {
+      CUDA(qrb::delta::launch_rscan(p, a->dtype, true, s), "delta backward segment launch");
+      CUDA(qrb::delta::launch_join(p, true, s), "delta backward join launch");
+    }
+    CUDA(qrb::delta::launch_rscan(p, a->dtype, false, s), "delta backward recurrence launch");
     if (p.bound > 0) CUDA(qrb::delta::launch_grad(p, a->dtype, s), "delta gradient launch");
   }
   return QRB_OK;

@@ -16,39 +16,48 @@ namespace qrb {
 namespace delta {
 namespace {
 
-__global__ void __launch_bounds__(1024) plan_kernel(Params p) {
-  __shared__ int part[1024];
-  const int tid = threadIdx.x;
-  const int per = (p.nseq + 1023) / 1024;
+// to[s] = sum of count(0 .. s - 1), never above `most`; to[nseq] the whole sum.  One block of 1024.
+template <typename F>
+__device__ void prefix(int nseq, int64_t most, int32_t* to, int* part, F count) {
+  const int tid = threadIdx.x, per = (nseq + 1023) / 1024;
   int64_t sum = 0;
-  for (int i = 0; i < per; ++i) {
-    const int s = tid * per + i;
-    if (s < p.nseq) {
-      int64_t b, t0, n;
-      seq_range(p, s, b, t0, n);
-      sum += (n + kChunk - 1) / kChunk;
-    }
-  }
-  part[tid] = (int)(sum < p.bound ? sum : p.bound);
+  for (int i = 0; i < per; ++i)
+    if (tid * per + i < nseq) sum += count(tid * per + i);
+  part[tid] = (int)min(sum, most);
   __syncthreads();
   for (int o = 1; o < 1024; o <<= 1) {
     int64_t v = part[tid];
     if (tid >= o) v += part[tid - o];
     __syncthreads();
-    part[tid] = (int)(v < p.bound ? v : p.bound);
+    part[tid] = (int)min(v, most);
     __syncthreads();
   }
   int64_t at = tid == 0 ? 0 : part[tid - 1];
   for (int i = 0; i < per; ++i) {
     const int s = tid * per + i;
-    if (s < p.nseq) {
-      p.cstart[s] = (int)at;
-      int64_t b, t0, n;
-      seq_range(p, s, b, t0, n);
-      at += (n + kChunk - 1) / kChunk;
-      if (at > p.bound) at = p.bound;
-      if (s == p.nseq - 1) p.cstart[p.nseq] = (int)at;
-    }
+    if (s >= nseq) break;
+    to[s] = (int)at;
+    at = min(at + count(s), most);
+    if (s == nseq - 1) to[nseq] = (int)at;
+  }
+  __syncthreads();
+}
+
+__global__ void __launch_bounds__(1024) plan_kernel(Params p) {
+  __shared__ int part[1024];
+  const int tid = threadIdx.x;
+  auto chunks = [&](int s) {
+    int64_t b, t0, n;
+    seq_range(p, s, b, t0, n);
+    return (n + kChunk - 1) / kChunk;
+  };
+  prefix(p.nseq, p.bound, p.cstart, part, chunks);
+  if (p.seg > 0) {
+    // of the chunks that have a slot, in case wrong offsets gave more
+    prefix(p.nseq, p.nsegs, p.segstart, part, [&](int s) {
+      return (int64_t)max(1, (p.cstart[s + 1] - p.cstart[s] + p.seg - 1) / p.seg);
+    });
+    return;
   }
   // Longest first, so that no long sequence is left to run alone at the end (24 packed prompts on 148
   // SMs: 58 chunks on the busiest instead of 82); calls of more sequences than threads level out anyway.
@@ -56,13 +65,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(Params p) {
     for (int s = tid; s < p.nseq; s += 1024) p.order[s] = s;
     return;
   }
-  __syncthreads();
   int mine = 0;
-  if (tid < p.nseq) {
-    int64_t b, t0, n;
-    seq_range(p, tid, b, t0, n);
-    mine = part[tid] = (int)((n + kChunk - 1) / kChunk);
-  }
+  if (tid < p.nseq) mine = part[tid] = (int)chunks(tid);
   __syncthreads();
   if (tid < p.nseq) {
     int rank = 0;

@@ -41,10 +41,13 @@ struct RBars {
   uint64_t full[2], sp, dop, ks, pd, f, xf, uw, ds, done, share[4], drain;
   uint32_t tmem;
   int abort;
+  Span span;   // here, not in registers that the loops need
 };
 static_assert(sizeof(RBars) <= 256, "barrier block");
 
-template <int DKP, typename T>
+// STATE: only the gradient of the state, of every segment but a sequence's first: from the final state's
+// gradient for the last, else from zero.
+template <int DKP, typename T, bool STATE>
 __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_constant__ Params p, int* err) {
   using L = RLayout<DKP, T>;
   constexpr int P = L::P, PS = L::PS, PG = L::PG, HK = DKP / kParts;
@@ -55,14 +58,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
   volatile int* abort = &bars.abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nb = (p.dv + kLanes - 1) / kLanes;
-  const int vb = blockIdx.x % nb, sh = blockIdx.x / nb, h = sh % p.hv, turn = sh / p.hv;
-  const int seq = p.offsets != nullptr ? p.order[turn] : turn;   // the longest sequences start first
-  const int hk = h / p.group;
+  const int vb = blockIdx.x % nb, sh = blockIdx.x / nb, h = sh % p.hv;
+  const Span mine = span_at(p, sh / p.hv);
+  if (mine.nc < 0 || (STATE && mine.first)) return;
+  const int hk = h / p.group, nc = mine.nc, slot0 = mine.slot0;
   const int quarters = min(4, (p.dv - vb * kLanes + 31) / 32);
-  int64_t b, t0, n;
-  seq_range(p, seq, b, t0, n);
-  int slot0, nc;
-  seq_slots(p, seq, slot0, nc);
 
   if (tid == 0) {
     mbar_init(&bars.full[0], 1);
@@ -71,6 +71,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
     for (uint64_t* x : {&bars.sp, &bars.dop, &bars.f, &bars.uw, &bars.done}) mbar_init(x, kParts * quarters);
     for (int i = 0; i < 4; ++i) mbar_init(&bars.share[i], kParts);
     bars.abort = 0;
+    bars.span = mine;
     fence_mbar_init();
   }
   if (warp == kIssuer) tmem_alloc(&bars.tmem, 512);
@@ -132,137 +133,149 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
       }
     }
   } else {
+    const Span& span = bars.span;
     const int q = warp & 3, part = warp >> 2;
     if (q < quarters) {
-    const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
-    const int lcol = 32 * q + lane, col = vb * kLanes + lcol;
-    const int tile = vb * 4 + q;
-    const int tb = kTok * part, kb = HK * part;
-    const bool on = col < p.dv;
-    const size_t sbase = ((size_t)seq * p.hv + h) * p.dk * p.dv;
-    const size_t scol = sbase + (size_t)kb * p.dv + min(col, p.dv - 1);
-    constexpr int kWS = tile_bytes(kTile, PS, DKP), kWF = tile_bytes(kTile, PS, kChunk);
-    float st[HK];
-    if (p.ds_end != nullptr)
-      load_column(p.ds_end + scol, p.dv, p.dk - kb, on, st);
-    else
+      const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
+      const int lcol = 32 * q + lane, col = vb * kLanes + lcol;
+      const int tile = vb * 4 + q;
+      const int tb = kTok * part, kb = HK * part;
+      const bool on = col < p.dv;
+      auto sbase = [&] { return (((size_t)span.seq * p.hv + h) * p.dk + kb) * p.dv; };
+      const int pitch = nb * kLanes;   // at the borders of segments, as in scan
+      auto border = [&](float* x, int g) { return x + (((size_t)g * p.hv + h) * DKP + kb) * pitch + col; };
+      constexpr int kWS = tile_bytes(kTile, PS, DKP), kWF = tile_bytes(kTile, PS, kChunk);
+      float st[HK];
+      if (!STATE && !(span.first && span.last)) {
+        load_column(border(p.seg_ds, span.last ? span.g0 : span.g + 1), pitch, HK, true, st);
+      } else if (span.last && p.ds_end != nullptr) {
+        load_column(p.ds_end + sbase() + min(col, p.dv - 1), p.dv, p.dk - kb, on, st);
+      } else {
 #pragma unroll
-      for (int j = 0; j < HK; ++j) st[j] = 0.f;
-    // pieces of dS' for the products, the first PG of them for the gradient kernel too
-    auto put_state = [&](int c) {
-      float y[HK];
+        for (int j = 0; j < HK; ++j) st[j] = 0.f;
+      }
+      if (STATE && span.last) store_column(border(p.seg_ds, span.g0), pitch, HK, st);
+      // pieces of dS' for the products, the first PG of them for the gradient kernel too
+      auto put_state = [&](int c) {
+        float y[HK];
 #pragma unroll
-      for (int i = 0; i < HK; ++i) y[i] = st[i];
-      put_pieces<PS, PG>(tl + L::tS + kb / 2, DKP / 2, y, p.dsp + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWS, lane,
-                         DKP, kb);
-      tmem_st_wait();
-      tc_fence_before();
-      warp_arrive(&bars.sp);
-    };
-    float sds = 0.f;
-    if (nc > 0) put_state(nc - 1);
-    for (int i = 0; i < nc; ++i) {
-      const uint32_t ph = i & 1;
-      const int c = nc - 1 - i;
-      const size_t at = slot_head(p, slot0 + c, h) * p.nv + tile;
-      const unsigned char* stage = sm + (i % L::kStages) * L::kStage;
-      const Gates gates(sm + L::kOffG + (i % L::kStages) * L::kGates, tb);
-      float x[kTok], u[kTok];
-      if (!warp_wait(&bars.full[i % L::kStages], (i / L::kStages) & 1, abort, err, 81)) break;
-      staged<T>(stage + L::kOffD, tb, lcol, x);
-      with_tokens(gates.gam, [&](int j, float g) { u[j] = x[j] * (p.scale * g); });
-      put_pieces<P, 0>(tl + L::tF + tb / 2, 32, x);
-      put_pieces<PS, 0>(tl + L::tO + tb / 2, 32, u);
-      tmem_st_wait();
-      tc_fence_before();
-      warp_arrive(&bars.dop);
-      {
-        // This warp's share of <S', dS'>: behind the last chunk from the final state, at every kAnchor-th
-        // chunk before it from the next chunk's first state, and between from the next chunk's share, as
-        // <S0, dS0> = <S', dS'> + sum (o.do - v.dV) over a chunk's tokens.
-        if (i % kAnchor == 0) {
-          float y[HK];
-          if (i > 0)
-            fetch_pieces<PS, HK>(p.s0p + (slot_head(p, slot0 + c + 1, h) * p.nv + tile) * kWS, lane, DKP, kb, y);
-          else
-            load_column(p.s_last + scol, p.dv, p.dk - kb, on, y);
-          sds = 0.f;
+        for (int i = 0; i < HK; ++i) y[i] = st[i];
+        unsigned char* to = p.dsp + (slot_head(p, slot0 + c, h) * p.nv + tile) * kWS;
+        put_pieces<PS, STATE ? 0 : PG>(tl + L::tS + kb / 2, DKP / 2, y, to, lane, DKP, kb);
+        tmem_st_wait();
+        tc_fence_before();
+        warp_arrive(&bars.sp);
+      };
+      float sds = 0.f;
+      if (nc > 0) put_state(nc - 1);
+      for (int i = 0; i < nc; ++i) {
+        const uint32_t ph = i & 1;
+        const int c = nc - 1 - i;
+        const size_t at = slot_head(p, slot0 + c, h) * p.nv + tile;
+        const unsigned char* stage = sm + (i % L::kStages) * L::kStage;
+        const Gates gates(sm + L::kOffG + (i % L::kStages) * L::kGates, tb);
+        float x[kTok], u[kTok];
+        if (!warp_wait(&bars.full[i % L::kStages], (i / L::kStages) & 1, abort, err, 81)) break;
+        staged<T>(stage + L::kOffD, tb, lcol, x);
+        with_tokens(gates.gam, [&](int j, float g) { u[j] = x[j] * (p.scale * g); });
+        put_pieces<P, 0>(tl + L::tF + tb / 2, 32, x);
+        put_pieces<PS, 0>(tl + L::tO + tb / 2, 32, u);
+        tmem_st_wait();
+        tc_fence_before();
+        warp_arrive(&bars.dop);
+        if (!STATE) {
+          // This warp's share of <S', dS'>: behind the last chunk from the state there, at every kAnchor-th
+          // chunk before it from the next chunk's first state, and between from the next chunk's share, as
+          // <S0, dS0> = <S', dS'> + sum (o.do - v.dV) over a chunk's tokens.
+          if (i % kAnchor == 0) {
+            float y[HK];
+            if (i > 0)
+              fetch_pieces<PS, HK>(p.s0p + (slot_head(p, slot0 + c + 1, h) * p.nv + tile) * kWS, lane, DKP, kb, y);
+            else if (!span.last)
+              load_column(border(p.seg_s, span.g + 1), pitch, HK, true, y);
+            else
+              load_column(p.s_last + sbase() + min(col, p.dv - 1), p.dv, p.dk - kb, on, y);
+            sds = 0.f;
 #pragma unroll
-          for (int a = 0; a < HK; ++a) sds += y[a] * st[a];
-          sds = warp_sum(sds);
+            for (int a = 0; a < HK; ++a) sds += y[a] * st[a];
+            sds = warp_sum(sds);
+          }
+          if (lane == 0) p.sds[at * kParts + part] = sds;
         }
-        if (lane == 0) p.sds[at * kParts + part] = sds;
-      }
-      if (!warp_wait(&bars.ks, ph, abort, err, 82)) break;
-      tc_fence_after();
-      ld_cols(tl + L::tK + tb, u);
-      with_tokens(gates.tail, [&](int j, float g) { u[j] *= g; });
-      if (!warp_wait(&bars.pd, ph, abort, err, 83)) break;
-      tc_fence_after();
-      ld_cols(tl + L::tP + tb, x);
-#pragma unroll
-      for (int j = 0; j < kTok; ++j) u[j] += x[j];
-      with_tokens(gates.bet, [&](int j, float g) { x[j] = g * u[j]; });
-      put_pieces<PS, 0>(tl + L::tF + tb / 2, 32, x);
-      tmem_st_wait();
-      tc_fence_before();
-      warp_arrive(&bars.f);
-      if (!warp_wait(&bars.xf, ph, abort, err, 84)) break;
-      tc_fence_after();
-      ld_cols(tl + L::tK + tb, x);
-#pragma unroll
-      for (int j = 0; j < kTok; ++j) u[j] += x[j];
-      float y[kTok];   // dV
-      with_tokens(gates.bet, [&](int j, float g) { y[j] = g * u[j]; });
-      with_tokens(gates.gam, [&](int j, float g) { x[j] = -g * y[j]; });
-      put_pieces<PS, 0>(tl + L::tF + tb / 2, 32, x);
-      tmem_st_wait();
-      tc_fence_before();
-      warp_arrive(&bars.uw);
-      const float glast = *gates.last;
-      {
-#pragma unroll
-        for (int j = 0; j < kTok; ++j) x[j] = u[j];
-        put_pieces<PG, PG>(kNoTmem, 0, x, p.dup + at * kWF, lane, kChunk, tb);
-        fetch_pieces<PS, kTok>(p.ep + at * kWF, lane, kChunk, tb, x);
-#pragma unroll
-        for (int j = 0; j < kTok; ++j) x[j] *= u[j];
-        const float s = sum_columns(x);
-        if ((lane & 1) == 0) p.edu[at * kChunk + tb + lane / 2] = s;
-      }
-      {
-        staged<T>(stage + L::kOffV, tb, lcol, x);
-#pragma unroll
-        for (int j = 0; j < kTok; ++j) x[j] *= y[j];
-        const float s = sum_columns(x);
-        if ((lane & 1) == 0) p.vdv[at * kChunk + tb + lane / 2] = s;
-        // on to the chunk before: the tokens' sums, each in two lanes
-        sds += warp_sum((lane & 1) == 0 ? p.odo[at * kChunk + tb + lane / 2] - s : 0.f);
-        const int64_t tok = (int64_t)c * kChunk + tb;
-        if (on)
-          store_tokens(static_cast<T*>(p.dv_) + ((b * p.time + t0 + tok) * p.hv + h) * p.dv + col,
-                       (int64_t)p.hv * p.dv, (int)min(n - tok, (int64_t)kTok), y);
-      }
-      fence_proxy_async();   // what this stage held is read before bulk copies may replace it
-      if (!warp_wait(&bars.ds, ph, abort, err, 85)) break;
-      tc_fence_after();
-      {
-        float d[HK];
-        ld_cols(tl + L::tD + kb, d);
-#pragma unroll
-        for (int a = 0; a < HK; ++a) st[a] = glast * st[a] + d[a];
-      }
-      tc_fence_before();
-      warp_arrive(&bars.done);
-      if (i + 1 < nc) {
-        warp_arrive(&bars.share[q]);   // the other quarters' columns are read before pieces go over them
-        if (!warp_wait(&bars.share[q], ph, abort, err, 86)) break;
+        if (!warp_wait(&bars.ks, ph, abort, err, 82)) break;
         tc_fence_after();
-        put_state(c - 1);
+        ld_cols(tl + L::tK + tb, u);
+        with_tokens(gates.tail, [&](int j, float g) { u[j] *= g; });
+        if (!warp_wait(&bars.pd, ph, abort, err, 83)) break;
+        tc_fence_after();
+        ld_cols(tl + L::tP + tb, x);
+#pragma unroll
+        for (int j = 0; j < kTok; ++j) u[j] += x[j];
+        with_tokens(gates.bet, [&](int j, float g) { x[j] = g * u[j]; });
+        put_pieces<PS, 0>(tl + L::tF + tb / 2, 32, x);
+        tmem_st_wait();
+        tc_fence_before();
+        warp_arrive(&bars.f);
+        if (!warp_wait(&bars.xf, ph, abort, err, 84)) break;
+        tc_fence_after();
+        ld_cols(tl + L::tK + tb, x);
+#pragma unroll
+        for (int j = 0; j < kTok; ++j) u[j] += x[j];
+        float y[kTok];   // dV
+        with_tokens(gates.bet, [&](int j, float g) { y[j] = g * u[j]; });
+        with_tokens(gates.gam, [&](int j, float g) { x[j] = -g * y[j]; });
+        put_pieces<PS, 0>(tl + L::tF + tb / 2, 32, x);
+        tmem_st_wait();
+        tc_fence_before();
+        warp_arrive(&bars.uw);
+        const float glast = *gates.last;
+        if (!STATE) {
+#pragma unroll
+          for (int j = 0; j < kTok; ++j) x[j] = u[j];
+          put_pieces<PG, PG>(kNoTmem, 0, x, p.dup + at * kWF, lane, kChunk, tb);
+          fetch_pieces<PS, kTok>(p.ep + at * kWF, lane, kChunk, tb, x);
+#pragma unroll
+          for (int j = 0; j < kTok; ++j) x[j] *= u[j];
+          const float s = sum_columns(x);
+          if ((lane & 1) == 0) p.edu[at * kChunk + tb + lane / 2] = s;
+        }
+        {
+          staged<T>(stage + L::kOffV, tb, lcol, x);
+#pragma unroll
+          for (int j = 0; j < kTok; ++j) x[j] *= y[j];
+          const float s = sum_columns(x);
+          if ((lane & 1) == 0) p.vdv[at * kChunk + tb + lane / 2] = s;
+          // on to the chunk before: the tokens' sums, each in two lanes
+          sds += warp_sum((lane & 1) == 0 ? p.odo[at * kChunk + tb + lane / 2] - s : 0.f);
+          const int64_t tok = (int64_t)c * kChunk + tb;
+          if (on)
+            store_tokens(static_cast<T*>(p.dv_) + ((span.b * p.time + span.t0 + tok) * p.hv + h) * p.dv + col,
+                         (int64_t)p.hv * p.dv, (int)min(span.n - tok, (int64_t)kTok), y);
+        }
+        fence_proxy_async();   // what this stage held is read before bulk copies may replace it
+        if (!warp_wait(&bars.ds, ph, abort, err, 85)) break;
+        tc_fence_after();
+        {
+          float d[HK];
+          ld_cols(tl + L::tD + kb, d);
+#pragma unroll
+          for (int a = 0; a < HK; ++a) st[a] = glast * st[a] + d[a];
+        }
+        tc_fence_before();
+        warp_arrive(&bars.done);
+        if (i + 1 < nc) {
+          warp_arrive(&bars.share[q]);   // the other quarters' columns are read before pieces go over them
+          if (!warp_wait(&bars.share[q], ph, abort, err, 86)) break;
+          tc_fence_after();
+          put_state(c - 1);
+        }
       }
-    }
-    if (p.ds_init != nullptr && on && !*abort)
-      store_column(p.ds_init + sbase + (size_t)kb * p.dv + col, p.dv, p.dk - kb, st);
+      if (*abort) {
+      } else if (STATE) {
+        store_column(border(p.seg_ds, span.g), pitch, HK, st);
+      } else if (span.first && p.ds_init != nullptr && on) {
+        store_column(p.ds_init + sbase() + col, p.dv, p.dk - kb, st);
+      }
     }
   }
   tc_fence_before();
@@ -273,26 +286,33 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
   }
 }
 
-template <int DKP, typename T>
+template <int DKP, typename T, bool STATE>
 cudaError_t run_rscan(const Params& p, cudaStream_t s) {
   constexpr int smem = RLayout<DKP, T>::kBytes;
   const double rows = (double)p.bound * kChunk * p.hv;
   int* err = device_error_flag();
   if (err == nullptr) return cudaErrorInvalidValue;
-  LaunchTimer t("delta_rscan_kernel", s, rows * 2.0 * p.dv * sizeof(T), rows * 6.0 * p.dk * p.dv);
-  cudaError_t e = allow_smem<rscan_kernel<DKP, T>>(smem);
+  LaunchTimer t(STATE ? "delta_rscan_state_kernel" : "delta_rscan_kernel", s, rows * 2.0 * p.dv * sizeof(T),
+                rows * 6.0 * p.dk * p.dv);
+  cudaError_t e = allow_smem<rscan_kernel<DKP, T, STATE>>(smem);
   if (e != cudaSuccess) return e;
-  const unsigned grid = (unsigned)p.nseq * p.hv * ((p.dv + kLanes - 1) / kLanes);
-  rscan_kernel<DKP, T><<<grid, kTcThreads, smem, s>>>(p, err);
+  const unsigned spans = (unsigned)(p.seg > 0 ? p.nsegs : p.nseq);
+  rscan_kernel<DKP, T, STATE><<<spans * p.hv * ((p.dv + kLanes - 1) / kLanes), kTcThreads, smem, s>>>(p, err);
   return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t pick_rscan(const Params& p, bool state_only, cudaStream_t s) {
+  if (state_only) return p.dk <= 64 ? run_rscan<64, T, true>(p, s) : run_rscan<128, T, true>(p, s);
+  return p.dk <= 64 ? run_rscan<64, T, false>(p, s) : run_rscan<128, T, false>(p, s);
 }
 
 }  // namespace
 
-cudaError_t launch_rscan(const Params& p, int dtype, cudaStream_t s) {
-  if (dtype == 1) return p.dk <= 64 ? run_rscan<64, __nv_bfloat16>(p, s) : run_rscan<128, __nv_bfloat16>(p, s);
-  if (dtype == 2) return p.dk <= 64 ? run_rscan<64, __half>(p, s) : run_rscan<128, __half>(p, s);
-  return p.dk <= 64 ? run_rscan<64, float>(p, s) : run_rscan<128, float>(p, s);
+cudaError_t launch_rscan(const Params& p, int dtype, bool state_only, cudaStream_t s) {
+  if (dtype == 1) return pick_rscan<__nv_bfloat16>(p, state_only, s);
+  if (dtype == 2) return pick_rscan<__half>(p, state_only, s);
+  return pick_rscan<float>(p, state_only, s);
 }
 
 }  // namespace delta

@@ -483,6 +483,69 @@ def test_long_sequence_in_parts():
     assert rel(torch.cat([o1, o2], 1), o) <= 2 * tol(BF, STATE_TOL[BF]) and rel(s2, s) <= 2 * STATE_TOL[BF]
 
 
+# Few heads and long sequences, which run as segments side by side: two segments, many, a last one of one
+# token, several sequences, two blocks of value columns, odd sizes.
+LONG = [(1, 600, 1, 1, 64, 64), (1, 4097, 1, 2, 128, 128), (2, 1473, 1, 1, 33, 200), (3, 1025, 2, 4, 64, 31),
+        (1, 3001, 1, 1, 128, 256), (1, 9999, 2, 2, 16, 16)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("size", LONG)
+def test_long(size, dtype):
+    b, t, hk, hv, dk, dv = size
+    x = make(*size, dtype)
+    do = make(b, t, hk, hv, dk, dv, dtype, seed=5)[2]
+    init, dS = states(b, hv, dk, dv), states(b, hv, dk, dv, 2)
+    o, s = api().gated_delta_rule(*x, initial_state=init)
+    check_forward(x, init, None, o, s)
+    grads = api().gated_delta_rule_backward(do, *x, initial_state=init, dfinal_state=dS)
+    check_backward(grads, do, dS, x, init, None)
+    over = init.clone()
+    api().gated_delta_rule(*x, initial_state=over, out=(torch.empty_like(o), over))
+    assert torch.equal(over, s)
+    again = api().gated_delta_rule_backward(do, *x, initial_state=init, dfinal_state=dS)
+    assert all(torch.equal(a, c) for a, c in zip(grads, again))
+    check_forward(x, None, None, *api().gated_delta_rule(*x))
+    check_backward(api().gated_delta_rule_backward(do, *x), do, None, x, None, None)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("lens", [[0, 2500, 3, 1100, 0, 64, 700], [1, 1, 4000], [1500, 1500], [5000], [0, 0, 1216, 0]])
+def test_long_packed(lens, dtype):
+    test_packed(lens, 70, dtype)
+
+
+@gpu
+def test_long_decay_and_values_that_are_not_finite():
+    """A closed gate empties the state between segments; a NaN stays behind its chunk, in its sequence."""
+    x = make(2, 2000, 1, 1, 64, 64, BF)
+    x[3][0, 500:1500:37] = -math.inf
+    x[3][1, 700] = -1e30
+    init = states(2, 1, 64, 64)
+    o, s = api().gated_delta_rule(*x, initial_state=init)
+    check_forward([t.clamp_min(-200) if i == 3 else t for i, t in enumerate(x)], init, None, o, s)
+    x[2][0, 1300, 0, 3] = float("nan")
+    p, r = api().gated_delta_rule(*x, initial_state=init)
+    assert torch.equal(p[1], o[1]) and torch.equal(r[1], s[1]) and torch.equal(p[0, :1280], o[0, :1280])
+    assert p[0, 1300:1301, 0, 3].isnan().all()
+
+
+@gpu
+def test_wrong_offsets_of_long_sequences_stay_inside():
+    x = make(1, 2000, 1, 1, 64, 64, BF)
+    guard = torch.full((6000, 64), 5.0, dtype=BF, device="cuda")
+    o = guard[2000:4000].view(1, 2000, 1, 64)
+    for offs in ([-50, 900, 100000], [1900, 20, 1950, 3, 2000], [0, 2 ** 31 - 1], [0, 2000, 0, 2000, 0, 2000], [5000, 6000]):
+        so = torch.tensor(offs, dtype=torch.int32, device="cuda")
+        s = torch.empty(len(offs) - 1, 1, 64, 64, device="cuda")
+        api().gated_delta_rule(*x, seq_offsets=so, out=(o, s))
+        api().gated_delta_rule_backward(x[2], *x, seq_offsets=so)
+        torch.cuda.synchronize()
+        assert (guard[:2000] == 5).all() and (guard[4000:] == 5).all()
+
+
 @gpu
 def test_many_short_sequences():
     n = 3000
