@@ -420,7 +420,7 @@ cudaError_t launch_plan(const Params& p, cudaStream_t s);
 cudaError_t launch_prep(const Params& p, int dtype, cudaStream_t s);
 cudaError_t launch_scan(const Params& p, int dtype, bool state_only, cudaStream_t s);
 cudaError_t launch_rscan(const Params& p, int dtype, bool state_only, cudaStream_t s);
-cudaError_t launch_join(const Params& p, bool backward, cudaStream_t s);
+cudaError_t launch_join(const Params& p, cudaStream_t s);
 cudaError_t launch_grad(const Params& p, int dtype, cudaStream_t s);
 cudaError_t launch_step(const qrb_delta_step_args& a, cudaStream_t s);
 

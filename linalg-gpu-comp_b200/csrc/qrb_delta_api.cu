@@ -2,7 +2,7 @@
 // the launch sequence.
 //   forward:  [plan] prep, scan
 //   backward: [plan] prep, scan (keeping every chunk's state and e), rscan, grad
-// with a state-only pass and a join before scan and rscan where long sequences are cut into segments.
+// where long sequences are cut into segments: prep, [state-only scan, state-only rscan], join, scan, ...
 // Backward repeats the forward recurrence instead of asking the caller to keep 4 dk dv bytes per
 // 64 tokens and head between the passes.
 #include <cstdarg>
@@ -90,12 +90,12 @@ int check_args(const qrb_delta_args* a) {
 // as much (0.6 in fp32), a join's step 1/4 and the two launches 3.5: a sequence of nc chunks costs
 // 2 seg + ns / 4 + 3.5 in ns segments, which is least at seg = sqrt(nc / 8) where there are SMs for so
 // many.  One sequence, 16 heads of 128 x 128, bf16: 512 tokens 57 us whole, 65 in four; 1024 tokens 99
-// and 79; 4096 tokens 373 and 234; backward, whose chunks take longer, 512 tokens 171 us whole, 135 in
-// four, 4096 tokens 1320 and 723.  The state-only pass has one more block per head, for the transition.
+// and 79; 4096 tokens 373 and 234; backward, whose chunks take longer, 512 tokens 171 us whole, 122 in
+// four, 4096 tokens 1320 and 638.  The state-only pass has one more block per head, for the transition.
 // Packed lengths are not known on the host: segments are cut as if one sequence held most of the tokens,
 // which costs little where it does not (a sequence of one segment has no first pass), unless the
 // sequences alone nearly fill the card.  7 packed sequences, 6 heads of 64 x 64, 3001 tokens, backward:
-// 605 us whole, 218 cut.
+// 605 us whole, 190 cut.
 struct Segments {
   int seg, nsegs;
 };
@@ -104,17 +104,23 @@ Segments segments(const qrb_delta_args& a, bool backward) {
   const int64_t room = qrb::sm_count() / (a.hv * (nb + 1));   // segments with an SM for each of their blocks
   const bool packed = a.seq_offsets != nullptr;
   Segments s{0, 0};
-  if (a.nseq < 1 || (packed ? 2 * room < 3 * a.nseq : room < 2 * a.nseq)) return s;
-  const int64_t nc = packed ? chunk_slots(a) : (a.time + kChunk - 1) / kChunk, each = packed ? room : room / a.nseq;
-  if (nc < (packed ? 16 : 6)) return s;
+  // Two segments need no transition, so they may have room where more have not; then the first pass is
+  // half a sequence's, which pays where it is clearly cheaper than the second: 4 x 2048 tokens, 16 heads
+  // of 128 x 128, backward in bf16 970 us whole, 845 in halves, forward in fp32 611 and 564.
+  const bool halves = !packed && room < 2 * a.nseq && (backward || a.dtype == QRB_F32) &&
+                      qrb::sm_count() / (a.hv * nb) >= 2 * a.nseq;
+  if (a.nseq < 1 || (packed ? 2 * room < 3 * a.nseq : room < 2 * a.nseq && !halves)) return s;
+  const int64_t nc = packed ? chunk_slots(a) : (a.time + kChunk - 1) / kChunk;
+  const int64_t each = packed ? room : halves ? 2 : room / a.nseq;
+  if (nc < (packed || halves ? 16 : 6)) return s;
   int64_t seg = (nc + each - 1) / each;
-  while (8 * seg * seg < nc) ++seg;
+  while (8 * seg * seg < nc && !halves) ++seg;
   if (packed) {
     if (seg < 3) seg = 3;
     s.nsegs = (int)(nc / seg + a.nseq);
   } else {
     const int64_t ns = (nc + seg - 1) / seg;
-    if (8 * seg + ns + (backward ? 6 : 14) > 4 * nc) return s;
+    if (!halves && 8 * seg + ns + (backward ? 6 : 14) > 4 * nc) return s;
     s.nsegs = (int)(ns * a.nseq);
   }
   s.seg = (int)seg;
@@ -286,14 +292,11 @@ int run(const qrb_delta_args* a, void* ws, size_t wsb, void* stream, bool backwa
   if (p.bound > 0) CUDA(qrb::delta::launch_prep(p, a->dtype, s), "delta chunk factor launch");
   if (p.seg > 0) {
     CUDA(qrb::delta::launch_scan(p, a->dtype, true, s), "delta segment launch");
-    CUDA(qrb::delta::launch_join(p, false, s), "delta join launch");
+    if (backward) CUDA(qrb::delta::launch_rscan(p, a->dtype, true, s), "delta backward segment launch");
+    CUDA(qrb::delta::launch_join(p, s), "delta join launch");
   }
   CUDA(qrb::delta::launch_scan(p, a->dtype, false, s), "delta recurrence launch");
   if (backward) {
-    if (p.seg > 0) {
-      CUDA(qrb::delta::launch_rscan(p, a->dtype, true, s), "delta backward segment launch");
-      CUDA(qrb::delta::launch_join(p, true, s), "delta backward join launch");
-    }
     CUDA(qrb::delta::launch_rscan(p, a->dtype, false, s), "delta backward recurrence launch");
     if (p.bound > 0) CUDA(qrb::delta::launch_grad(p, a->dtype, s), "delta gradient launch");
   }

@@ -28,14 +28,14 @@ struct JoinLayout {
 };
 
 template <int DKP, bool BACK>
-__global__ void __launch_bounds__(JoinLayout<DKP>::kThreads) join_kernel(Params p) {
+__device__ __forceinline__ void join(const Params& p, int block) {
   using L = JoinLayout<DKP>;
   extern __shared__ __align__(16) unsigned char sm[];
   float* X = reinterpret_cast<float*>(sm + 2 * L::kA);   // [row][column]
   float* parts = X + DKP * kCols;                        // [group][row][column]
   const int tid = threadIdx.x;
   const int pitch = (p.dv + kLanes - 1) / kLanes * kLanes, tiles = (p.dv + kCols - 1) / kCols;
-  const int tile = blockIdx.x % tiles, sh = blockIdx.x / tiles, h = sh % p.hv, seq = sh / p.hv;
+  const int tile = block % tiles, sh = block / tiles, h = sh % p.hv, seq = sh / p.hv;
   int g0, ns;
   if (p.offsets == nullptr) {
     ns = max(1, (p.nchunk + p.seg - 1) / p.seg);
@@ -113,23 +113,32 @@ __global__ void __launch_bounds__(JoinLayout<DKP>::kThreads) join_kernel(Params 
   }
 }
 
-template <int DKP, bool BACK>
+// The blocks of the second half of the grid, if there is one, go backward.
+template <int DKP>
+__global__ void __launch_bounds__(JoinLayout<DKP>::kThreads) join_kernel(const __grid_constant__ Params p, unsigned half) {
+  if (blockIdx.x < half)
+    join<DKP, false>(p, blockIdx.x);
+  else
+    join<DKP, true>(p, blockIdx.x - half);
+}
+
+template <int DKP>
 cudaError_t run_join(const Params& p, cudaStream_t s) {
   constexpr int smem = JoinLayout<DKP>::kBytes;
-  cudaError_t e = allow_smem<join_kernel<DKP, BACK>>(smem);
+  cudaError_t e = allow_smem<join_kernel<DKP>>(smem);
   if (e != cudaSuccess) return e;
   const double cells = (double)p.nsegs * p.hv * DKP * DKP;
   LaunchTimer t("delta_join_kernel", s, 4.0 * cells, 2.0 * cells * p.dv);
-  const unsigned grid = (unsigned)p.nseq * p.hv * ((p.dv + kCols - 1) / kCols);
-  join_kernel<DKP, BACK><<<grid, JoinLayout<DKP>::kThreads, smem, s>>>(p);
+  const unsigned half = (unsigned)p.nseq * p.hv * ((p.dv + kCols - 1) / kCols);
+  join_kernel<DKP><<<p.backward ? 2 * half : half, JoinLayout<DKP>::kThreads, smem, s>>>(p, half);
   return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t launch_join(const Params& p, bool backward, cudaStream_t s) {
-  if (backward) return p.dk <= 64 ? run_join<64, true>(p, s) : run_join<128, true>(p, s);
-  return p.dk <= 64 ? run_join<64, false>(p, s) : run_join<128, false>(p, s);
+cudaError_t launch_join(const Params& p, cudaStream_t s) {
+  if (p.offsets == nullptr && p.nsegs <= 2 * p.nseq) return cudaSuccess;   // nothing between first and last
+  return p.dk <= 64 ? run_join<64>(p, s) : run_join<128>(p, s);
 }
 
 }  // namespace delta

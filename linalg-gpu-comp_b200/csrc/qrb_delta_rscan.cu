@@ -46,7 +46,7 @@ struct RBars {
 static_assert(sizeof(RBars) <= 256, "barrier block");
 
 // STATE: only the gradient of the state, of every segment but a sequence's first: from the final state's
-// gradient for the last, else from zero.
+// gradient for the last, else from zero.  It runs beside scan's state-only pass, launched just before it.
 template <int DKP, typename T, bool STATE>
 __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_constant__ Params p, int* err) {
   using L = RLayout<DKP, T>;
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
   const int nb = (p.dv + kLanes - 1) / kLanes;
   const int vb = blockIdx.x % nb, sh = blockIdx.x / nb, h = sh % p.hv;
   const Span mine = span_at(p, sh / p.hv);
-  if (mine.nc < 0 || (STATE && mine.first)) return;
+  if (mine.nc < 0 || (STATE && mine.first)) return;   // (with no other blocks, scan's pass had none either)
   const int hk = h / p.group, nc = mine.nc, slot0 = mine.slot0;
   const int quarters = min(4, (p.dv - vb * kLanes + 31) / 32);
 
@@ -284,6 +284,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (STATE) wait_for_last();
 }
 
 template <int DKP, typename T, bool STATE>
@@ -297,8 +298,17 @@ cudaError_t run_rscan(const Params& p, cudaStream_t s) {
   cudaError_t e = allow_smem<rscan_kernel<DKP, T, STATE>>(smem);
   if (e != cudaSuccess) return e;
   const unsigned spans = (unsigned)(p.seg > 0 ? p.nsegs : p.nseq);
-  rscan_kernel<DKP, T, STATE><<<spans * p.hv * ((p.dv + kLanes - 1) / kLanes), kTcThreads, smem, s>>>(p, err);
-  return cudaGetLastError();
+  cudaLaunchAttribute beside{};
+  beside.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  beside.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(spans * p.hv * ((p.dv + kLanes - 1) / kLanes));
+  cfg.blockDim = dim3(kTcThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = &beside;
+  cfg.numAttrs = STATE ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, rscan_kernel<DKP, T, STATE>, p, err);
 }
 
 template <typename T>

@@ -73,6 +73,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nb = (p.dv + kLanes - 1) / kLanes, nbx = nb + STATE;
   const int vb = blockIdx.x % nbx, sh = blockIdx.x / nbx, h = sh % p.hv;
+  if (STATE) let_next_start();   // rscan's state-only pass, which needs nothing from this one
   const Span mine = span_at<CUT>(p, sh / p.hv);
   const bool unit = STATE && vb == nb;
   if (mine.nc < 0 || (STATE && (mine.last || (unit && mine.first)))) return;

@@ -19,6 +19,11 @@ using namespace sm100;
 
 constexpr int kParts = 4;                   // threads that share a value column
 constexpr int kTok = kChunk / kParts;       // tokens of a thread
+// Two kernels that may run at the same time (their launches say so): the first lets the second start once
+// all its blocks have, and the second does not end before the first has.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 constexpr int kIssuer = kLanes * kParts / 32, kLoader = kIssuer + 1;   // sixteen warps compute, one issues MMAs, one loads
 constexpr int kTcThreads = 32 * (kLoader + 1);
 constexpr int kSmemLimit = 232448;
