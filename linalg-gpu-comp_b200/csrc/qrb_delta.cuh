@@ -84,6 +84,7 @@ struct Params {
   int zero_tail, backward;         // zero the rows behind the last sequence
   // workspace, per chunk slot and head
   unsigned char *kt, *qt, *xt, *pt, *s0p, *dsp, *ep, *dup;
+  unsigned char* dop;              // pieces of dO as tiles like du's, where grad_on_tc
   unsigned char *vt, *dot;         // v, dO: kChunk x 128 tiles, zero behind the sequence and dv
   float* gates;                    // gamma[64], tail[64], beta[64]
   double* gsum;                    // G[64]
@@ -415,6 +416,36 @@ __device__ __forceinline__ Span span_at(const Params& p, int turn) {
 
 __device__ __forceinline__ size_t slot_head(const Params& p, int c, int h) { return (size_t)c * p.hv + h; }
 
+// One chunk's dbeta and dg from the sums the recurrences left: a warp, two tokens a lane.
+__device__ __forceinline__ void gate_sums(const Params& p, const Chunk& ch, size_t at, int h, int lane) {
+  float x[2] = {0.f, 0.f}, db[2] = {0.f, 0.f}, sds = 0.f;
+  for (int n = 0; n < p.nv; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const size_t i = (at * p.nv + n) * kChunk + 2 * lane + e;
+      x[e] += p.odo[i] - p.vdv[i];
+      db[e] += p.edu[i];
+    }
+  for (int i = lane; i < 4 * p.nv; i += 32) sds += p.sds[at * p.nv * 4 + i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sds += __shfl_xor_sync(0xffffffffu, sds, o);
+  float s = x[0] + x[1];             // suffix sums
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float y = __shfl_down_sync(0xffffffffu, s, o);
+    if (lane + o < 32) s += y;
+  }
+  const int64_t to = (ch.b * p.time + ch.t0 + 2 * lane) * p.hv + h;
+  if (2 * lane < ch.len) {
+    p.dg[to] = s + sds;
+    p.dbeta[to] = db[0];
+  }
+  if (2 * lane + 1 < ch.len) {
+    p.dg[to + p.hv] = s - x[0] + sds;
+    p.dbeta[to + p.hv] = db[1];
+  }
+}
+
 // ---- launchers ----
 cudaError_t launch_plan(const Params& p, cudaStream_t s);
 cudaError_t launch_prep(const Params& p, int dtype, cudaStream_t s);
@@ -422,6 +453,12 @@ cudaError_t launch_scan(const Params& p, int dtype, bool state_only, cudaStream_
 cudaError_t launch_rscan(const Params& p, int dtype, bool state_only, cudaStream_t s);
 cudaError_t launch_join(const Params& p, cudaStream_t s);
 cudaError_t launch_grad(const Params& p, int dtype, cudaStream_t s);
+template <typename T>
+cudaError_t launch_grad_tc(const Params& p, cudaStream_t s);
+// The gradients of 16-bit inputs with dk above 64 go through tcgen05: 128 rows of state columns fill its M,
+// and two-piece tiles its shared memory (4 x 2048 tokens, 16 heads of 128 x 128, bf16: 120 us
+// against 292 with mma.sync).
+constexpr bool grad_on_tc(int dk, int dtype) { return dk > 64 && dtype != 0; }
 cudaError_t launch_step(const qrb_delta_step_args& a, cudaStream_t s);
 
 }  // namespace delta

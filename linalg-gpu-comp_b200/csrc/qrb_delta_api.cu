@@ -128,7 +128,7 @@ Segments segments(const qrb_delta_args& a, bool backward) {
 }
 
 struct Layout {
-  size_t cstart, kt, qt, xt, pt, gates, gsum, s0p, dsp, ep, dup, odo, vdv, edu, sds, s_last, vt, dot, total;
+  size_t cstart, kt, qt, xt, pt, gates, gsum, s0p, dsp, ep, dup, odo, vdv, edu, sds, s_last, vt, dot, dop, total;
   size_t seg_s, seg_a, seg_ds;
 };
 
@@ -158,6 +158,7 @@ Layout layout(const qrb_delta_args& a, bool backward) {
   if (backward) l.seg_ds = take(cells * ((a.dv + 127) / 128) * 128);
   if (backward) {
     l.dot = take(staged);
+    if (grad_on_tc(a.dk, a.dtype)) l.dop = take(n * a.hv * nv * tile_bytes(kTile, pi, kChunk));
     l.gsum = take(n * a.hv * kChunk * 8);
     l.s0p = take(n * a.hv * nv * tile_bytes(kTile, ps, dkp));
     l.dsp = take(n * a.hv * nv * tile_bytes(kTile, ps, dkp));
@@ -277,6 +278,7 @@ int run(const qrb_delta_args* a, void* ws, size_t wsb, void* stream, bool backwa
   p.pt = w + l.pt;
   p.vt = w + l.vt;
   p.dot = w + l.dot;
+  p.dop = w + l.dop;
   p.gates = reinterpret_cast<float*>(w + l.gates);
   p.gsum = reinterpret_cast<double*>(w + l.gsum);
   p.s0p = w + l.s0p;

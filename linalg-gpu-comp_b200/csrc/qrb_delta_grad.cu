@@ -1,5 +1,6 @@
 // Gradients of q, k, g and beta of the gated delta rule, chunk by chunk (mathematics in
-// qrb_delta.cuh).
+// qrb_delta.cuh), with mma.sync: for fp32, whose three pieces leave no room for tiles in flight beside
+// tcgen05's operands, and for dk up to 64, half of its rows.  qrb_delta_gradtc.cu has the others.
 //
 // With every chunk's S0, e, dS' and du in the workspace the chunks are independent: one block
 // per (chunk, q/k head) adds the heads that share it in order, so no atomics are needed and
@@ -159,33 +160,7 @@ __global__ void __launch_bounds__(512) grad_kernel(Params p) {
         tq_[j][r] += aq[j][r];
         tk_[j][r] += ay[j][r];
       }
-    if (warp == 0) {                     // dbeta, dg: two tokens a lane
-      float x[2] = {0.f, 0.f}, db[2] = {0.f, 0.f}, sds = 0.f;
-      for (int n = 0; n < p.nv; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const size_t i = (at * p.nv + n) * kChunk + 2 * lane + e;
-          x[e] += p.odo[i] - p.vdv[i];
-          db[e] += p.edu[i];
-        }
-      for (int i = lane; i < 4 * p.nv; i += 32) sds += p.sds[at * p.nv * 4 + i];
-      sds = warp_sum(sds);
-      float s = x[0] + x[1];             // suffix sums
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const float y = __shfl_down_sync(0xffffffffu, s, o);
-        if (lane + o < 32) s += y;
-      }
-      const int64_t to = (ch.b * p.time + ch.t0 + 2 * lane) * p.hv + h;
-      if (2 * lane < ch.len) {
-        p.dg[to] = s + sds;
-        p.dbeta[to] = db[0];
-      }
-      if (2 * lane + 1 < ch.len) {
-        p.dg[to + p.hv] = s - x[0] + sds;
-        p.dbeta[to + p.hv] = db[1];
-      }
-    }
+    if (warp == 0) gate_sums(p, ch, at, h, lane);
   }
   const int64_t tok = ch.b * p.time + ch.t0;
 #pragma unroll
@@ -216,8 +191,10 @@ cudaError_t run_grad(const Params& p, cudaStream_t s) {
 }  // namespace
 
 cudaError_t launch_grad(const Params& p, int dtype, cudaStream_t s) {
-  if (dtype == 1) return p.dk <= 64 ? run_grad<64, __nv_bfloat16>(p, s) : run_grad<128, __nv_bfloat16>(p, s);
-  if (dtype == 2) return p.dk <= 64 ? run_grad<64, __half>(p, s) : run_grad<128, __half>(p, s);
+  if (grad_on_tc(p.dk, dtype))
+    return dtype == 1 ? launch_grad_tc<__nv_bfloat16>(p, s) : launch_grad_tc<__half>(p, s);
+  if (dtype == 1) return run_grad<64, __nv_bfloat16>(p, s);
+  if (dtype == 2) return run_grad<64, __half>(p, s);
   return p.dk <= 64 ? run_grad<64, float>(p, s) : run_grad<128, float>(p, s);
 }
 

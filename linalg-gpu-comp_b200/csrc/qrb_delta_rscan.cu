@@ -178,7 +178,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
         if (!warp_wait(&bars.full[i % L::kStages], (i / L::kStages) & 1, abort, err, 81)) break;
         staged<T>(stage + L::kOffD, tb, lcol, x);
         with_tokens(gates.gam, [&](int j, float g) { u[j] = x[j] * (p.scale * g); });
-        put_pieces<P, 0>(tl + L::tF + tb / 2, 32, x);
+        // (for the gradient kernel too, where it takes them as tiles)
+        constexpr int keep = !STATE && grad_on_tc(DKP, sizeof(T) == 2) ? P : 0;
+        put_pieces<P, keep>(tl + L::tF + tb / 2, 32, x, p.dop + at * tile_bytes(kTile, P, kChunk), lane, kChunk, tb);
         put_pieces<PS, 0>(tl + L::tO + tb / 2, 32, u);
         tmem_st_wait();
         tc_fence_before();
@@ -239,7 +241,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
           const float s = sum_columns(x);
           if ((lane & 1) == 0) p.edu[at * kChunk + tb + lane / 2] = s;
         }
-        {
+        if (!STATE) {
           staged<T>(stage + L::kOffV, tb, lcol, x);
 #pragma unroll
           for (int j = 0; j < kTok; ++j) x[j] *= y[j];
