@@ -98,6 +98,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
         bulk_load(d + L::kOffX, p.xt + at * L::kX, L::kX, bar);
         bulk_load(d + L::kOffQ, p.qt + qk, L::kK, bar);
         bulk_load(d + L::kOffV, p.vt + (at * nb + vb) * L::kV, L::kV, bar);
+        if (!STATE) {   // what the sums of this chunk will read
+          constexpr int kWS = tile_bytes(kTile, PS, DKP), kWF = tile_bytes(kTile, PS, kChunk);
+          bulk_prefetch(p.ep + (at * p.nv + 4 * vb) * kWF, quarters * kWF);
+          bulk_prefetch(p.odo + (at * p.nv + 4 * vb) * kChunk, quarters * kChunk * 4);
+          if (i > 0 && i % kAnchor == 0)
+            bulk_prefetch(p.s0p + (slot_head(p, slot0 + c + 1, h) * p.nv + 4 * vb) * kWS, quarters * kWS);
+        }
       }
       if (*abort)   // loads in flight must land before the block's memory goes
         for (int s = 0; s < L::kStages; ++s)

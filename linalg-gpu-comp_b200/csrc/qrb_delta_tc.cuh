@@ -111,6 +111,11 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
+// Brings contiguous global memory (the same alignment) into L2.
+__device__ __forceinline__ void bulk_prefetch(const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
+
 constexpr uint32_t kNoTmem = 0xffffffffu;
 
 // N values of this lane as PS pieces of N / 2 columns each, piece_cols apart.  KEEP > 0: the first KEEP
