@@ -36,7 +36,8 @@ typedef struct {
  * offsets lie on the device, start at 0 and do not decrease (others are clamped to the tensors:
  * no access leaves them, but results are unspecified).  Empty sequences are allowed.  Rows behind
  * the last sequence are not read; outputs there stay as they are, or with zero_tail become 0.
- * g may be any number up to +inf's overflow; -inf (and all below -120) empties the state.
+ * g may be positive as long as its sum over any stretch of a sequence stays below 88 (exp of it must be
+ * finite); -inf (and all below -120) empties the state.
  * Forward:  q, k, v, g, beta, initial_state (NULL: zeros) -> o, final_state (NULL: not stored).
  * Backward: also d_o and dfinal_state (NULL: zeros) -> dq, dk_, dv_, dg, dbeta (dense, shaped like
  * q, k, v, g, beta) and dinitial_state (NULL: not stored).  States are dense fp32

@@ -60,8 +60,9 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, seq_of
 
     ``q``, ``k``: (batch, time, heads_k, dk) with dk <= 128; ``v``: (batch, time, heads, dv) with dv <= 256
     and heads a multiple of heads_k (value head h reads q/k head ``h // (heads // heads_k)``); ``g`` (the
-    decay's logarithm, -inf empties the state) and ``beta``: (batch, time, heads) float32.  Any strides;
-    tensors whose last dimension is not dense are copied.  ``scale`` defaults to dk ** -0.5,
+    decay's logarithm; -inf empties the state, and what is positive must not add up to 88 or more) and
+    ``beta``: (batch, time, heads) float32.  Any strides; tensors whose last dimension is not dense are
+    copied.  ``scale`` defaults to dk ** -0.5,
     ``initial_state`` (sequences, heads, dk, dv) float32 to zeros.
 
     ``seq_offsets`` (sequences + 1, int32 or int64, on the device) packs sequences of different lengths,
