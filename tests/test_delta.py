@@ -533,6 +533,35 @@ def test_long_decay_and_values_that_are_not_finite():
 
 
 @gpu
+@pytest.mark.parametrize("offs", [None, [0, 2500, 2500, 2503, 4097]])
+def test_long_captured(offs):
+    """Both passes in one graph, replayed with other values, beside the same calls on another stream."""
+    x = make(1, 4097, 2, 2, 96, 64, BF)
+    so = None if offs is None else torch.tensor(offs, device="cuda")
+    n = 1 if offs is None else len(offs) - 1
+    init, dS = states(n, 2, 96, 64), states(n, 2, 96, 64, 2)
+
+    def both(x, init):
+        return (*api().gated_delta_rule(*x, initial_state=init, seq_offsets=so),
+                *api().gated_delta_rule_backward(x[2], *x, initial_state=init, seq_offsets=so, dfinal_state=dS))
+    both(x, init)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        got = both(x, init)
+    y, init2 = make(1, 4097, 2, 2, 96, 64, BF, seed=9), states(n, 2, 96, 64, 7)
+    want = both(y, init2)
+    for a, b in zip((*x, init), (*y, init2)):
+        a.copy_(b)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        beside = both(y, init2)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(torch.equal(a, b) for a, b in zip(beside, want))
+
+
+@gpu
 def test_wrong_offsets_of_long_sequences_stay_inside():
     x = make(1, 2000, 1, 1, 64, 64, BF)
     guard = torch.full((6000, 64), 5.0, dtype=BF, device="cuda")
