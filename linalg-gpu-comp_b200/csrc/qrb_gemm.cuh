@@ -75,6 +75,61 @@ __device__ __forceinline__ float phi(float x) {
   const float half = 0.5f * t * __expf(fmaf(-z, z, q));   // erfc(z) / 2
   return x < 0.f ? half : 1.f - half;
 }
+// Packed fp32 arithmetic: two values an instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// x Phi(x) of two values: phi with s = z sqrt(log2 e) in place of z, q in units of log2 e and with erfc's
+// factor 1/2 in it.
+__device__ __forceinline__ void gelu2(float& x, float& y) {
+  auto both = [](float c) { return pair(c, c); };
+  const uint64_t xy = pair(x, y), a = pair(fabsf(x), fabsf(y));
+  const uint64_t s = mul2(a, both(8.493218003e-01f)), n = mul2(a, both(-8.493218003e-01f));
+  float u, v;
+  split(fma2(s, both(4.162773056e-01f), both(1.f)), u, v);
+  const uint64_t t = pair(rcp(u), rcp(v));
+  uint64_t q = both(2.516222965e-01f);
+  q = fma2(q, t, both(-1.210104463e+00f));
+  q = fma2(q, t, both(2.194834290e+00f));
+  q = fma2(q, t, both(-1.688721258e+00f));
+  q = fma2(q, t, both(4.347611031e-01f));
+  q = fma2(q, t, both(-2.811356677e-01f));
+  q = fma2(q, t, both(1.423633349e-01f));
+  q = fma2(q, t, both(5.393846184e-01f));
+  q = fma2(q, t, both(1.442744166e+00f));
+  q = fma2(q, t, both(-2.825748311e+00f));
+  split(fma2(n, s, q), u, v);
+  const uint64_t half = mul2(t, pair(ex2(u), ex2(v)));   // erfc(z) / 2
+  float h, k;
+  split(half, h, k);
+  split(fma2(half, both(-1.f), both(1.f)), u, v);
+  split(mul2(xy, pair(x < 0.f ? h : u, y < 0.f ? k : v)), x, y);
+}
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 
 __device__ __forceinline__ float activate(float x, int act) {
@@ -96,6 +151,7 @@ __device__ __forceinline__ float slope(float x, int act) {
 // act over N values at once: one test for all of them.
 template <int N>
 __device__ __forceinline__ void activate_all(float (&x)[N], int act) {
+  static_assert(N % 2 == 0, "pairs");
   if (act == QRB_ACT_NONE) return;
   if (act == QRB_ACT_RELU) {
 #pragma unroll
@@ -105,7 +161,7 @@ __device__ __forceinline__ void activate_all(float (&x)[N], int act) {
     for (int i = 0; i < N; ++i) x[i] = activate(x[i], QRB_ACT_SILU);
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = activate(x[i], QRB_ACT_GELU);
+    for (int i = 0; i < N; i += 2) gelu2(x[i], x[i + 1]);
   }
 }
 
