@@ -141,6 +141,37 @@ def test_strides(m, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("size", [(300, 72, 1001), (129, 8, 257), (1023, 200, 13), (513, 64, 70)])
+def test_rows_with_room_behind(size, dtype):
+    """Rows that begin on 16 bytes and end inside a unit of them: what lies behind stays as it was."""
+    m, k, n = size
+    x, w, b, res, _ = make(m, k, n, dtype)
+    ld = (n + 15) // 8 * 8
+    big = [torch.full((m, ld), 7.0, dtype=dtype, device="cuda") for _ in range(2)]
+    big[0][:, :n] = res
+    for act in ("none", "gelu"):
+        out = api().linear(x, w, b, activation=act, residual=big[0][:, :n], out=big[1][:, :n])
+        assert rel(out, reference(x, w, b, act, res)[1]) <= tol(dtype)
+        assert (big[1][:, n:] == 7).all()
+        assert torch.equal(out, api().linear(x, w, b, activation=act, residual=res))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("m", [1, 40, 200])
+def test_activations_at_their_ends(m, dtype):
+    b = torch.tensor([math.inf, -math.inf, math.nan, 0.0, -0.0, 6e4, -6e4, 30.0, -30.0, 1e-4], device="cuda").to(dtype)
+    x, w = torch.zeros(m, 16, dtype=dtype, device="cuda"), torch.ones(10, 16, dtype=dtype, device="cuda")
+    for act in ACTS:
+        y, want = api().linear(x, w, b, activation=act), ACTS[act](b.double())
+        for i in (0, 2, 3, 4, 5, 6, 7, 8, 9):     # -inf: the limit or, as inf * 0, NaN
+            got = y[:, i].double()
+            assert got.isnan().all() if want[i].isnan() else torch.allclose(got, want[i], rtol=1e-2, atol=1e-6), (act, i)
+        assert (y[:, 1].isnan() | (y[:, 1] == ACTS[act](b.double())[1].nan_to_num(0.0, 0.0, -math.inf))).all(), act
+
+
+@gpu
 def test_rows_are_independent():
     """Rows of the result come from their rows of x alone, whatever the others hold."""
     for m in (5, 300):
