@@ -455,10 +455,9 @@ cudaError_t launch_join(const Params& p, cudaStream_t s);
 cudaError_t launch_grad(const Params& p, int dtype, cudaStream_t s);
 template <typename T>
 cudaError_t launch_grad_tc(const Params& p, cudaStream_t s);
-// The gradients of 16-bit inputs with dk above 64 go through tcgen05: 128 rows of state columns fill its M,
-// and two-piece tiles its shared memory (4 x 2048 tokens, 16 heads of 128 x 128, bf16: 120 us
-// against 292 with mma.sync).
-constexpr bool grad_on_tc(int dk, int dtype) { return dk > 64 && dtype != 0; }
+// The gradients of 16-bit inputs go through tcgen05, whose shared memory two pieces of every tile fill
+// (4 x 2048 tokens, 16 heads of 128 x 128, bf16: 120 us against 292 with mma.sync).
+constexpr bool grad_on_tc(int dtype) { return dtype != 0; }
 cudaError_t launch_step(const qrb_delta_step_args& a, cudaStream_t s);
 
 }  // namespace delta

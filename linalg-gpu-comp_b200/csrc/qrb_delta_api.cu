@@ -158,7 +158,7 @@ Layout layout(const qrb_delta_args& a, bool backward) {
   if (backward) l.seg_ds = take(cells * ((a.dv + 127) / 128) * 128);
   if (backward) {
     l.dot = take(staged);
-    if (grad_on_tc(a.dk, a.dtype)) l.dop = take(n * a.hv * nv * tile_bytes(kTile, pi, kChunk));
+    if (grad_on_tc(a.dtype)) l.dop = take(n * a.hv * nv * tile_bytes(kTile, pi, kChunk));
     l.gsum = take(n * a.hv * kChunk * 8);
     l.s0p = take(n * a.hv * nv * tile_bytes(kTile, ps, dkp));
     l.dsp = take(n * a.hv * nv * tile_bytes(kTile, ps, dkp));

@@ -1,6 +1,6 @@
 // Gradients of q, k, g and beta of the gated delta rule, chunk by chunk (mathematics in
 // qrb_delta.cuh), with mma.sync: for fp32, whose three pieces leave no room for tiles in flight beside
-// tcgen05's operands, and for dk up to 64, half of its rows.  qrb_delta_gradtc.cu has the others.
+// tcgen05's operands.  qrb_delta_gradtc.cu has the 16-bit types.
 //
 // With every chunk's S0, e, dS' and du in the workspace the chunks are independent: one block
 // per (chunk, q/k head) adds the heads that share it in order, so no atomics are needed and
@@ -191,10 +191,7 @@ cudaError_t run_grad(const Params& p, cudaStream_t s) {
 }  // namespace
 
 cudaError_t launch_grad(const Params& p, int dtype, cudaStream_t s) {
-  if (grad_on_tc(p.dk, dtype))
-    return dtype == 1 ? launch_grad_tc<__nv_bfloat16>(p, s) : launch_grad_tc<__half>(p, s);
-  if (dtype == 1) return run_grad<64, __nv_bfloat16>(p, s);
-  if (dtype == 2) return run_grad<64, __half>(p, s);
+  if (grad_on_tc(dtype)) return dtype == 1 ? launch_grad_tc<__nv_bfloat16>(p, s) : launch_grad_tc<__half>(p, s);
   return p.dk <= 64 ? run_grad<64, float>(p, s) : run_grad<128, float>(p, s);
 }
 

@@ -1,10 +1,12 @@
-// Gradients of q and k (and the sums of g's and beta's) for 16-bit inputs with dk above 64, on the tensor
-// cores through tcgen05; qrb_delta_grad.cu has the other sizes and the mathematics in words.
+// Gradients of q and k (and the sums of g's and beta's) for 16-bit inputs, on the tensor cores through
+// tcgen05; qrb_delta_grad.cu has fp32 and the mathematics in words.
 //
 // The transposed gradients are formed, tensor-memory lane = q/k column, so that S0, dS', K and Q are A
 // operands of 128 rows in the layouts they were written in, with value columns (or tokens) along k:
 //     [aq | ay]^T = S0 [dO | du]^T        au^T = dS' e^T        [az ; an] = [dO ; du] e
 //     dq^T = scale gam aq^T + K^T Z^T     dk^T = tail bet au^T - gam bet ay^T + Q^T Z + K^T (N + N^T)
+// For dk up to 64 the rows are S0's and dS's, K's and Q's side by side: half of what is computed is not
+// read, and the upper half of the lanes hands its part of dk to the lower one through shared memory.
 // with Z, N the masked and decayed az, an.  Two pieces of S0, dS', e, du, Z, N leave 2^-18 of each, far
 // below the 16-bit outputs.  A block walks over (chunk, q/k head) pairs: one thread loads value tiles of 32
 // columns into a ring, one issues the products, sixteen warps scale and store, and one warp adds up dg and
@@ -19,26 +21,34 @@ namespace {
 
 constexpr int kGateWarp = kLoader + 1, kGradThreads = 32 * (kGateWarp + 1);
 
-template <typename T>
+template <int DKP, typename T>
 struct TLayout {
-  static constexpr int DK = 128, P = Pieces<T>::kIn, PS = 2;
-  static constexpr int kStages = P == 1 ? 3 : 2;
-  static constexpr int kT = kTile * kChunk * 2, kS = kTile * DK * 2;   // a piece of a token tile, of a state tile
-  static constexpr int kWS = tile_bytes(kTile, kBackPieces, DK), kWF = tile_bytes(kTile, kBackPieces, kChunk);
-  // one piece: dO | du | du'; two: dO | du | dO' | du', so that [dO ; du] and the second pieces lie together
-  static constexpr int kOffDU = kT, kOffLo = P == 1 ? kT : 2 * kT, kOffE = (P + 2) * kT, kOffS = kOffE + 2 * kT,
-                       kOffDS = kOffS + 2 * kS, kStage = kOffDS + 2 * kS;
-  static constexpr int kK = tile_bytes(kChunk, P, DK), kZ = tile_bytes(kChunk, PS, kChunk);
+  static constexpr bool kHalf = DKP == 64;   // S0 and dS', K and Q share the 128 rows
+  static constexpr int P = Pieces<T>::kIn, PS = 2;
+  static constexpr int kStages = kHalf ? (P == 1 ? 4 : 3) : (P == 1 ? 3 : 2);
+  static constexpr int kT = kTile * kChunk * 2, kS = kTile * DKP * 2;   // a piece of a token tile, of a state tile
+  static constexpr int kWS = tile_bytes(kTile, kBackPieces, DKP), kWF = tile_bytes(kTile, kBackPieces, kChunk);
+  // First pieces dO | du, then (dk above 64) second pieces, e, S0 and dS' with both pieces each; or e, second
+  // pieces with e's, and [S0 | dS'] a piece.  Second pieces: du', and dO' before it where there is one, so
+  // that [dO ; du] lie together and so do [dO' ; du'].
+  static constexpr int kOffDU = kT, kOffE = kHalf ? 2 * kT : (P + 2) * kT;
+  static constexpr int kOffLo = kHalf ? 3 * kT : 2 * kT, kOffDULo = kOffLo + (P - 1) * kT;
+  static constexpr int kOffELo = kHalf ? kOffDULo + kT : kOffE + kT;
+  static constexpr int kOffS = kOffELo + kT, kOffDS = kHalf ? kOffS + kS : kOffS + 2 * kS;
+  static constexpr int kStep = kHalf ? 2 * kS : kS;   // between pieces of S0 and of dS'
+  static constexpr int kStage = kOffS + 4 * kS;
+  static constexpr int kK = tile_bytes(kChunk, P, DKP), kZ = tile_bytes(kChunk, PS, kChunk);
   static constexpr int kOffK = kStages * kStage, kOffQ = kOffK + kK, kOffZ = kOffQ + kK, kOffN = kOffZ + kZ;
-  static constexpr int kBar = kOffN + kZ;
+  static constexpr int kOffX = kOffN + kZ;   // kHalf: what the upper lanes hold of dk
+  static constexpr int kBar = kOffX + (kHalf ? kChunk * 64 * 4 : 0);
   static constexpr int kBytes = kBar + 256 + 1024;   // 1024: alignment
-  static_assert(kBytes <= kSmemLimit, "shared memory of one block");
-  // tensor memory columns
-  static constexpr uint32_t tA = 0, tU = 128, tZ = 192, tLo = 256, tDQ = 320, tDK = 384;
+  static_assert(kBytes <= kSmemLimit && kStage % 1024 == 0, "shared memory of one block");
+  // tensor memory columns: [aq | ay], au | [az ; an] | their second pieces of dO, du | dq | dk | kHalf: dk of N
+  static constexpr uint32_t tA = 0, tU = 128, tZ = 192, tLo = 256, tDQ = 320, tDK = 384, tDN = kHalf ? 448 : 384;
 };
 
 struct GradBars {
-  uint64_t full[3], empty[3], kq, acc, zn, read, done, drain;
+  uint64_t full[4], empty[4], kq, acc, zn, read, done, over, drain;
   uint32_t tmem;
   int abort;
 };
@@ -73,9 +83,9 @@ __device__ __forceinline__ void put_row(unsigned char* tile, int row, int col, f
   }
 }
 
-template <typename T>
+template <int DKP, typename T>
 __global__ void __launch_bounds__(kGradThreads, 1) grad_tc_kernel(const __grid_constant__ Params p, int* err) {
-  using L = TLayout<T>;
+  using L = TLayout<DKP, T>;
   constexpr int P = L::P;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -85,12 +95,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_tc_kernel(const __grid_c
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t items = (int64_t)p.bound * p.hk;
   if (tid == 0) {
-    for (int i = 0; i < 3; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&bars.full[i], 1);
       mbar_init(&bars.empty[i], 1);
     }
     for (uint64_t* x : {&bars.kq, &bars.acc, &bars.done, &bars.drain}) mbar_init(x, 1);
     for (uint64_t* x : {&bars.zn, &bars.read}) mbar_init(x, 4 * kParts);
+    mbar_init(&bars.over, 2 * kParts);
     bars.abort = 0;
     fence_mbar_init();
   }
@@ -110,7 +121,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_tc_kernel(const __grid_c
   if (warp == kLoader) {
     // ---------------- loads: one thread ----------------
     if (lane == 0) {
-      uint32_t tiles = 0, unit = 0;
+      uint32_t tiles = 0, unit = 0, pairs = 0;
       bool ok = true;
       for (int64_t i = first; i < items && ok; i = next(i)) {
         const int c = (int)(i / p.hk), hk = (int)(i - (int64_t)c * p.hk);
@@ -121,31 +132,52 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_tc_kernel(const __grid_c
             if (tiles >= L::kStages &&
                 !(ok = mbar_wait_abort(&bars.empty[stage], (tiles / L::kStages - 1) & 1, abort, err, 91)))
               break;
+            // Once a unit, in order, and before its last tile, so that this unit's own products cannot be done (a
+            // wait by parity tells a phase from its neighbours only): the last one's are.  K and Q, which go
+            // where the last pair's lay, could not come earlier; the tiles before this one could.
+            if (n == min(p.nv, L::kStages) - 1) {
+              if (unit > 0 && !(ok = mbar_wait_abort(&bars.done, (unit - 1) & 1, abort, err, 92))) break;
+              if (hh == 0) {
+                const size_t qk = ((size_t)c * p.hk + hk) * L::kK;
+                mbar_arrive_expect_tx(&bars.kq, 2 * L::kK);
+                bulk_load(sm + L::kOffK, p.kt + qk, L::kK, &bars.kq);
+                bulk_load(sm + L::kOffQ, p.qt + qk, L::kK, &bars.kq);
+                ++pairs;
+              }
+            }
             unsigned char* d = sm + stage * L::kStage;
             uint64_t* bar = &bars.full[stage];
             const unsigned char *o = p.dop + (at + n) * P * L::kT, *u = p.dup + (at + n) * L::kWF;
             mbar_arrive_expect_tx(bar, L::kStage);
+            const unsigned char *e = p.ep + (at + n) * L::kWF, *s0 = p.s0p + (at + n) * L::kWS,
+                                *ds = p.dsp + (at + n) * L::kWS;
             bulk_load(d, o, L::kT, bar);
-            if (P == 1) {
+            if (P > 1) bulk_load(d + L::kOffLo, o + L::kT, L::kT, bar);
+            if (L::kOffDULo == L::kOffDU + L::kT) {
               bulk_load(d + L::kOffDU, u, 2 * L::kT, bar);
             } else {
               bulk_load(d + L::kOffDU, u, L::kT, bar);
-              bulk_load(d + L::kOffLo, o + L::kT, L::kT, bar);
-              bulk_load(d + L::kOffLo + L::kT, u + L::kT, L::kT, bar);
+              bulk_load(d + L::kOffDULo, u + L::kT, L::kT, bar);
             }
-            bulk_load(d + L::kOffE, p.ep + (at + n) * L::kWF, 2 * L::kT, bar);
-            bulk_load(d + L::kOffS, p.s0p + (at + n) * L::kWS, 2 * L::kS, bar);
-            bulk_load(d + L::kOffDS, p.dsp + (at + n) * L::kWS, 2 * L::kS, bar);
-            // K and Q go where the last pair's lay, once its products are done
-            if (hh == 0 && n == min(p.nv, L::kStages) - 1) {
-              if (unit > 0 && !(ok = mbar_wait_abort(&bars.done, (unit - 1) & 1, abort, err, 92))) break;
-              const size_t qk = ((size_t)c * p.hk + hk) * L::kK;
-              mbar_arrive_expect_tx(&bars.kq, 2 * L::kK);
-              bulk_load(sm + L::kOffK, p.kt + qk, L::kK, &bars.kq);
-              bulk_load(sm + L::kOffQ, p.qt + qk, L::kK, &bars.kq);
+            if (L::kHalf) {
+              bulk_load(d + L::kOffE, e, L::kT, bar);
+              bulk_load(d + L::kOffELo, e + L::kT, L::kT, bar);
+              for (int i = 0; i < 2; ++i) {
+                bulk_load(d + L::kOffS + i * L::kStep, s0 + i * L::kS, L::kS, bar);
+                bulk_load(d + L::kOffDS + i * L::kStep, ds + i * L::kS, L::kS, bar);
+              }
+            } else {
+              bulk_load(d + L::kOffE, e, 2 * L::kT, bar);
+              bulk_load(d + L::kOffS, s0, 2 * L::kS, bar);
+              bulk_load(d + L::kOffDS, ds, 2 * L::kS, bar);
             }
           }
         }
+      }
+      if (*abort) {   // loads in flight must land before the block's memory goes
+        for (uint32_t i = 0; i < L::kStages; ++i)
+          if (tiles > i) mbar_wait(&bars.full[i], ((tiles - 1 - i) / L::kStages) & 1, 1u << 22);
+        if (pairs > 0) mbar_wait(&bars.kq, (pairs - 1) & 1, 1u << 22);
       }
     }
     __syncwarp();
@@ -153,11 +185,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_tc_kernel(const __grid_c
     // ---------------- products: one thread ----------------
     if (lane == 0) {
       constexpr uint32_t kAmn = 1u << 15;
-      constexpr uint32_t wide = idesc_bf16(128, 1) | kAmn, mn = idesc_bf16(64, 1) | kAmn, km = idesc_bf16(64, 0) | kAmn;
+      constexpr uint32_t all = idesc_bf16(192, 1) | kAmn, wide = idesc_bf16(128, 1) | kAmn;
+      constexpr uint32_t mn = idesc_bf16(64, 1) | kAmn, km = idesc_bf16(64, 0) | kAmn;
       // tiles of the recurrences: 16-byte units of 8 columns, 32 value rows apart; 16 rows a step
       auto unitd = [](uint32_t a, int k) { return sdesc_make(a + 256u * k, 128, kTile * 16, 0); };
-      // K, Q: columns as M; Z, N: rows (tokens) as N or across them; 16 tokens a step
-      auto across = [](uint32_t a, int k) { return sdesc_sw128(a + 2048u * k, kChunk * 128, 1024); };
+      // K, Q: columns as M (K's 128, or K's 64 and Q's); Z, N: rows (tokens) as N or across them; 16 tokens a step
+      auto across = [](uint32_t a, int k) {
+        return sdesc_sw128(a + 2048u * k, L::kHalf ? L::kK : kChunk * 128, 1024);
+      };
       auto along = [](uint32_t a, int k) { return sdesc_sw128(a + 32u * k, 16, 1024); };
       const uint32_t base = smem_u32(sm);
       uint32_t tiles = 0, unit = 0, item = 0;
@@ -169,21 +204,29 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_tc_kernel(const __grid_c
             const uint32_t stage = tiles % L::kStages;
             if (!(ok = mbar_wait_abort(&bars.full[stage], (tiles / L::kStages) & 1, abort, err, 94))) break;
             tc_fence_after();
-            const uint32_t d = base + stage * L::kStage, du = d + L::kOffDU, lo = d + L::kOffLo, e = d + L::kOffE,
-                           s = d + L::kOffS, ds = d + L::kOffDS;
+            const uint32_t d = base + stage * L::kStage, lo = d + L::kOffLo, dul = d + L::kOffDULo, e = d + L::kOffE,
+                           el = d + L::kOffELo, s = d + L::kOffS, ds = d + L::kOffDS;
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k) {
               const uint32_t acc = n > 0 || k > 0;
-              mma_ss(tmem + L::tA, unitd(s + L::kS, k), unitd(d, k), wide, acc);
-              mma_ss(tmem + L::tA, unitd(s, k), unitd(d, k), wide, 1);
-              mma_ss(tmem + L::tA + 64, unitd(s, k), unitd(P == 1 ? du + L::kT : lo + L::kT, k), mn, 1);
-              if (P > 1) mma_ss(tmem + L::tA, unitd(s, k), unitd(lo, k), mn, 1);
-              mma_ss(tmem + L::tU, unitd(ds + L::kS, k), unitd(e, k), mn, acc);
-              mma_ss(tmem + L::tU, unitd(ds, k), unitd(e + L::kT, k), mn, 1);
-              mma_ss(tmem + L::tU, unitd(ds, k), unitd(e, k), mn, 1);
-              mma_ss(tmem + L::tZ, unitd(d, k), unitd(e + L::kT, k), mn, acc);
+              if (L::kHalf) {   // [S0 ; dS'] [dO | du | e]
+                mma_ss(tmem + L::tA, unitd(s + L::kStep, k), unitd(d, k), all, acc);
+                mma_ss(tmem + L::tA, unitd(s, k), unitd(d, k), all, 1);
+                if (P > 1) mma_ss(tmem + L::tA, unitd(s, k), unitd(lo, k), all, 1);
+                else mma_ss(tmem + L::tA + 64, unitd(s, k), unitd(dul, k), wide, 1);
+              } else {
+                mma_ss(tmem + L::tA, unitd(s + L::kStep, k), unitd(d, k), wide, acc);
+                mma_ss(tmem + L::tA, unitd(s, k), unitd(d, k), wide, 1);
+                mma_ss(tmem + L::tA + 64, unitd(s, k), unitd(dul, k), mn, 1);
+                if (P > 1) mma_ss(tmem + L::tA, unitd(s, k), unitd(lo, k), mn, 1);
+                mma_ss(tmem + L::tU, unitd(ds + L::kStep, k), unitd(e, k), mn, acc);
+                mma_ss(tmem + L::tU, unitd(ds, k), unitd(el, k), mn, 1);
+                mma_ss(tmem + L::tU, unitd(ds, k), unitd(e, k), mn, 1);
+              }
+              mma_ss(tmem + L::tZ, unitd(d, k), unitd(el, k), mn, acc);
               mma_ss(tmem + L::tZ, unitd(d, k), unitd(e, k), mn, 1);
-              mma_ss(tmem + L::tLo, unitd(lo, k), unitd(e, k), mn, acc);   // (one piece: du over du')
+              // the lower half du', the upper one dO' or, with one piece, nothing that is read
+              mma_ss(tmem + L::tLo, unitd(dul - L::kT, k), unitd(e, k), mn, acc);
             }
             mma_commit(&bars.empty[stage]);
           }
@@ -192,8 +235,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_tc_kernel(const __grid_c
           if (!(ok = mbar_wait_abort(&bars.zn, unit & 1, abort, err, 95))) break;
           if (hh == 0 && !(ok = mbar_wait_abort(&bars.kq, item & 1, abort, err, 96))) break;
           tc_fence_after();
-          const uint32_t K = base + L::kOffK, Q = base + L::kOffQ, Z = base + L::kOffZ, N = base + L::kOffN;
-          constexpr uint32_t kZp = kChunk * 128, kKp = 2 * kZp;   // a piece of Z or N, of K or Q
+          const uint32_t K = base + L::kOffK, Z = base + L::kOffZ, N = base + L::kOffN;
+          constexpr uint32_t kZp = kChunk * 128, kKp = kChunk * 2 * DKP;   // a piece of Z or N, of K or Q
 #pragma unroll
           for (int w = 1; w >= 0; --w)
 #pragma unroll
@@ -203,11 +246,12 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_tc_kernel(const __grid_c
 #pragma unroll
               for (int k = 0; k < kChunk / 16; ++k) {
                 const uint32_t acc = !(w == 1 && a == 0 && k == 0);
-                const uint64_t ka = across(K + a * kKp, k), qa = across(Q + a * kKp, k);
+                const uint64_t ka = across(K + a * kKp, k), qa = L::kHalf ? ka : across(K + L::kK + a * kKp, k);
+                // across of Z and N: one block of 64 columns, so that the distance between blocks is not used
                 mma_ss(tmem + L::tDQ, ka, along(Z + z * kZp, k), km, acc);
                 mma_ss(tmem + L::tDK, qa, across(Z + z * kZp, k), mn, acc);
-                mma_ss(tmem + L::tDK, ka, along(N + z * kZp, k), km, 1);
-                mma_ss(tmem + L::tDK, ka, across(N + z * kZp, k), mn, 1);
+                mma_ss(tmem + L::tDN, ka, along(N + z * kZp, k), km, L::kHalf ? acc : 1);
+                mma_ss(tmem + L::tDN, ka, across(N + z * kZp, k), mn, 1);
               }
             }
           mma_commit(&bars.done);
@@ -229,8 +273,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_tc_kernel(const __grid_c
     // ---------------- scaling and stores ----------------
     const int q = warp & 3, part = warp >> 2, tb = kTok * part;
     const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16) + tb;
-    const int col = 32 * q + lane;        // q/k column
-    const int row = col & (kChunk - 1);   // token of az (the first half of the lanes) and an
+    // q/k column; kHalf: the upper lanes (K's and dS's products lie in them) hand over what they have of dk
+    const bool upper = L::kHalf && q >= 2;
+    const int col = (32 * q + lane) & (DKP - 1);
+    const int row = (32 * q + lane) & (kChunk - 1);   // token of az (the first half of the lanes) and an
     uint32_t unit = 0;
     bool ok = true;
     for (int64_t i = first; i < items && ok; i = next(i)) {
@@ -269,27 +315,47 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_tc_kernel(const __grid_c
         tc_fence_before();
         warp_arrive(&bars.zn);
         const float4 *gam = reinterpret_cast<const float4*>(gates + tb), *tail = gam + kChunk / 4, *bet = tail + kChunk / 4;
-        ld_cols(tl + L::tA, x);
-        with_tokens(gam, [&](int j, float g) { dq[j] += p.scale * g * x[j]; });
-        ld_cols(tl + L::tA + 64, x);
-        with_tokens(gam, [&](int j, float g) { x[j] *= -g; });
-        ld_cols(tl + L::tU, f);
-        with_tokens(tail, [&](int j, float g) { x[j] += g * f[j]; });
-        with_tokens(bet, [&](int j, float g) { dk[j] += g * x[j]; });
+        float* over = reinterpret_cast<float*>(sm + L::kOffX) + tb * 64 + col;
+        if (!upper) {
+          ld_cols(tl + L::tA, x);
+          with_tokens(gam, [&](int j, float g) { dq[j] += p.scale * g * x[j]; });
+          ld_cols(tl + L::tA + 64, x);
+          with_tokens(gam, [&](int j, float g) { x[j] *= -g; });
+        } else {
+#pragma unroll
+          for (int j = 0; j < kTok; ++j) x[j] = 0.f;
+        }
+        if (!L::kHalf || upper) {
+          ld_cols(tl + L::tU, f);
+          with_tokens(tail, [&](int j, float g) { x[j] += g * f[j]; });
+        }
+        with_tokens(bet, [&](int j, float g) { x[j] *= g; });
         tc_fence_before();
         warp_arrive(&bars.read);
         if (!(ok = warp_wait(&bars.done, unit & 1, abort, err, 98))) break;
         tc_fence_after();
-        ld_cols(tl + L::tDQ, x);
+        if (upper) {
+          ld_cols(tl + L::tDK, f);
 #pragma unroll
-        for (int j = 0; j < kTok; ++j) dq[j] += x[j];
-        ld_cols(tl + L::tDK, x);
+          for (int j = 0; j < kTok; ++j) over[j * 64] = x[j] + f[j];
+          warp_arrive(&bars.over);
+        } else {
+          ld_cols(tl + L::tDN, f);
 #pragma unroll
-        for (int j = 0; j < kTok; ++j) dk[j] += x[j];
+          for (int j = 0; j < kTok; ++j) dk[j] += x[j] + f[j];
+          ld_cols(tl + L::tDQ, x);
+#pragma unroll
+          for (int j = 0; j < kTok; ++j) dq[j] += x[j];
+          if (L::kHalf) {
+            if (!(ok = warp_wait(&bars.over, unit & 1, abort, err, 99))) break;
+#pragma unroll
+            for (int j = 0; j < kTok; ++j) dk[j] += over[j * 64];
+          }
+        }
         tc_fence_before();
       }
       if (!ok) break;
-      if (col < p.dk) {
+      if (!upper && col < p.dk) {
         const Chunk ch = chunk_at(p, c);
         const size_t to = ((size_t)(ch.b * p.time + ch.t0 + tb) * p.hk + hk) * p.dk + col;
         const int64_t stride = (int64_t)p.hk * p.dk;
@@ -308,18 +374,23 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_tc_kernel(const __grid_c
 
 }  // namespace
 
-template <typename T>
-cudaError_t launch_grad_tc(const Params& p, cudaStream_t s) {
-  constexpr int smem = TLayout<T>::kBytes;
+template <int DKP, typename T>
+cudaError_t run_grad_tc(const Params& p, cudaStream_t s) {
+  constexpr int smem = TLayout<DKP, T>::kBytes;
   const double rows = (double)p.bound * kChunk * p.hv;
   int* err = device_error_flag();
   if (err == nullptr) return cudaErrorInvalidValue;
   LaunchTimer t("delta_grad_tc_kernel", s, rows * 4.0 * p.dk * sizeof(T), rows * (6.0 * p.dv + 8.0 * kChunk) * p.dk);
-  cudaError_t e = allow_smem<grad_tc_kernel<T>>(smem);
+  cudaError_t e = allow_smem<grad_tc_kernel<DKP, T>>(smem);
   if (e != cudaSuccess) return e;
   const int64_t items = (int64_t)p.bound * p.hk;
-  grad_tc_kernel<T><<<(unsigned)(items < sm_count() ? items : sm_count()), kGradThreads, smem, s>>>(p, err);
+  grad_tc_kernel<DKP, T><<<(unsigned)(items < sm_count() ? items : sm_count()), kGradThreads, smem, s>>>(p, err);
   return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_grad_tc(const Params& p, cudaStream_t s) {
+  return p.dk <= 64 ? run_grad_tc<64, T>(p, s) : run_grad_tc<128, T>(p, s);
 }
 template cudaError_t launch_grad_tc<__nv_bfloat16>(const Params&, cudaStream_t);
 template cudaError_t launch_grad_tc<__half>(const Params&, cudaStream_t);

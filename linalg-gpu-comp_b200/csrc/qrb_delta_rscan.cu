@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
         staged<T>(stage + L::kOffD, tb, lcol, x);
         with_tokens(gates.gam, [&](int j, float g) { u[j] = x[j] * (p.scale * g); });
         // (for the gradient kernel too, where it takes them as tiles)
-        constexpr int keep = !STATE && grad_on_tc(DKP, sizeof(T) == 2) ? P : 0;
+        constexpr int keep = !STATE && grad_on_tc(sizeof(T) == 2) ? P : 0;
         put_pieces<P, keep>(tl + L::tF + tb / 2, 32, x, p.dop + at * tile_bytes(kTile, P, kChunk), lane, kChunk, tb);
         put_pieces<PS, 0>(tl + L::tO + tb / 2, 32, u);
         tmem_st_wait();

@@ -486,7 +486,8 @@ def test_long_sequence_in_parts():
 # Few heads and long sequences, which run as segments side by side: two segments, many, a last one of one
 # token, several sequences, two blocks of value columns, odd sizes, two segments on two thirds of the SMs.
 LONG = [(1, 600, 1, 1, 64, 64), (1, 4097, 1, 2, 128, 128), (2, 1473, 1, 1, 33, 200), (3, 1025, 2, 4, 64, 31),
-        (1, 3001, 1, 1, 128, 256), (1, 9999, 2, 2, 16, 16), (2, 1050, 16, 32, 32, 40)]
+        (1, 3001, 1, 1, 128, 256), (1, 9999, 2, 2, 16, 16), (2, 1050, 16, 32, 32, 40),
+        (2, 1300, 8, 16, 128, 20)]
 
 
 @gpu
