@@ -5,9 +5,10 @@
 // operands of 128 rows in the layouts they were written in, with value columns (or tokens) along k:
 //     [aq | ay]^T = S0 [dO | du]^T        au^T = dS' e^T        [az ; an] = [dO ; du] e
 //     dq^T = scale gam aq^T + K^T Z^T     dk^T = tail bet au^T - gam bet ay^T + Q^T Z + K^T (N + N^T)
+// with Z, N the masked and decayed az, an.
 // For dk up to 64 the rows are S0's and dS's, K's and Q's side by side: half of what is computed is not
 // read, and the upper half of the lanes hands its part of dk to the lower one through shared memory.
-// with Z, N the masked and decayed az, an.  Two pieces of S0, dS', e, du, Z, N leave 2^-18 of each, far
+// Two pieces of S0, dS', e, du, Z, N leave 2^-18 of each, far
 // below the 16-bit outputs.  A block walks over (chunk, q/k head) pairs: one thread loads value tiles of 32
 // columns into a ring, one issues the products, sixteen warps scale and store, and one warp adds up dg and
 // dbeta.  Heads of a group are added in order, in registers.
