@@ -11,6 +11,7 @@
 // Measured (dk = dv = 128, bf16, 128 blocks at once): 12.3 us a chunk, 336 KB at 3.5 TB/s; the state alone
 // takes 6.3.
 #include "qrb_delta_tc.cuh"
+#include "qrb_ring.cuh"
 
 namespace qrb {
 namespace delta {
@@ -40,7 +41,7 @@ struct RLayout {
 };
 
 struct RBars {
-  uint64_t full[2], sp, dop, ks, pd, f, xf, uw, ds, done, share[4], drain;
+  uint64_t full[2], empty[2], sp, dop, ks, pd, f, xf, uw, ds, share[4], drain;   // full, empty: see qrb_ring.cuh
   uint32_t tmem;
   int abort;
   Span span;   // here, not in registers that the loops need
@@ -52,6 +53,7 @@ static_assert(sizeof(RBars) <= 256, "barrier block");
 template <int DKP, typename T, bool STATE>
 __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_constant__ Params p, int* err) {
   using L = RLayout<DKP, T>;
+  using R = Ring<L::kStages>;
   constexpr int P = L::P, PS = L::PS, PG = L::PG, HK = DKP / kParts;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -70,7 +72,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
     mbar_init(&bars.full[0], 1);
     mbar_init(&bars.full[1], 1);
     for (uint64_t* x : {&bars.ks, &bars.pd, &bars.xf, &bars.ds, &bars.drain}) mbar_init(x, 1);
-    for (uint64_t* x : {&bars.sp, &bars.dop, &bars.f, &bars.uw, &bars.done}) mbar_init(x, kParts * quarters);
+    for (uint64_t* x : {&bars.sp, &bars.dop, &bars.f, &bars.uw, &bars.empty[0], &bars.empty[1]})
+      mbar_init(x, kParts * quarters);
     for (int i = 0; i < 4; ++i) mbar_init(&bars.share[i], kParts);
     bars.abort = 0;
     bars.span = mine;
@@ -87,8 +90,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
     if (lane == 0) {
       int i = 0;
       for (; i < nc; ++i) {
-        const int stage = i % L::kStages, c = nc - 1 - i;
-        if (i >= L::kStages && !mbar_wait_abort(&bars.done, (i - L::kStages) & 1, abort, err, 71)) break;
+        const int stage = R::stage(i), c = nc - 1 - i;
+        if (i >= L::kStages && !mbar_wait_abort(&bars.empty[stage], R::phase(i - L::kStages), abort, err, 71)) break;
         unsigned char* d = sm + stage * L::kStage;
         uint64_t* bar = &bars.full[stage];
         const size_t qk = ((size_t)(slot0 + c) * p.hk + hk) * L::kK, at = slot_head(p, slot0 + c, h);
@@ -110,14 +113,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
       }
       if (*abort)   // loads in flight must land before the block's memory goes
         for (int s = 0; s < L::kStages; ++s)
-          if (i > s) mbar_wait(&bars.full[s], ((i - 1 - s) / L::kStages) & 1, 1u << 22);
+          if (i > s) mbar_wait(&bars.full[s], R::phase(i - 1 - s), 1u << 22);
     }
   } else if (warp == kIssuer) {
     // ---------------- MMAs: one thread ----------------
     if (lane == 0) {
       for (int i = 0; i < nc; ++i) {
-        const uint32_t ph = i & 1, sb = smem_u32(sm + (i % L::kStages) * L::kStage);
-        if (!mbar_wait_abort(&bars.full[i % L::kStages], (i / L::kStages) & 1, abort, err, 72)) break;
+        const uint32_t ph = i & 1, sb = smem_u32(sm + R::stage(i) * L::kStage);
+        if (!mbar_wait_abort(&bars.full[R::stage(i)], R::phase(i), abort, err, 72)) break;
         if (!mbar_wait_abort(&bars.sp, ph, abort, err, 73)) break;
         tc_fence_after();
         mma_pieces<64, DKP, false, PS, P, PS>(tmem + L::tK, tmem + L::tS, DKP / 2, sb, 0);
@@ -181,10 +184,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
         const uint32_t ph = i & 1;
         const int c = nc - 1 - i;
         const size_t at = slot_head(p, slot0 + c, h) * p.nv + tile;
-        const unsigned char* stage = sm + (i % L::kStages) * L::kStage;
-        const Gates gates(sm + L::kOffG + (i % L::kStages) * L::kGates, tb);
+        const unsigned char* stage = sm + R::stage(i) * L::kStage;
+        const Gates gates(sm + L::kOffG + R::stage(i) * L::kGates, tb);
         float x[kTok], u[kTok];
-        if (!warp_wait(&bars.full[i % L::kStages], (i / L::kStages) & 1, abort, err, 81)) break;
+        if (!warp_wait(&bars.full[R::stage(i)], R::phase(i), abort, err, 81)) break;
         staged<T>(stage + L::kOffD, tb, lcol, x);
         with_tokens(gates.gam, [&](int j, float g) { u[j] = x[j] * (p.scale * g); });
         // (for the gradient kernel too, where it takes them as tiles)
@@ -273,7 +276,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rscan_kernel(const __grid_const
           for (int a = 0; a < HK; ++a) st[a] = glast * st[a] + d[a];
         }
         tc_fence_before();
-        warp_arrive(&bars.done);
+        warp_arrive(&bars.empty[R::stage(i)]);
         if (i + 1 < nc) {
           warp_arrive(&bars.share[q]);   // the other quarters' columns are read before pieces go over them
           if (!warp_wait(&bars.share[q], ph, abort, err, 86)) break;

@@ -16,6 +16,7 @@
 // Measured (dk = dv = 128): 5.6 us a chunk in bf16, 24 packed sequences of 16384 tokens with 32 heads 327 us
 // (58 chunks an SM); 7.8 us where it stores for a backward pass, which moves 240 KB a chunk.
 #include "qrb_delta_tc.cuh"
+#include "qrb_ring.cuh"
 
 namespace qrb {
 namespace delta {
@@ -48,7 +49,7 @@ struct ScanLayout {
 };
 
 struct ScanBars {
-  uint64_t full[2], sp, ks, qs, f, xf, uw, sq, ds, pu, o, share[4], drain;
+  uint64_t full[2], empty[2], sp, ks, qs, f, xf, uw, sq, ds, pu, share[4], drain;   // full, empty: see qrb_ring.cuh
   uint32_t tmem;
   int abort;
   Span span;   // here, not in registers that the loops need
@@ -64,6 +65,7 @@ static_assert(sizeof(ScanBars) <= 256, "barrier block");
 template <int DKP, typename T, int PS, int MODE, bool CUT>
 __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_constant__ Params p, int* err) {
   using L = ScanLayout<DKP, T, PS, MODE>;
+  using R = Ring<L::kStages>;
   constexpr bool STORE = MODE == kStore, STATE = MODE == kState;
   constexpr int PG = Pieces<T>::kS;   // pieces of S0 kept for dq and dk
   constexpr int P = L::P, PX = L::PX, HK = DKP / kParts;   // HK: state rows of one thread
@@ -87,7 +89,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
     mbar_init(&bars.full[0], 1);
     mbar_init(&bars.full[1], 1);
     for (uint64_t* x : {&bars.ks, &bars.qs, &bars.xf, &bars.ds, &bars.pu, &bars.drain}) mbar_init(x, 1);
-    for (uint64_t* x : {&bars.sp, &bars.f, &bars.uw, &bars.sq, &bars.o}) mbar_init(x, kParts * quarters);
+    for (uint64_t* x : {&bars.sp, &bars.f, &bars.uw, &bars.sq, &bars.empty[0], &bars.empty[1]})
+      mbar_init(x, kParts * quarters);
     for (int i = 0; i < 4; ++i) mbar_init(&bars.share[i], kParts);
     bars.abort = 0;
     bars.span = mine;
@@ -104,9 +107,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
     if (lane == 0) {
       int c = 0;
       for (; c < nc; ++c) {
-        const int stage = c % L::kStages;
+        const int stage = R::stage(c);
         // the chunk that held this stage is done with: all its products and reads
-        if (c >= L::kStages && !mbar_wait_abort(&bars.o, (c - L::kStages) & 1, abort, err, 51)) break;
+        if (c >= L::kStages && !mbar_wait_abort(&bars.empty[stage], R::phase(c - L::kStages), abort, err, 51)) break;
         unsigned char* d = sm + stage * L::kStage;
         uint64_t* bar = &bars.full[stage];
         const size_t qk = ((size_t)(slot0 + c) * p.hk + hk) * L::kK, at = slot_head(p, slot0 + c, h);
@@ -122,14 +125,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
       }
       if (*abort)   // loads in flight must land before the block's memory goes
         for (int s = 0; s < L::kStages; ++s)
-          if (c > s) mbar_wait(&bars.full[s], ((c - 1 - s) / L::kStages) & 1, 1u << 22);
+          if (c > s) mbar_wait(&bars.full[s], R::phase(c - 1 - s), 1u << 22);
     }
   } else if (warp == kIssuer) {
     // ---------------- MMAs: one thread ----------------
     if (lane == 0) {
       for (int c = 0; c < nc; ++c) {
-        const uint32_t ph = c & 1, sb = smem_u32(sm + (c % L::kStages) * L::kStage);
-        if (!mbar_wait_abort(&bars.full[c % L::kStages], (c / L::kStages) & 1, abort, err, 52)) break;
+        const uint32_t ph = c & 1, sb = smem_u32(sm + R::stage(c) * L::kStage);
+        if (!mbar_wait_abort(&bars.full[R::stage(c)], R::phase(c), abort, err, 52)) break;
         if (!mbar_wait_abort(&bars.sp, ph, abort, err, 53)) break;
         tc_fence_after();
         mma_pieces<64, DKP, false, PS, P, PS>(tmem + L::tK, tmem + L::tS, DKP / 2, sb, 0);
@@ -139,7 +142,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
         mma_pieces<64, 64, false, PX, PX, PX>(tmem + L::tK, tmem + L::tF, 32, sb + L::kOffX, 0);
         mma_commit(&bars.xf);
         if (!STATE) {
-          if (c > 0 && !mbar_wait_abort(&bars.o, ph ^ 1, abort, err, 55)) break;   // the last chunk's o is read
+          // the last chunk's o is read
+          if (c > 0 && !mbar_wait_abort(&bars.empty[R::stage(c - 1)], R::phase(c - 1), abort, err, 55)) break;
           tc_fence_after();
           mma_pieces<64, DKP, false, PS, P, PS>(tmem + L::tQ, tmem + L::tS, DKP / 2, sb + L::kOffQ, 0);
           mma_commit(&bars.qs);
@@ -203,10 +207,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
       if (nc > 0) put_state(0);
       for (int c = 0; c < nc; ++c) {
         const uint32_t ph = c & 1;
-        const unsigned char* stage = sm + (c % L::kStages) * L::kStage;
-        const Gates gates(sm + L::kOffG + (c % L::kStages) * L::kGates, tb);
+        const unsigned char* stage = sm + R::stage(c) * L::kStage;
+        const Gates gates(sm + L::kOffG + R::stage(c) * L::kGates, tb);
         float e[kTok], x[kTok];
-        if (!warp_wait(&bars.full[c % L::kStages], (c / L::kStages) & 1, abort, err, 61)) break;
+        if (!warp_wait(&bars.full[R::stage(c)], R::phase(c), abort, err, 61)) break;
         staged<T>(stage + L::kOffV, tb, lcol, e);
         if (unit) {
 #pragma unroll
@@ -275,7 +279,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scan_kernel(const __grid_consta
         if (STORE) staged<T>(stage + L::kOffD, tb, lcol, e);
         tc_fence_before();
         fence_proxy_async();   // what this stage held is read before bulk copies may replace it
-        warp_arrive(&bars.o);
+        warp_arrive(&bars.empty[R::stage(c)]);
         if (STORE) {
 #pragma unroll
           for (int i = 0; i < kTok; ++i) x[i] *= e[i];
