@@ -17,6 +17,12 @@ inline void check_status(int status) {
   }
 }
 
+// Tells autograd that a caller's tensor was written, so that a backward pass that kept it raises, as after
+// torch's own in-place operations.  (A tensor of inference mode has no version to raise.)
+inline void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void bind_delta(pybind11::module_& m);
 void bind_linear(pybind11::module_& m);
 

@@ -148,6 +148,8 @@ std::tuple<at::Tensor, at::Tensor> forward(const at::Tensor& q, const at::Tensor
   in.a.final_state = s.data_ptr<float>();
   at::Tensor ws = in.workspace(false);
   check_status(qrb_delta_forward(&in.a, ws.data_ptr(), ws.numel(), stream_of(q)));
+  if (out_o.has_value()) written(o);
+  if (out_state.has_value()) written(s);
   return {o, s};
 }
 
@@ -249,6 +251,8 @@ at::Tensor step(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_
   a.slot_stride_out = so.stride(0);
   a.o = o.data_ptr();
   check_status(qrb_delta_step(&a, stream_of(q)));
+  written(so);
+  if (out.has_value()) written(o);
   return o;
 }
 

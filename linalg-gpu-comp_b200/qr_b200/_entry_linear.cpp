@@ -116,6 +116,7 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> forward(const at::Tensor& x, c
   const size_t nb = qrb_linear_workspace_size(&a);
   at::Tensor ws = at::empty({static_cast<int64_t>(nb)}, x.options().dtype(at::kByte));
   check_status(qrb_linear_forward(&a, ws.data_ptr(), nb, stream_of(x)));
+  if (out.has_value()) written(y);
   return {y, pre};
 }
 

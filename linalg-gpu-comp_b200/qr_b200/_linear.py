@@ -2,8 +2,9 @@
 (include/qrb200_nn.h): tensor-core products with everything else in their epilogue.
 
 float32 (with float32 accuracy), bfloat16 and float16; sums are fp32 and each result is rounded
-once.  All work is enqueued on torch's current stream of x's device; inputs are never modified;
-wrong arguments raise TypeError or ValueError before anything is enqueued; results repeat.
+once.  All work is enqueued on torch's current stream of x's device; inputs are not modified, and a
+backward pass that had kept what ``out`` names raises, as after torch's own in-place operations; wrong
+arguments raise TypeError or ValueError before anything is enqueued; results repeat.
 """
 from __future__ import annotations
 

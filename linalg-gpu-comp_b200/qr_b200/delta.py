@@ -10,8 +10,10 @@ Per head a state ``S`` (dk x dv) passes through scaled Householder-like transfor
 ``gated_delta_rule`` runs whole sequences in the chunked compact-WY form blocked QR uses for its
 reflectors, ``gated_delta_rule_backward`` is its gradient, and ``gated_delta_step`` advances one
 token per row for generation.  float32, bfloat16 and float16; states, ``g`` and ``beta`` are
-float32.  All work is enqueued on torch's current stream of the inputs' device; inputs are never
-modified; wrong arguments raise TypeError or ValueError before anything is enqueued.
+float32.  All work is enqueued on torch's current stream of the inputs' device; wrong arguments raise
+TypeError or ValueError before anything is enqueued.  Inputs are not modified, but for the states that
+``gated_delta_step`` advances in place and what ``out`` names; a backward pass that had kept a tensor
+written so raises, as after torch's own in-place operations.
 """
 from __future__ import annotations
 

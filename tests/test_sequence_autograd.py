@@ -1,0 +1,103 @@
+"""What the sequence operators tell autograd: tensors they write, and derivatives they do not have."""
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+MODIFIED = "modified by an inplace operation"
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _built():
+    import build
+    build.build()
+    build.build_entry()
+
+
+def api():
+    import qr_b200
+    return qr_b200
+
+
+def rule_args(device="cuda", time=20):
+    r = lambda *s: torch.randn(*s, device=device)
+    k = torch.nn.functional.normalize(r(2, time, 1, 32), dim=-1)
+    return r(2, time, 1, 32), k, r(2, time, 2, 48), -r(2, time, 2).abs(), r(2, time, 2).sigmoid(), r(2, 2, 32, 48)
+
+
+def token(x):
+    return [t[:, 0].contiguous() for t in x]
+
+
+WRITES = {
+    "step": lambda x, pool: api().gated_delta_step(*token(x), pool),
+    "step into another pool": lambda x, pool: api().gated_delta_step(*token(x), torch.zeros_like(pool), state_out=pool),
+    "final state": lambda x, pool: api().gated_delta_rule(*x, out=(torch.empty_like(x[2]), pool)),
+    "final state over the initial one": lambda x, pool: api().gated_delta_rule(
+        *x, initial_state=pool, out=(torch.empty_like(x[2]), pool)),
+    "step on a view": lambda x, pool: api().gated_delta_step(*[t[:1] for t in token(x)], pool[1:]),
+}
+
+
+@gpu
+@pytest.mark.parametrize("write", WRITES)
+def test_a_state_written_before_the_backward_pass_is_noticed(write):
+    *x, pool = rule_args()
+    leaf = x[2].clone().requires_grad_()
+    o, _ = api().gated_delta_rule(x[0], x[1], leaf, *x[3:], initial_state=pool)
+    version = pool._version
+    with torch.no_grad():
+        WRITES[write](x, pool)
+    assert pool._version > version
+    with pytest.raises(RuntimeError, match=MODIFIED):
+        o.sum().backward()
+
+
+@gpu
+def test_outputs_written_before_the_backward_pass_are_noticed():
+    *x, pool = rule_args()
+    leaf = x[0].clone().requires_grad_()
+    o, _ = api().gated_delta_rule(leaf, *x[1:])
+    with torch.no_grad():
+        api().gated_delta_rule(*(t.clone() for t in x), out=(x[2], torch.empty_like(pool)))
+    with pytest.raises(RuntimeError, match=MODIFIED):
+        o.sum().backward()
+    o, _ = api().gated_delta_rule(leaf, *x[1:])
+    with torch.no_grad():
+        api().gated_delta_step(*(t.clone() for t in token(x)), pool, out=x[2].view(40, 2, 48)[:2])
+    with pytest.raises(RuntimeError, match=MODIFIED):
+        o.sum().backward()
+    a, w, z = torch.randn(6, 16, device="cuda"), torch.randn(8, 16, device="cuda").requires_grad_(), torch.randn(6, 8, device="cuda")
+    y = api().linear(a, w)
+    with torch.no_grad():
+        api().linear(z, torch.randn(16, 8, device="cuda"), out=a)
+    with pytest.raises(RuntimeError, match=MODIFIED):
+        y.sum().backward()
+
+
+@gpu
+def test_inputs_keep_their_versions():
+    *x, pool = rule_args()
+    other = torch.empty_like(pool)
+    a, w = torch.randn(6, 16, device="cuda"), torch.randn(8, 16, device="cuda")
+    read = [*x, pool, a, w]
+    before = [t._version for t in read]
+    api().gated_delta_rule(*x, initial_state=pool, out=(torch.empty_like(x[2]), other))
+    api().gated_delta_rule_backward(x[2], *x, initial_state=pool)
+    api().gated_delta_step(*token(x), pool, state_out=other)
+    api().linear(a, w)
+    api().linear_backward(torch.randn(6, 8, device="cuda"), a, w)
+    assert [t._version for t in read] == before
+    leaf = x[2].clone().requires_grad_()
+    api().gated_delta_rule(x[0], x[1], leaf, *x[3:], initial_state=pool)[0].sum().backward()
+    assert torch.isfinite(leaf.grad).all()
+
+
+@gpu
+def test_states_of_inference_mode_are_written():
+    with torch.inference_mode():
+        *x, pool = rule_args()
+        want = pool.clone()
+        api().gated_delta_step(*token(x), want)
+    with torch.no_grad():
+        api().gated_delta_step(*token(x), pool)
+    assert torch.equal(pool, want)
