@@ -5,6 +5,8 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
+#include <type_traits>
+
 #include "qrb200.h"
 
 namespace qrb_entry {
@@ -15,6 +17,16 @@ inline void check_status(int status) {
     qrb_last_error(buf, sizeof buf);
     TORCH_CHECK(false, "libqrb200 error ", status, ": ", buf);
   }
+}
+
+// These calls have no forward-mode derivative: a result without a tangent would read as one of zero.
+template <typename... T>
+void check_no_tangent(const char* call, const T&... tensors) {
+  auto has = [](const auto& t) {
+    if constexpr (std::is_same_v<std::decay_t<decltype(t)>, at::Tensor>) return t._fw_grad(0).defined();
+    else return t.has_value() && t->_fw_grad(0).defined();
+  };
+  if ((has(tensors) || ...)) TORCH_CHECK_NOT_IMPLEMENTED(false, call, " has no forward-mode derivative");
 }
 
 // Tells autograd that a caller's tensor was written, so that a backward pass that kept it raises, as after

@@ -120,6 +120,7 @@ std::tuple<at::Tensor, at::Tensor> forward(const at::Tensor& q, const at::Tensor
                                            const std::optional<at::Tensor>& seq_offsets,
                                            const std::optional<at::Tensor>& out_o,
                                            const std::optional<at::Tensor>& out_state) {
+  check_no_tangent("gated_delta_rule", q, k, v, g, beta, initial_state, out_o, out_state);
   Inputs in(q, k, v, g, beta, scale, initial_state, seq_offsets);
   if (out_o.has_value()) {
     check_like(*out_o, "out[0]", q, q.scalar_type(), v.sizes());
@@ -157,6 +158,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, std::opti
     const at::Tensor& d_o, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g,
     const at::Tensor& beta, std::optional<double> scale, const std::optional<at::Tensor>& initial_state,
     const std::optional<at::Tensor>& seq_offsets, const std::optional<at::Tensor>& dfinal_state) {
+  check_no_tangent("gated_delta_rule_backward", d_o, q, k, v, g, beta, initial_state, dfinal_state);
   Inputs in(q, k, v, g, beta, scale, initial_state, seq_offsets);
   check_like(d_o, "do", q, q.scalar_type(), v.sizes());
   if (dfinal_state.has_value())
@@ -194,6 +196,7 @@ at::Tensor step(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_
                 const at::Tensor& beta, const at::Tensor& state, std::optional<double> scale,
                 const std::optional<at::Tensor>& slots, const std::optional<at::Tensor>& state_out,
                 const std::optional<at::Tensor>& out) {
+  check_no_tangent("gated_delta_step", q_, k_, v_, g, beta, state, state_out, out);
   qrb_delta_step_args a{};
   a.dtype = dtype_of(q_, "q");
   TORCH_CHECK_VALUE(q_.dim() == 3, "q must have shape (batch, heads, dk) (got ", q_.sizes(), ")");

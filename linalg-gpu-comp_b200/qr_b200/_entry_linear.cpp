@@ -71,6 +71,7 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> forward(const at::Tensor& x, c
                                                           const std::string& activation,
                                                           const std::optional<at::Tensor>& residual, bool want_pre,
                                                           const std::optional<at::Tensor>& out) {
+  check_no_tangent("linear", x, w, bias, residual, out);
   qrb_linear_args a{};
   a.dtype = dtype_of(x);
   a.activation = activation_of(activation);
@@ -123,6 +124,7 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> forward(const at::Tensor& x, c
 std::tuple<std::optional<at::Tensor>, std::optional<at::Tensor>, std::optional<at::Tensor>> backward(
     const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w, const std::string& activation,
     const std::optional<at::Tensor>& pre, bool with_dx, bool with_dw, bool with_bias) {
+  check_no_tangent("linear_backward", dy, x, w, pre);
   qrb_linear_backward_args a{};
   a.dtype = dtype_of(x);
   a.activation = activation_of(activation);

@@ -39,7 +39,8 @@ def linear(x, w, bias=None, *, activation="none", residual=None, return_pre=Fals
     ``return_pre`` also returns ``x w^T + bias`` rounded to the type, which ``linear_backward`` needs for an
     activation.  ``out`` takes the result; it may be ``residual`` itself.  Any strides: rows that are not
     dense are copied, and rows that are not 16-byte aligned are laid out in scratch memory first.
-    Differentiable with respect to x, w, bias and residual.
+    Differentiable with respect to x, w, bias and residual, once; forward-mode tangents are refused
+    (NotImplementedError).
     """
     if _wants_grad(x, w, bias, residual):
         if out is not None or return_pre:

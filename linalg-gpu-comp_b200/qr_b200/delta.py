@@ -72,7 +72,7 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, seq_of
     the last sequence are not read; their o is 0, or with ``out=(o, final_state)`` left as it was.
 
     Differentiable with respect to q, k, v, g, beta and initial_state (autograd calls
-    ``gated_delta_rule_backward``).  A value that is not finite may spoil its sequence from the start of
+    ``gated_delta_rule_backward``, once); forward-mode tangents are refused (NotImplementedError).  A value that is not finite may spoil its sequence from the start of
     its 64-token chunk on.
     """
     if _wants_grad(q, k, v, g, beta, initial_state):

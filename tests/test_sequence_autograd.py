@@ -101,3 +101,46 @@ def test_states_of_inference_mode_are_written():
     with torch.no_grad():
         api().gated_delta_step(*token(x), pool)
     assert torch.equal(pool, want)
+
+
+# ---- forward mode: no derivative, so no result either ----
+def calls(device):
+    *x, pool = rule_args(device)
+    a, w, b, r = (torch.randn(*s, device=device) for s in ((6, 16), (8, 16), (8,), (6, 8)))
+    rule = dict(zip(("q", "k", "v", "g", "beta"), x))
+    return {
+        "gated_delta_rule": dict(rule, initial_state=pool),
+        "gated_delta_rule_backward": dict(rule, do=torch.randn_like(x[2]), initial_state=pool,
+                                          dfinal_state=torch.randn_like(pool)),
+        "gated_delta_step": dict(zip(rule, token(x)), state=pool, state_out=torch.zeros_like(pool)),
+        "linear": dict(x=a, w=w, bias=b, residual=r),
+        "linear_backward": dict(dy=r, x=a, w=w, activation="silu", pre=r.clone()),
+    }
+
+
+def refuse_each_tangent(device, grad):
+    import torch.autograd.forward_ad as ad
+    for name, args in calls(device).items():
+        for which in [n for n, t in args.items() if isinstance(t, torch.Tensor)]:
+            with ad.dual_level(), torch.set_grad_enabled(grad):
+                primal = args[which].clone().requires_grad_(grad)
+                dual = ad.make_dual(primal, torch.ones_like(primal))
+                # with gradients too, torch's own refusal of the recorded function
+                match = "forward" if not grad else None
+                with pytest.raises(RuntimeError if grad else NotImplementedError, match=match):
+                    getattr(api(), name)(**dict(args, **{which: dual}))
+
+
+def test_tangents_are_refused():
+    refuse_each_tangent("cpu", False)
+
+
+@gpu
+def test_tangents_are_refused_on_the_device():
+    refuse_each_tangent("cuda", False)
+    refuse_each_tangent("cuda", True)
+    for name, args in calls("cuda").items():
+        which = "x" if "linear" in name else "q"
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(lambda t: getattr(api(), name)(**dict(args, **{which: t})), (args[which],),
+                           (torch.ones_like(args[which]),))
