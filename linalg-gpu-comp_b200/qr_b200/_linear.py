@@ -42,9 +42,9 @@ def linear(x, w, bias=None, *, activation="none", residual=None, return_pre=Fals
     Differentiable with respect to x, w, bias and residual, once; forward-mode tangents are refused
     (NotImplementedError).
     """
-    if _wants_grad(x, w, bias, residual):
+    if _wants_grad(x, w, bias, residual, out):
         if out is not None or return_pre:
-            raise ValueError("out and return_pre are not supported with inputs that require gradients")
+            raise ValueError("out and return_pre are not supported where out or an input requires gradients")
         _refuse_capture("linear", "linear_backward")
         return _Linear.apply(x, w, bias, residual, activation)
     y, pre = _fast().linear_forward(x, w, bias, activation, residual, return_pre, out)

@@ -75,9 +75,9 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, seq_of
     ``gated_delta_rule_backward``, once); forward-mode tangents are refused (NotImplementedError).  A value that is not finite may spoil its sequence from the start of
     its 64-token chunk on.
     """
+    if out is not None and _wants_grad(q, k, v, g, beta, initial_state, *out):
+        raise ValueError("out is not supported where it or an input requires gradients")
     if _wants_grad(q, k, v, g, beta, initial_state):
-        if out is not None:
-            raise ValueError("out is not supported with inputs that require gradients")
         _refuse_capture("gated_delta_rule", "gated_delta_rule_backward")
         return _GatedDeltaRule.apply(q, k, v, g, beta, initial_state, scale, seq_offsets)
     o, s = (None, None) if out is None else out
@@ -105,7 +105,7 @@ def gated_delta_step(q, k, v, g, beta, state, *, scale=None, slots=None, state_o
     not overlap ``state`` otherwise.  A negative slot marks a padding row: its o is 0.  A slot outside the
     pool, or one that an earlier row holds, is refused: that row's o is NaN and it changes no state.
     """
-    if _wants_grad(q, k, v, g, beta, state):
+    if _wants_grad(q, k, v, g, beta, state, state_out, out):
         raise RuntimeError("gated_delta_step has no gradient: call it under torch.no_grad(), or train with "
                            "gated_delta_rule")
     return _fast().delta_step(q, k, v, g, beta, state, scale, slots, state_out, out)

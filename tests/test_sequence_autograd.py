@@ -144,3 +144,20 @@ def test_tangents_are_refused_on_the_device():
         with pytest.raises(RuntimeError):
             torch.func.jvp(lambda t: getattr(api(), name)(**dict(args, **{which: t})), (args[which],),
                            (torch.ones_like(args[which]),))
+
+
+def test_outputs_that_require_gradients_are_refused():
+    *x, pool = rule_args("cpu")
+    o, s = torch.empty_like(x[2]), torch.empty_like(pool)
+    leaf = lambda t: t.clone().requires_grad_()
+    for out in ((leaf(o), s), (o, leaf(s)), (leaf(o) * 2, s)):
+        with pytest.raises(ValueError, match="requires gradients"):
+            api().gated_delta_rule(*x, out=out)
+    for change in (dict(state_out=leaf(pool)), dict(out=leaf(o[:, 0])), dict(state_out=leaf(pool) * 2)):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            api().gated_delta_step(*token(x), pool, **change)
+    a, w = torch.zeros(6, 16), torch.zeros(8, 16)
+    with pytest.raises(ValueError, match="requires gradients"):
+        api().linear(a, w, out=leaf(torch.zeros(6, 8)))
+    with torch.no_grad(), pytest.raises(ValueError, match="no CPU path"):
+        api().linear(a, w, out=leaf(torch.zeros(6, 8)))
