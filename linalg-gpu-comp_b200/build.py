@@ -85,7 +85,7 @@ def build_entry(force: bool = False, verbose: bool = False) -> Path:
     import torch.utils.cpp_extension as ce
 
     out = _entry_out()
-    deps = [*ENTRY_SRC, PKG / "qr_b200" / "_entry.h", OUT, *INCLUDE.glob("*.h"), Path(__file__)]
+    deps = [*ENTRY_SRC, *(PKG / "qr_b200").glob("*.h"), OUT, *INCLUDE.glob("*.h"), Path(__file__)]
     if not force and out.exists() and all(d.stat().st_mtime <= out.stat().st_mtime for d in deps):
         return out
     cxx = shutil.which("g++") or "c++"

@@ -1,6 +1,7 @@
 // Compiled call path of the linear layer (include/qrb200_nn.h): argument checks with Python's
 // error types, ATen outputs and workspace, torch's current stream of x's device.
 #include "_entry.h"
+#include "_overlap.h"
 
 #include "qrb200_nn.h"
 
@@ -84,6 +85,11 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> forward(const at::Tensor& x, c
     check_like(*out, "out", x, shape);
     TORCH_CHECK_VALUE(out->is_contiguous() || (out->dim() == 2 && out->stride(1) == 1 && out->stride(0) >= n),
                       "out must be contiguous, or a matrix of dense rows");
+    // blocks write rows of the result while others still read these
+    TORCH_CHECK_VALUE(!overlap(*out, x) && !overlap(*out, w) && !(bias.has_value() && overlap(*out, *bias)),
+                      "out must not overlap x, w or bias");
+    TORCH_CHECK_VALUE(!residual.has_value() || same_place(*out, *residual) || !overlap(*out, *residual),
+                      "out may be residual itself, but not overlap it otherwise");
   }
   check_cuda(x);
   c10::cuda::CUDAGuard guard(x.device());
