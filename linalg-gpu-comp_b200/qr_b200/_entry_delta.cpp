@@ -1,6 +1,7 @@
 // Compiled call path of the gated delta rule (include/qrb200_nn.h): argument checks with
 // Python's error types, ATen outputs and workspace, torch's current stream of q's device.
 #include "_entry.h"
+#include "_overlap.h"
 
 #include "qrb200_nn.h"
 
@@ -129,6 +130,22 @@ std::tuple<at::Tensor, at::Tensor> forward(const at::Tensor& q, const at::Tensor
   if (out_state.has_value()) {
     check_like(*out_state, "out[1]", q, at::kFloat, {in.a.nseq, in.a.hv, in.a.dk, in.a.dv});
     TORCH_CHECK_VALUE(out_state->is_contiguous(), "out[1] must be contiguous");
+  }
+  // What the recurrence writes while other blocks read: q, k, v, g and beta are not among it, the kernel before
+  // lays them out.
+  if (out_o.has_value()) {
+    TORCH_CHECK_VALUE(out_o->is_contiguous() || !Runs(*out_o).meets_itself(), "out[0]'s elements must not share memory");
+    TORCH_CHECK_VALUE(!(initial_state.has_value() && overlap(*out_o, *initial_state)) &&
+                          !(seq_offsets.has_value() && overlap(*out_o, *seq_offsets)) &&
+                          !(out_state.has_value() && overlap(*out_o, *out_state)),
+                      "out[0] must not overlap initial_state, seq_offsets or out[1]");
+  }
+  if (out_state.has_value()) {
+    TORCH_CHECK_VALUE(!initial_state.has_value() || same_place(*out_state, *initial_state) ||
+                          !overlap(*out_state, *initial_state),
+                      "out[1] may be initial_state itself, but not overlap it otherwise");
+    TORCH_CHECK_VALUE(!(seq_offsets.has_value() && overlap(*out_state, *seq_offsets)),
+                      "out[1] must not overlap seq_offsets");
   }
   check_cuda(q);
   c10::cuda::CUDAGuard guard(q.device());

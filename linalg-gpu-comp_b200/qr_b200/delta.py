@@ -70,6 +70,8 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, seq_of
     ``seq_offsets`` (sequences + 1, int32 or int64, on the device) packs sequences of different lengths,
     empty ones too, along the time of a batch of one; it starts at 0 and does not decrease.  Rows behind
     the last sequence are not read; their o is 0, or with ``out=(o, final_state)`` left as it was.
+    ``out`` takes the results: final_state may be ``initial_state`` itself, but neither may overlap it otherwise,
+    nor ``seq_offsets`` or one another.
 
     Differentiable with respect to q, k, v, g, beta and initial_state (autograd calls
     ``gated_delta_rule_backward``, once); forward-mode tangents are refused (NotImplementedError).  A value that is not finite may spoil its sequence from the start of

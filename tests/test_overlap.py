@@ -94,3 +94,36 @@ def test_random_views_of_one_buffer():
         with pytest.raises(ValueError, match="must not overlap" if meets else TAKEN):
             api().linear(**a)
     assert yes > 100 and no > 100
+
+
+def rule_case(**change):
+    a = dict(q=torch.zeros(1, 8, 1, 4), k=torch.zeros(1, 8, 1, 4), v=torch.zeros(1, 8, 2, 6), g=torch.zeros(1, 8, 2),
+             beta=torch.zeros(1, 8, 2), initial_state=torch.zeros(2, 2, 4, 6),
+             seq_offsets=torch.tensor([0, 3, 8], dtype=torch.int32))
+    a.update(change)
+    return a
+
+
+def test_rule_out():
+    buf = torch.zeros(1000)
+    o, state = buf[:96].view(1, 8, 2, 6), buf[200:296].view(2, 2, 4, 6)
+
+    def refused(match, out, **change):
+        with pytest.raises(ValueError, match=match):
+            api().gated_delta_rule(**rule_case(**change), out=out)
+
+    refused(TAKEN, (o, state))
+    refused(TAKEN, (o, state), initial_state=state)
+    refused(TAKEN, (o, state), initial_state=buf[296:392].view(2, 2, 4, 6))
+    refused(r"out\[1\] may be initial_state itself", (o, state), initial_state=buf[206:302].view(2, 2, 4, 6))
+    refused(r"out\[0\] must not overlap", (o, state), initial_state=buf[95:191].view(2, 2, 4, 6))
+    refused(r"out\[0\] must not overlap", (o, buf[95:191].view(2, 2, 4, 6)))
+    ints = torch.zeros(100, dtype=torch.int32)
+    f = ints.view(torch.float32)
+    refused(r"out\[0\] must not overlap", (f[:96].view(1, 8, 2, 6), state), seq_offsets=ints[95:98])
+    refused(r"out\[1\] must not overlap seq_offsets", (o, f[:96].view(2, 2, 4, 6)), seq_offsets=ints[93:96])
+    refused(TAKEN, (o, f[:96].view(2, 2, 4, 6)), seq_offsets=ints[96:99])
+    refused("share memory", (torch.zeros(1, 8, 1, 6).expand(1, 8, 2, 6), state))
+    refused("share memory", (buf.as_strided((1, 8, 2, 6), (96, 6, 3, 1)), state))
+    refused(TAKEN, (buf.as_strided((1, 8, 2, 6), (0, 6, 48, 1)), state))          # heads apart, tokens together
+    refused(TAKEN, (buf.as_strided((1, 8, 2, 6), (0, 20, 9, 1)), buf[500:596].view(2, 2, 4, 6)))
