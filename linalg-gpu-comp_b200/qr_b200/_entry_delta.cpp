@@ -135,17 +135,15 @@ std::tuple<at::Tensor, at::Tensor> forward(const at::Tensor& q, const at::Tensor
   // lays them out.
   if (out_o.has_value()) {
     TORCH_CHECK_VALUE(out_o->is_contiguous() || !Runs(*out_o).meets_itself(), "out[0]'s elements must not share memory");
-    TORCH_CHECK_VALUE(!(initial_state.has_value() && overlap(*out_o, *initial_state)) &&
-                          !(seq_offsets.has_value() && overlap(*out_o, *seq_offsets)) &&
-                          !(out_state.has_value() && overlap(*out_o, *out_state)),
+    const Range to(*out_o);
+    TORCH_CHECK_VALUE(!overlap(to, initial_state) && !overlap(to, seq_offsets) && !overlap(to, out_state),
                       "out[0] must not overlap initial_state, seq_offsets or out[1]");
   }
   if (out_state.has_value()) {
     TORCH_CHECK_VALUE(!initial_state.has_value() || same_place(*out_state, *initial_state) ||
                           !overlap(*out_state, *initial_state),
                       "out[1] may be initial_state itself, but not overlap it otherwise");
-    TORCH_CHECK_VALUE(!(seq_offsets.has_value() && overlap(*out_state, *seq_offsets)),
-                      "out[1] must not overlap seq_offsets");
+    TORCH_CHECK_VALUE(!overlap(*out_state, seq_offsets), "out[1] must not overlap seq_offsets");
   }
   check_cuda(q);
   c10::cuda::CUDAGuard guard(q.device());
@@ -236,12 +234,30 @@ at::Tensor step(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_
   if (slots.has_value()) check_like(*slots, "slots", q_, at::kInt, {b});
   else
     TORCH_CHECK_VALUE(state.size(0) >= b, "state must have a slot for each of the ", b, " rows (got ", state.size(0), ")");
+  if (out.has_value()) {
+    check_like(*out, "out", q_, q_.scalar_type(), v_.sizes());
+    TORCH_CHECK_VALUE(out->is_contiguous(), "out must be contiguous");
+  }
+  // What some blocks write while others read: a block reads all of q and k, but of v only what it then writes.
+  const Range to_state(so), read[] = {q_, k_, g, beta, slots}, rv(v_);
+  auto meets = [&](const Range& t) {
+    for (const Range& r : read)
+      if (overlap(t, r)) return true;
+    return false;
+  };
+  TORCH_CHECK_VALUE(&so == &state || same_place(so, state) || !overlap(to_state, state),
+                    "state_out may be state itself, but not overlap it otherwise");
+  TORCH_CHECK_VALUE(!meets(to_state) && !overlap(to_state, rv), "state_out must not overlap q, k, v, g, beta or slots");
+  if (out.has_value()) {
+    const Range to(*out);
+    TORCH_CHECK_VALUE(!meets(to) && !overlap(to, state) && !overlap(to, to_state) &&
+                          (same_place(*out, v_) || !overlap(to, rv)),
+                      "out must not overlap q, k, g, beta, slots, state or state_out, nor v unless it is v itself");
+  }
   check_cuda(q_);
   c10::cuda::CUDAGuard guard(q_.device());
   at::Tensor q = dense_last(q_), k = dense_last(k_), v = dense_last(v_), o, sl;
   if (out.has_value()) {
-    check_like(*out, "out", q_, q_.scalar_type(), v_.sizes());
-    TORCH_CHECK_VALUE(out->is_contiguous(), "out must be contiguous");
     o = *out;
   } else {
     o = at::empty(v_.sizes(), v_.options());

@@ -86,9 +86,10 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> forward(const at::Tensor& x, c
     TORCH_CHECK_VALUE(out->is_contiguous() || (out->dim() == 2 && out->stride(1) == 1 && out->stride(0) >= n),
                       "out must be contiguous, or a matrix of dense rows");
     // blocks write rows of the result while others still read these
-    TORCH_CHECK_VALUE(!overlap(*out, x) && !overlap(*out, w) && !(bias.has_value() && overlap(*out, *bias)),
+    const Range to(*out);
+    TORCH_CHECK_VALUE(!overlap(to, x) && !overlap(to, w) && !overlap(to, bias),
                       "out must not overlap x, w or bias");
-    TORCH_CHECK_VALUE(!residual.has_value() || same_place(*out, *residual) || !overlap(*out, *residual),
+    TORCH_CHECK_VALUE(!residual.has_value() || same_place(*out, *residual) || !overlap(to, *residual),
                       "out may be residual itself, but not overlap it otherwise");
   }
   check_cuda(x);

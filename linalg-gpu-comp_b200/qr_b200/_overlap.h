@@ -8,13 +8,14 @@
 #include <ATen/ATen.h>
 
 #include <algorithm>
+#include <optional>
 #include <vector>
 
 namespace qrb_entry {
 
 class Runs {
  public:
-  explicit Runs(const at::Tensor& t) : base_(reinterpret_cast<intptr_t>(t.data_ptr())), length_(t.element_size()) {
+  explicit Runs(const at::Tensor& t) : base_(reinterpret_cast<intptr_t>(t.const_data_ptr())), length_(t.element_size()) {
     empty_ = t.numel() == 0;
     for (int64_t i = 0; i < t.dim(); ++i) {
       if (t.size(i) <= 1) continue;
@@ -92,22 +93,32 @@ class Runs {
   }
 };
 
-// Bytes from the first element to behind the last.
-inline int64_t extent(const at::Tensor& t) {
-  int64_t n = 1;
-  for (int64_t i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
-  return t.numel() == 0 ? 0 : n * static_cast<int64_t>(t.element_size());
-}
+// A tensor and the bytes from its first element to behind its last, taken once for several comparisons.
+struct Range {
+  const at::Tensor* t = nullptr;
+  intptr_t lo = 0, hi = 0;
+  Range(const at::Tensor& x) : t(&x) {
+    const auto sizes = x.sizes(), strides = x.strides();
+    int64_t n = 1;
+    for (size_t i = 0; i < sizes.size(); ++i) {
+      if (sizes[i] == 0) return;
+      n += (sizes[i] - 1) * strides[i];
+    }
+    lo = reinterpret_cast<intptr_t>(x.const_data_ptr());
+    hi = lo + n * static_cast<int64_t>(x.element_size());
+  }
+  Range(const std::optional<at::Tensor>& x) {
+    if (x.has_value()) *this = Range(*x);
+  }
+};
 
-inline bool overlap(const at::Tensor& a, const at::Tensor& b) {
-  const auto p = reinterpret_cast<intptr_t>(a.data_ptr()), q = reinterpret_cast<intptr_t>(b.data_ptr());
-  if (p + extent(a) <= q || q + extent(b) <= p) return false;   // nearly always
-  return Runs(a).meets(Runs(b));
+inline bool overlap(const Range& a, const Range& b) {
+  return a.lo < b.hi && b.lo < a.hi && Runs(*a.t).meets(Runs(*b.t));
 }
 
 // Both name the same elements at the same places.
 inline bool same_place(const at::Tensor& a, const at::Tensor& b) {
-  if (a.data_ptr() != b.data_ptr() || a.scalar_type() != b.scalar_type() || a.sizes() != b.sizes()) return false;
+  if (a.const_data_ptr() != b.const_data_ptr() || a.scalar_type() != b.scalar_type() || a.sizes() != b.sizes()) return false;
   for (int64_t i = 0; i < a.dim(); ++i)
     if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
   return true;

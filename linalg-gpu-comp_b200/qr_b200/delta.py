@@ -104,7 +104,8 @@ def gated_delta_step(q, k, v, g, beta, state, *, scale=None, slots=None, state_o
 
     Row i advances state ``slots[i]`` (int32 on the device; default i) in place, or from ``state`` into the
     same slot of ``state_out``, which may be another pool (other slots of it are left as they are) but must
-    not overlap ``state`` otherwise.  A negative slot marks a padding row: its o is 0.  A slot outside the
+    not overlap ``state`` otherwise.  ``out`` takes o; neither may overlap an input, but out may be ``v``
+    itself.  A negative slot marks a padding row: its o is 0.  A slot outside the
     pool, or one that an earlier row holds, is refused: that row's o is NaN and it changes no state.
     """
     if _wants_grad(q, k, v, g, beta, state, state_out, out):

@@ -127,3 +127,71 @@ def test_rule_out():
     refused("share memory", (buf.as_strided((1, 8, 2, 6), (96, 6, 3, 1)), state))
     refused(TAKEN, (buf.as_strided((1, 8, 2, 6), (0, 6, 48, 1)), state))          # heads apart, tokens together
     refused(TAKEN, (buf.as_strided((1, 8, 2, 6), (0, 20, 9, 1)), buf[500:596].view(2, 2, 4, 6)))
+
+
+def step_case(**change):
+    a = dict(q=torch.zeros(2, 1, 4), k=torch.zeros(2, 1, 4), v=torch.zeros(2, 2, 6), g=torch.zeros(2, 2),
+             beta=torch.zeros(2, 2), state=torch.zeros(3, 2, 4, 6))
+    a.update(change)
+    return a
+
+
+def test_step_state_out_and_out():
+    def refused(match, **change):
+        with pytest.raises(ValueError, match=match):
+            api().gated_delta_step(**step_case(**change))
+
+    buf = torch.zeros(3000)
+    pool = buf[:144].view(3, 2, 4, 6)
+    refused(TAKEN, state=pool, state_out=pool)
+    refused(TAKEN, state=pool, state_out=buf[:144].view(3, 2, 4, 6))
+    refused(TAKEN, state=pool, state_out=buf[144:288].view(3, 2, 4, 6))
+    refused("state itself", state=pool, state_out=buf[48:192].view(3, 2, 4, 6))       # one slot further
+    refused("state itself", state=pool, state_out=buf[1:145].view(3, 2, 4, 6))
+    both = buf[:288].view(3, 2, 2, 4, 6)                                              # two pools, slot by slot
+    refused(TAKEN, state=both[:, 0], state_out=both[:, 1])
+    refused("state itself", state=both[:, 0], state_out=buf[47:47 + 288].view(3, 2, 2, 4, 6)[:, 0])
+    for name, shape in dict(q=(2, 1, 4), k=(2, 1, 4), v=(2, 2, 6), g=(2, 2), beta=(2, 2)).items():
+        n = torch.Size(shape).numel()
+        refused("state_out must not overlap", state=pool, **{name: buf[140:140 + n].view(shape)})
+        refused("state_out must not overlap", state_out=pool, **{name: buf[140:140 + n].view(shape)})
+        refused(TAKEN, state=pool, **{name: buf[144:144 + n].view(shape)})
+        out = buf[500:524].view(2, 2, 6)
+        refused("out must not overlap", out=out, **{name: buf[523:523 + n].view(shape)})
+        refused(TAKEN, out=out, **{name: buf[524:524 + n].view(shape)})
+    refused("out must not overlap", out=buf[140:164].view(2, 2, 6), state=pool)
+    refused("out must not overlap", out=buf[140:164].view(2, 2, 6), state_out=pool)
+    refused(TAKEN, out=out, v=out)
+    ints = torch.zeros(24, dtype=torch.int32)
+    refused("out must not overlap", out=ints.view(torch.float32).view(2, 2, 6), slots=ints[22:])
+
+
+@gpu
+def test_step_out_over_v():
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    r = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    for dtype in (torch.bfloat16, torch.float32):
+        q, k, v = r(5, 2, 64).to(dtype), r(5, 2, 64).to(dtype), r(5, 4, 100).to(dtype)
+        g, beta, state = -r(5, 4).abs(), r(5, 4).sigmoid(), r(5, 4, 64, 100)
+        kept = torch.empty_like(state)
+        want = api().gated_delta_step(q, k, v, g, beta, state, state_out=kept)
+        assert api().gated_delta_step(q, k, v, g, beta, state, out=v).data_ptr() == v.data_ptr()
+        assert torch.equal(v, want) and torch.equal(state, kept)
+
+
+@gpu
+def test_outputs_beside_inputs():
+    """Results in slices of the buffers that the inputs lie in."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    wide = torch.randn(300, 200, generator=gen, device="cuda").bfloat16()
+    w = torch.randn(64, 96, generator=gen, device="cuda").bfloat16()
+    want, x = api().linear(wide[:, :96].contiguous(), w), wide[:, :96].clone()
+    assert torch.equal(api().linear(wide[:, :96], w, out=wide[:, 96:160]), want) and torch.equal(wide[:, :96], x)
+    pools = torch.randn(4, 2, 2, 32, 32, generator=gen, device="cuda")
+    tok = [torch.randn(4, 2, 32, generator=gen, device="cuda") for _ in range(3)]
+    g, beta = torch.full((4, 2), -0.5, device="cuda"), torch.full((4, 2), 0.5, device="cuda")
+    old = pools[:, 0].clone()
+    dense = old.clone()
+    want = api().gated_delta_step(*tok, g, beta, dense)
+    assert torch.equal(api().gated_delta_step(*tok, g, beta, pools[:, 0], state_out=pools[:, 1]), want)
+    assert torch.equal(pools[:, 1], dense) and torch.equal(pools[:, 0], old)
