@@ -41,8 +41,9 @@ typedef struct {
  * Forward:  q, k, v, g, beta, initial_state (NULL: zeros) -> o, final_state (NULL: not stored).
  * Backward: also d_o and dfinal_state (NULL: zeros) -> dq, dk_, dv_, dg, dbeta (dense, shaped like
  * q, k, v, g, beta) and dinitial_state (NULL: not stored).  States are dense fp32
- * (nseq, hv, dk, dv); final_state may be initial_state.  A value that is not finite may spoil
- * every output of its sequence from the start of its 64-token chunk. */
+ * (nseq, hv, dk, dv); final_state may be initial_state.  A value that is not finite (a
+ * state, u or an fp32 input above 3.38e38 counts as one) may spoil every output of its sequence from the start
+ * of its 64-token chunk, and every gradient of its sequence. */
 typedef struct {
   int dtype;                       /* qrb_dtype of q, k, v, o and their gradients */
   int hk, hv, dk, dv;
@@ -95,7 +96,7 @@ QRB_API int qrb_delta_step(const qrb_delta_step_args* a, void* stream);
 /* The linear layer y = act(x w^T + bias) + residual: x (m x k), w (n x k), y (m x n), row-major with
  * row strides ldx, ldw, ... in elements, all of one dtype; fp32 accumulation, rounded once.  bias (n),
  * residual and pre (m x n) may be NULL; pre receives x w^T + bias, rounded, for the backward pass.
- * fp32 products carry fp32 accuracy (three bf16 planes per operand).  Results repeat.  y may be
+ * fp32 products carry fp32 accuracy (three bf16 planes per operand; below 2^-109 the last ones underflow).  Results repeat.  y may be
  * residual (same rows); it must not alias x, w or bias.  The workspace size depends on the pointers'
  * alignment as well as on the sizes. */
 typedef struct {

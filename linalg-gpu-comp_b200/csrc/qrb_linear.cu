@@ -53,6 +53,8 @@ __device__ __forceinline__ void put8f(void* to, int64_t i, int64_t plane, const 
       for (int h = 0; h < 2; ++h) {
         const float x = j + h < count ? e[j + h] : 0.f;
         pc[0][h] = __float2bfloat16_rn(x);
+        // the last half step below fp32's largest value would round to infinity: down, the rest follows
+        if (__hisinf(pc[0][h]) && fabsf(x) <= 3.402823466e38f) pc[0][h] = __float2bfloat16_rz(x);
         float r = x - __bfloat162float(pc[0][h]);
         if (!(fabsf(r) <= 3.4e38f)) r = 0.f;
         pc[1][h] = __float2bfloat16_rn(r);
