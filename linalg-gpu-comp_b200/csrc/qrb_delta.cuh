@@ -116,7 +116,6 @@ constexpr int kChainPieces = 3;  // of X, F and W
 // states' third pieces are then kept and read half as often; at every eighth dg was 1.8e-6 off.
 constexpr int kAnchor = 2;
 
-
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
@@ -146,10 +145,6 @@ __device__ __forceinline__ uint32_t tile_off(int rows, int row, int col) {
 __device__ __forceinline__ uint32_t unit_off(int rows, int row, int col) {
   return (uint32_t)((col >> 3) * rows * 16 + row * 16 + ((col & 7) << 1));
 }
-template <bool U>
-__device__ __forceinline__ uint32_t any_off(int rows, int row, int col) {
-  return U ? unit_off(rows, row, col) : tile_off(rows, row, col);
-}
 
 __device__ __forceinline__ uint32_t pack2(__nv_bfloat16 a, __nv_bfloat16 b) {
   return (uint32_t)__bfloat16_as_ushort(a) | ((uint32_t)__bfloat16_as_ushort(b) << 16);
@@ -174,18 +169,6 @@ __device__ __forceinline__ void put2(unsigned char* tile, int rows, int pcols, i
   }
 }
 
-template <int P>
-__device__ __forceinline__ float2 get2(const unsigned char* tile, int rows, int pcols, int row, int col) {
-  float2 r = make_float2(0.f, 0.f);
-#pragma unroll
-  for (int p = P - 1; p >= 0; --p) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + tile_off(rows, row, p * pcols + col));
-    r.x += __uint_as_float(w << 16);
-    r.y += __uint_as_float(w & 0xffff0000u);
-  }
-  return r;
-}
-
 __device__ __forceinline__ uint32_t s_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -208,13 +191,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// acc (16 x 8 NT) += A[m0 .. m0+15][k0 .. k1) B[k0 .. k1)[n0 .. n0 + 8 NT).
-// AT: A is stored with k along the rows; BT: B is stored with k along the rows (otherwise n).
-// AU / BU: A / B is a tile of the recurrences (unit_off).
-// PA / PB pieces lie apc / bpc columns apart; products of pieces i + j >= PM are dropped
-// (PM is the piece count of the fp32 operands: what is dropped is below their own rounding).
-// One warp; k0, k1 multiples of 16, NT even.  Fragment layout of m16n8k16: lane 4 g + t holds
-// rows g and g + 8, columns 2 t and 2 t + 1 of each 16 x 8 block of acc.
 // A lane's ldmatrix address is a constant part and a part that the step of k (or the piece and the column
 // group) moves: 16-byte units of a swizzled row are XORed, everything else is added.
 template <bool U>
@@ -231,6 +207,13 @@ struct LaneAddr {
   }
 };
 
+// acc (16 x 8 NT) += A[m0 .. m0+15][k0 .. k1) B[k0 .. k1)[n0 .. n0 + 8 NT).
+// AT: A is stored with k along the rows; BT: B is stored with k along the rows (otherwise n).
+// AU / BU: A / B is a tile of the recurrences (unit_off).
+// PA / PB pieces lie apc / bpc columns apart; products of pieces i + j >= PM are dropped
+// (PM is the piece count of the fp32 operands: what is dropped is below their own rounding).
+// One warp; k0, k1 multiples of 16, NT even.  Fragment layout of m16n8k16: lane 4 g + t holds
+// rows g and g + 8, columns 2 t and 2 t + 1 of each 16 x 8 block of acc.
 template <int NT, bool AT, bool BT, int PA, int PB, int PM, bool AU = false, bool BU = false>
 __device__ __forceinline__ void mma_tile(float (&acc)[NT][4], const unsigned char* A, int arows, int apc, int m0,
                                          const unsigned char* B, int brows, int bpc, int n0, int k0, int k1) {

@@ -9,10 +9,9 @@
 //   * Large outputs: pairs of blocks (cta_group::2) on 256 x 256 tiles, each block loading 128 rows of
 //     A and 128 of B: 32 KB per 512 cycles of MMAs.  One block on 128 x 256 needs 48 KB for the same
 //     time, more than L2 delivers to every SM at once (4096 x 2048 x 8192 took twice its MMA time).
-//   * Smaller ones: single blocks on 128 x 256, 128 or 64 tiles.
-//
+//   * Smaller ones: single blocks on 128 x 128 or 64 tiles.
 //   * Few rows (m <= 128): the operands change places, so the 128-row side of the MMA is the weight
-//     and its 16 .. 128 column side the rows: no tensor-core row is wasted on padding, and the
+//     and its 64 or 128 column side the rows: no tensor-core row is wasted on padding, and the
 //     weight streams through once.
 //   * Few tiles: the blocks divide k; fp32 partials are added in order by reduce_kernel, which
 //     then runs the epilogue, so results repeat.
@@ -61,7 +60,7 @@ struct Cfg {
   static constexpr int kRowsB = PAIR ? BN / 2 : BN;   // rows of B this block loads
   static constexpr uint32_t kA = kBM * kBK * 2, kB = kRowsB * kBK * 2, kStage = kA + kB;
   static constexpr uint32_t kTurn = 8 * 32 * 33 * 4;   // a 32 x 32 tile for each epilogue warp to turn
-  static constexpr int kStages = kStage > 40960 ? 3 : (kStage > 24576 ? 5 : 6);
+  static constexpr int kStages = kStage > 24576 ? 5 : 6;
   static constexpr uint32_t kBar = kStages * kStage;
   static constexpr uint32_t kOffTurn = kBar + 256;
   static constexpr uint32_t kSmem = kOffTurn + kTurn + 1024;
@@ -527,8 +526,10 @@ struct Plan {
 
 // Tile shape and split of an m x n x k product.  Up to 128 rows: swapped, the narrowest tile that
 // holds them.  Otherwise pairs on 256 x 256 where these fill two thirds of the SMs (or nearly: the
-// last, partly filled wave counts), then the widest single tile that does (a wide tile reads the least
-// shared memory per MMA, an idle SM costs more), and where even 64 columns do not, k is split.
+// last, partly filled wave counts), else single blocks on 128 x 128 where these do (a wide tile reads the
+// least shared memory per MMA, an idle SM costs more), else on 128 x 64; where even those leave half of the
+// SMs idle, k is split.  (Blocks on 128 x 256 are at most twice the pairs, so they never fill two thirds
+// where pairs do not fill one.)
 Plan plan(int64_t m, int64_t n, int64_t k, int pieces) {
   Plan p{};
   const int sms = sm_count();
@@ -546,8 +547,7 @@ Plan plan(int64_t m, int64_t n, int64_t k, int pieces) {
     t = tiles(m <= 64 ? 64 : 128, 0);
   } else {
     t = tiles(256, 1);
-    if (t * 3 < sms) t = tiles(256, 0);
-    if (!p.pair && t * 3 < sms * 2) t = tiles(128, 0);
+    if (t * 3 < sms) t = tiles(128, 0);
     if (!p.pair && t * 3 < sms * 2) t = tiles(64, 0);
   }
   // a split is worth at least four stages of work, and there are 16 at most
@@ -595,8 +595,6 @@ size_t scratch(int64_t m, int64_t n, int64_t k, int pieces) {
   return p.splits > 1 ? (size_t)p.splits * m * n : 0;
 }
 
-int launches(int64_t m, int64_t n, int64_t k, int pieces) { return plan(m, n, k, pieces).splits > 1 ? 2 : 1; }
-
 cudaError_t multiply(const Operand& A, const Operand& B, int64_t m, int64_t n, int64_t k, bool half, const Epilogue& e,
                      float* ws, cudaStream_t s) {
   const Plan p = plan(m, n, k, A.pieces);
@@ -642,8 +640,7 @@ cudaError_t multiply(const Operand& A, const Operand& B, int64_t m, int64_t n, i
     LaunchTimer t("linear_gemm_kernel", s, bytes, 2.0 * m * n * k);
     if (p.pair) r = run<256, true>(ma, mb, g, s);
     else if (p.bn == 64) r = run<64, false>(ma, mb, g, s);
-    else if (p.bn == 128) r = run<128, false>(ma, mb, g, s);
-    else r = run<256, false>(ma, mb, g, s);
+    else r = run<128, false>(ma, mb, g, s);
   }
   if (r != cudaSuccess || p.splits == 1) return r;
   LaunchTimer t("linear_reduce_kernel", s, 4.0 * p.splits * m * n, (double)p.splits * m * n);

@@ -14,7 +14,7 @@ namespace gemm {
 
 // A matrix of `mn` output rows (or columns) by k, bf16 or fp16, 16-byte aligned rows of `ld`
 // elements: k along the rows of memory, or with mn_major mn along them.  `pieces` planes of
-// `plane` elements each (fp32 operands are three bf16 planes, see split_kernel).
+// `plane` elements each (fp32 operands are three bf16 planes, laid out by put8f in qrb_linear.cu).
 struct Operand {
   const void* p;
   int64_t ld, plane;
@@ -39,7 +39,6 @@ size_t scratch(int64_t m, int64_t n, int64_t k, int pieces);
 // y (m x n) = epilogue(A (m x k) B (n x k)^T).
 cudaError_t multiply(const Operand& A, const Operand& B, int64_t m, int64_t n, int64_t k, bool half, const Epilogue& e,
                      float* ws, cudaStream_t s);
-int launches(int64_t m, int64_t n, int64_t k, int pieces);
 bool supported();   // the driver's tensor map encoder is there
 
 __device__ __forceinline__ float load1(const void* p, int64_t i, int dtype) {
