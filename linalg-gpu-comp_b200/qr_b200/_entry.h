@@ -29,6 +29,16 @@ void check_no_tangent(const char* call, const T&... tensors) {
   if ((has(tensors) || ...)) TORCH_CHECK_NOT_IMPLEMENTED(false, call, " has no forward-mode derivative");
 }
 
+// Whether autograd would record a function of these tensors.
+template <typename... T>
+bool wants_grad(const T&... tensors) {
+  auto one = [](const auto& t) {
+    if constexpr (std::is_same_v<std::decay_t<decltype(t)>, at::Tensor>) return t.requires_grad();
+    else return t.has_value() && t->requires_grad();
+  };
+  return at::GradMode::is_enabled() && (one(tensors) || ...);
+}
+
 // Tells autograd that a caller's tensor was written, so that a backward pass that kept it raises, as after
 // torch's own in-place operations.  (A tensor of inference mode has no version to raise.)
 inline void written(const at::Tensor& t) {

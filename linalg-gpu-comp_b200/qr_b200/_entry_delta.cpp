@@ -211,6 +211,8 @@ at::Tensor step(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_
                 const at::Tensor& beta, const at::Tensor& state, std::optional<double> scale,
                 const std::optional<at::Tensor>& slots, const std::optional<at::Tensor>& state_out,
                 const std::optional<at::Tensor>& out) {
+  TORCH_CHECK(!wants_grad(q_, k_, v_, g, beta, state, state_out, out),
+              "gated_delta_step has no gradient: call it under torch.no_grad(), or train with gated_delta_rule");
   check_no_tangent("gated_delta_step", q_, k_, v_, g, beta, state, state_out, out);
   qrb_delta_step_args a{};
   a.dtype = dtype_of(q_, "q");

@@ -108,7 +108,4 @@ def gated_delta_step(q, k, v, g, beta, state, *, scale=None, slots=None, state_o
     itself.  A negative slot marks a padding row: its o is 0.  A slot outside the
     pool, or one that an earlier row holds, is refused: that row's o is NaN and it changes no state.
     """
-    if _wants_grad(q, k, v, g, beta, state, state_out, out):
-        raise RuntimeError("gated_delta_step has no gradient: call it under torch.no_grad(), or train with "
-                           "gated_delta_rule")
     return _fast().delta_step(q, k, v, g, beta, state, scale, slots, state_out, out)
