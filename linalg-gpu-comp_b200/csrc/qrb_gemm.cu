@@ -15,6 +15,10 @@
 //     weight streams through once.
 //   * Few tiles: the blocks divide k; fp32 partials are added in order by reduce_kernel, which
 //     then runs the epilogue, so results repeat.
+//   * Long k: the tensor cores' accumulation truncates, one-sidedly, so its bias grows with the number of
+//     additions (16 products each): 1.0e-7 of a sum of one sign each, 6.7e-3 of one of 2^20 rows, where
+//     rounding to bf16 is at most 3.9e-3 off.  k is cut, as for few tiles, where that bias would pass a
+//     half of the output's rounding.
 //   * fp32: three bf16 planes per operand, x = x0 + x1 + x2 to 2^-27; the six products x_i w_j with
 //     i + j < 3.  The five small ones have an accumulator of their own, and k is cut at 512 (fp32
 //     partials beyond): the tensor cores' accumulation truncates, and its bias grows with the
@@ -39,7 +43,9 @@ using namespace sm100;
 
 constexpr int kBM = 128, kBK = 64, kThreads = 384;   // warps: producer, MMA, 2 idle, 8 epilogue
 constexpr int kMaxTerms = 6;
-constexpr int64_t kMaxSplitK32 = 512;    // longest k of one fp32 accumulation
+// Longest k of one accumulation.  fp32: see the head of this file.  16 bits: 2^18 / 16 additions leave up to
+// 1.7e-3, less than half of bf16's eps / 2 = 3.9e-3; 2^15 / 16 leave 2.1e-4 of fp16's 4.9e-4.
+constexpr int64_t kMaxSplitK32 = 512, kMaxSplitBf16 = 1 << 18, kMaxSplitF16 = 1 << 15;
 
 struct GemmArgs {
   int64_t M, N;                 // MMA orientation: A's rows, B's rows
@@ -530,7 +536,7 @@ struct Plan {
 // least shared memory per MMA, an idle SM costs more), else on 128 x 64; where even those leave half of the
 // SMs idle, k is split.  (Blocks on 128 x 256 are at most twice the pairs, so they never fill two thirds
 // where pairs do not fill one.)
-Plan plan(int64_t m, int64_t n, int64_t k, int pieces) {
+Plan plan(int64_t m, int64_t n, int64_t k, int pieces, bool half) {
   Plan p{};
   const int sms = sm_count();
   p.kblocks = (int)((k + kBK - 1) / kBK);
@@ -555,10 +561,9 @@ Plan plan(int64_t m, int64_t n, int64_t k, int pieces) {
   if (splits > (p.kblocks + 3) / 4) splits = (p.kblocks + 3) / 4;
   if (splits > 16) splits = 16;
   if (splits < 1) splits = 1;
-  if (pieces > 1) {
-    const int64_t need = (p.kblocks + kMaxSplitK32 / kBK - 1) / (kMaxSplitK32 / kBK);
-    if (splits < need) splits = need;
-  }
+  const int64_t longest = (pieces > 1 ? kMaxSplitK32 : half ? kMaxSplitF16 : kMaxSplitBf16) / kBK;
+  const int64_t need = (p.kblocks + longest - 1) / longest;
+  if (splits < need) splits = need;
   p.per_split = (int)((p.kblocks + splits - 1) / splits);
   p.splits = (p.kblocks + p.per_split - 1) / p.per_split;
   return p;
@@ -589,15 +594,15 @@ cudaError_t run(const CUtensorMap& ma, const CUtensorMap& mb, const GemmArgs& g,
 
 bool supported() { return encoder() != nullptr; }
 
-size_t scratch(int64_t m, int64_t n, int64_t k, int pieces) {
+size_t scratch(int64_t m, int64_t n, int64_t k, int pieces, bool half) {
   if (m < 1 || n < 1 || k < 1) return 0;
-  const Plan p = plan(m, n, k, pieces);
+  const Plan p = plan(m, n, k, pieces, half);
   return p.splits > 1 ? (size_t)p.splits * m * n : 0;
 }
 
 cudaError_t multiply(const Operand& A, const Operand& B, int64_t m, int64_t n, int64_t k, bool half, const Epilogue& e,
                      float* ws, cudaStream_t s) {
-  const Plan p = plan(m, n, k, A.pieces);
+  const Plan p = plan(m, n, k, A.pieces, half);
   GemmArgs g{};
   const Operand &a = p.swap ? B : A, &b = p.swap ? A : B;
   g.M = p.swap ? n : m;

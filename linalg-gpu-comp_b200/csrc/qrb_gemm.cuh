@@ -35,7 +35,7 @@ struct Epilogue {
 };
 
 // fp32 scratch elements of multiply() (0 when the product is not split along k).
-size_t scratch(int64_t m, int64_t n, int64_t k, int pieces);
+size_t scratch(int64_t m, int64_t n, int64_t k, int pieces, bool half);
 // y (m x n) = epilogue(A (m x k) B (n x k)^T).
 cudaError_t multiply(const Operand& A, const Operand& B, int64_t m, int64_t n, int64_t k, bool half, const Epilogue& e,
                      float* ws, cudaStream_t s);

@@ -442,7 +442,7 @@ FwdLayout fwd_layout(const qrb_linear_args& a) {
   l.w = at;
   if (!direct(a.dtype, a.w, a.ldw, a.k)) at += layout_bytes(a.dtype, a.n, a.k);
   l.part = at;
-  at += al(qrb::gemm::scratch(a.m, a.n, a.k, a.dtype == QRB_F32 ? 3 : 1) * 4);
+  at += al(qrb::gemm::scratch(a.m, a.n, a.k, a.dtype == QRB_F32 ? 3 : 1, a.dtype == QRB_F16) * 4);
   l.total = at;
   return l;
 }
@@ -474,7 +474,8 @@ BwdLayout bwd_layout(const qrb_linear_backward_args& a) {
   l.sums = at;
   at += al((size_t)((a.m + qrb::gemm::kSumRows - 1) / qrb::gemm::kSumRows) * a.n * 4);
   l.part = at;
-  size_t p1 = qrb::gemm::scratch(a.m, a.k, a.n, pieces), p2 = qrb::gemm::scratch(a.n, a.k, a.m, pieces);
+  const bool half = a.dtype == QRB_F16;
+  const size_t p1 = qrb::gemm::scratch(a.m, a.k, a.n, pieces, half), p2 = qrb::gemm::scratch(a.n, a.k, a.m, pieces, half);
   at += al((p1 > p2 ? p1 : p2) * 4);
   l.total = at;
   return l;

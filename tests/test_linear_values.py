@@ -47,3 +47,22 @@ def test_largest_values(m):
     x[0, 4] = math.inf                                                # which stays what it is
     y = api().linear(x, w.abs())
     assert (y[0] == math.inf).all() and torch.isfinite(y[1:]).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype,m", [(HF, 2 ** 18), (BF, 2 ** 20)])
+def test_sums_over_many_rows(dtype, m):
+    """dw of many rows, of one sign each, where every SM has a tile of its own and nothing else cuts the sum.  The
+    tensor cores' additions truncate, and what that takes off may be half of the output's rounding, eps / 4, in the
+    mean; the rounding itself is at most eps / 2 of each value."""
+    n, k, g = 2048, 1664, gen(1)
+    dy, x = (torch.empty(m, c, dtype=dtype, device="cuda") for c in (n, k))
+    for i in range(0, m, 2 ** 16):
+        dy[i:i + 2 ** 16] = torch.rand(2 ** 16, n, generator=g, device="cuda") / 16
+        x[i:i + 2 ** 16] = torch.rand(2 ** 16, k, generator=g, device="cuda") / 64
+    _, dw, db = api().linear_backward(dy, x, torch.empty(n, k, dtype=dtype, device="cuda"), with_dx=False, with_bias=True)
+    want = sum(a.double().T @ b.double() for a, b in zip(dy[:, :128].split(2 ** 16), x[:, -128:].split(2 ** 16)))
+    eps = torch.finfo(dtype).eps
+    off = dw[:128, -128:].double() / want - 1
+    assert off.mean().abs() <= eps / 4 and off.abs().max() <= eps / 4 + eps / 2
+    assert (db[:128].double() / sum(a.double().sum(0) for a in dy[:, :128].split(2 ** 16)) - 1).abs().max() <= eps / 2 + 2.0 ** -14
