@@ -40,7 +40,8 @@ typedef struct {
  * finite); -inf (and all below -120) empties the state.
  * Forward:  q, k, v, g, beta, initial_state (NULL: zeros) -> o, final_state (NULL: not stored).
  * Backward: also d_o and dfinal_state (NULL: zeros) -> dq, dk_, dv_, dg, dbeta (dense, shaped like
- * q, k, v, g, beta) and dinitial_state (NULL: not stored).  States are dense fp32
+ * q, k, v, g, beta) and dinitial_state (NULL: not stored); dg is good to about 1e-6 of the sums of o do and
+ * v dv over a chunk, which it is the difference of.  States are dense fp32
  * (nseq, hv, dk, dv); final_state may be initial_state.  A value that is not finite (a
  * state, u or an fp32 input above 3.38e38 counts as one) may spoil every output of its sequence from the start
  * of its 64-token chunk, and every gradient of its sequence. */

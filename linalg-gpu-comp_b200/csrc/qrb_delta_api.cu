@@ -86,16 +86,17 @@ int check_args(const qrb_delta_args* a) {
 }
 
 // Segments of `seg` chunks (0: whole sequences) and how many there may be at most.  With one chunk of the
-// full recurrence as the unit (5.5 us at dk = dv = 128 in bf16), one of the state-only pass takes about
+// full recurrence as the unit (5.6 us at dk = dv = 128 in bf16), one of the state-only pass takes about
 // as much (0.6 in fp32), a join's step 1/4 and the two launches 3.5: a sequence of nc chunks costs
 // 2 seg + ns / 4 + 3.5 in ns segments, which is least at seg = sqrt(nc / 8) where there are SMs for so
-// many.  One sequence, 16 heads of 128 x 128, bf16: 512 tokens 57 us whole, 65 in four; 1024 tokens 99
-// and 79; 4096 tokens 373 and 234; backward, whose chunks take longer, 512 tokens 171 us whole, 122 in
-// four, 4096 tokens 1320 and 638.  The state-only pass has one more block per head, for the transition.
+// many.  One sequence, 16 heads of 128 x 128, bf16, as called: 512 tokens 63 us whole, 67 in four (captured
+// 60 and 59); 1024 tokens 105 and 88; 4096 tokens 379 and 245; backward, whose chunks take longer, 512 tokens
+// 189 us whole, 139 in four, 4096 tokens 1204 and 552.  The state-only pass has one more block per head, for
+// the transition.
 // Packed lengths are not known on the host: segments are cut as if one sequence held most of the tokens,
 // which costs little where it does not (a sequence of one segment has no first pass), unless the
-// sequences alone nearly fill the card.  7 packed sequences, 6 heads of 64 x 64, 3001 tokens, backward:
-// 605 us whole, 190 cut.
+// sequences alone nearly fill the card.  7 packed sequences, 6 heads of 64 x 64, 3001 tokens, fp16, backward:
+// 610 us whole, 181 cut.
 struct Segments {
   int seg, nsegs;
 };
@@ -106,7 +107,10 @@ Segments segments(const qrb_delta_args& a, bool backward) {
   Segments s{0, 0};
   // Two segments need no transition, so they may have room where more have not; then the first pass is
   // half a sequence's, which pays where it is clearly cheaper than the second: 4 x 2048 tokens, 16 heads
-  // of 128 x 128, backward in bf16 970 us whole, 845 in halves, forward in fp32 611 and 564.
+  // of 128 x 128, backward in bf16 792 us whole, 673 in halves, forward in fp32 615 and 568, but in bf16 258
+  // and 279.  (Where there is room for exactly two with their transition, `room` = 2 nseq, the test of cost at
+  // the end is never met, so 25 to 37 heads and sequences run whole at any length: forward in bf16 that is
+  // right, 8192 tokens of 32 heads 809 us whole and 832 in halves, backward it is not, 2564 and 1901.)
   const bool halves = !packed && room < 2 * a.nseq && (backward || a.dtype == QRB_F32) &&
                       qrb::sm_count() / (a.hv * nb) >= 2 * a.nseq;
   if (a.nseq < 1 || (packed ? 2 * room < 3 * a.nseq : room < 2 * a.nseq && !halves)) return s;

@@ -13,7 +13,7 @@
 // cores' queue is full, which in a computing warp made every other one wait for it) and another loads
 // the chunk tiles by bulk copies, two chunks in flight where they fit (issuing those takes 800 cycles a
 // chunk).  An N = 64 MMA takes 47 cycles by itself, 60 to 120 while the warps use tensor memory.
-// Measured (dk = dv = 128): 5.6 us a chunk in bf16, 24 packed sequences of 16384 tokens with 32 heads 327 us
+// Measured (dk = dv = 128): 5.6 us a chunk in bf16, 24 packed sequences of 16384 tokens with 32 heads 332 us
 // (58 chunks an SM); 7.8 us where it stores for a backward pass, which moves 240 KB a chunk.
 #include "qrb_delta_tc.cuh"
 #include "qrb_ring.cuh"

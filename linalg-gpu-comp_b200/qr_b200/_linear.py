@@ -55,6 +55,8 @@ def linear_backward(dy, x, w, *, activation="none", pre=None, with_bias=False, w
     """``(dx, dw, dbias)`` of ``linear`` for the gradient dy of its result; those not asked for are None.
 
     ``pre`` is what ``linear(..., return_pre=True)`` returned (needed with an activation only).  The gradient
-    of the residual is dy itself.  Can be captured into a CUDA graph.
+    of the residual is dy itself.  With 16-bit types dp = dy act'(pre) is rounded to the type before its two
+    products, which is as much again as rounding dx and dw (in bf16 2.3e-3 of error in place of 1.7e-3); dbias
+    is summed before that, in fp32.  Records no gradients of its own.  Can be captured into a CUDA graph.
     """
     return _fast().linear_backward(dy, x, w, activation, pre, with_dx, with_dw, with_bias)

@@ -92,7 +92,10 @@ def gated_delta_rule_backward(do, q, k, v, g, beta, *, scale=None, initial_state
 
     The other arguments are those of ``gated_delta_rule``; dinitial_state is None without an initial state.
     The forward recurrence is run again, so nothing has to be kept between the passes.  q/k heads that
-    several value heads share get the sum of their gradients, added in head order: results repeat.  Can be
+    several value heads share get the sum of their gradients, added in head order: results repeat.  dg is the
+    difference of sums of o do and v dv over up to 64 tokens and is good to about 1e-6 of those: where a gate is
+    nearly closed, its true value (which goes to 0) may be smaller.  A value that is not finite may spoil every
+    gradient of its sequence.  Records no gradients of its own.  Can be
     captured into a CUDA graph.
     """
     return _fast().delta_backward(do, q, k, v, g, beta, scale, initial_state, seq_offsets, dfinal_state)
