@@ -40,11 +40,12 @@ typedef struct {
  * finite); -inf (and all below -120) empties the state.
  * Forward:  q, k, v, g, beta, initial_state (NULL: zeros) -> o, final_state (NULL: not stored).
  * Backward: also d_o and dfinal_state (NULL: zeros) -> dq, dk_, dv_, dg, dbeta (dense, shaped like
- * q, k, v, g, beta) and dinitial_state (NULL: not stored); dg is good to about 1e-6 of the sums of o do and
- * v dv over a chunk, which it is the difference of.  States are dense fp32
- * (nseq, hv, dk, dv); final_state may be initial_state.  A value that is not finite (a
- * state, u or an fp32 input above 3.38e38 counts as one) may spoil every output of its sequence from the start
- * of its 64-token chunk, and every gradient of its sequence. */
+ * q, k, v, g, beta) and dinitial_state (NULL: not stored); dg is good to about 1e-6 of the sums of
+ * o do and v dv over a chunk, which it is the difference of.  States are dense fp32 (nseq, hv, dk, dv);
+ * final_state may be initial_state.  Else no output may overlap a state, seq_offsets or another
+ * output, and no gradient an input.  A value that is not finite (a state, u or an fp32 input above
+ * 3.38e38 counts as one) may spoil every output of its sequence from the start of its 64-token chunk,
+ * and every gradient of its sequence. */
 typedef struct {
   int dtype;                       /* qrb_dtype of q, k, v, o and their gradients */
   int hk, hv, dk, dv;
@@ -76,7 +77,8 @@ QRB_API int qrb_delta_backward(const qrb_delta_args* a, void* workspace, size_t 
  * (num_slots x hv x dk x dv, fp32, the last three dense, slot_stride elements apart), writes the
  * advanced state to the same slot of state_out (which may be `state`) and o.  A row whose slot is
  * negative is padding: its o is 0 and no state is touched.  A row whose slot is num_slots or more,
- * or is held by an earlier row, gets o = NaN and no state is touched.  No workspace. */
+ * or is held by an earlier row, gets o = NaN and no state is touched.  o may be v; else neither output may overlap
+ * an input or the other.  No workspace. */
 typedef struct {
   int dtype;
   int hk, hv, dk, dv;
