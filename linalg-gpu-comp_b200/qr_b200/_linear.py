@@ -37,8 +37,9 @@ def linear(x, w, bias=None, *, activation="none", residual=None, return_pre=Fals
     type; ``activation`` is "none", "relu", "silu" or "gelu" (the exact, erf form).
 
     ``return_pre`` also returns ``x w^T + bias`` rounded to the type, which ``linear_backward`` needs for an
-    activation.  ``out`` takes the result; it may be ``residual`` itself, and overlap no input otherwise.  Any strides: rows that are not
-    dense are copied, and rows that are not 16-byte aligned are laid out in scratch memory first.
+    activation.  ``out`` takes the result; it may be ``residual`` itself, and overlap no input otherwise.  Any
+    strides: rows that are not dense are copied, and rows that are not 16-byte aligned are laid out in scratch
+    memory first.
     Differentiable with respect to x, w, bias and residual, once; forward-mode tangents are refused
     (NotImplementedError).
     """

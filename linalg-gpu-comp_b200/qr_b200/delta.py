@@ -74,8 +74,8 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, seq_of
     nor ``seq_offsets`` or one another.
 
     Differentiable with respect to q, k, v, g, beta and initial_state (autograd calls
-    ``gated_delta_rule_backward``, once); forward-mode tangents are refused (NotImplementedError).  A value that is not finite may spoil its sequence from the start of
-    its 64-token chunk on.
+    ``gated_delta_rule_backward``), once; forward-mode tangents are refused (NotImplementedError).  A value that
+    is not finite may spoil its sequence from the start of its 64-token chunk on.
     """
     if out is not None and _wants_grad(q, k, v, g, beta, initial_state, *out):
         raise ValueError("out is not supported where it or an input requires gradients")
@@ -95,8 +95,7 @@ def gated_delta_rule_backward(do, q, k, v, g, beta, *, scale=None, initial_state
     several value heads share get the sum of their gradients, added in head order: results repeat.  dg is the
     difference of sums of o do and v dv over up to 64 tokens and is good to about 1e-6 of those: where a gate is
     nearly closed, its true value (which goes to 0) may be smaller.  A value that is not finite may spoil every
-    gradient of its sequence.  Records no gradients of its own.  Can be
-    captured into a CUDA graph.
+    gradient of its sequence.  Records no gradients of its own.  Can be captured into a CUDA graph.
     """
     return _fast().delta_backward(do, q, k, v, g, beta, scale, initial_state, seq_offsets, dfinal_state)
 
@@ -107,8 +106,8 @@ def gated_delta_step(q, k, v, g, beta, state, *, scale=None, slots=None, state_o
 
     Row i advances state ``slots[i]`` (int32 on the device; default i) in place, or from ``state`` into the
     same slot of ``state_out``, which may be another pool (other slots of it are left as they are) but must
-    not overlap ``state`` otherwise.  ``out`` takes o; neither may overlap an input, but out may be ``v``
-    itself.  A negative slot marks a padding row: its o is 0.  A slot outside the
-    pool, or one that an earlier row holds, is refused: that row's o is NaN and it changes no state.
+    not overlap ``state`` otherwise.  ``out`` takes o.  Neither may overlap an input, but out may be ``v``.
+    A negative slot marks a padding row: its o is 0.  A slot outside the pool, or one that an earlier row holds,
+    is refused: that row's o is NaN and it changes no state.
     """
     return _fast().delta_step(q, k, v, g, beta, state, scale, slots, state_out, out)
